@@ -33,6 +33,8 @@ STATUS_BITS = {
     1 << 3: "the tensor-core completion barrier ran out of time",
     1 << 4: "the sequence-split exchange found a record of another step (the ranks' calls do not line up)",
     1 << 5: "a sequence length or row led outside the page table",
+    1 << 6: "an infinity or a not-a-number was stored to a 4-bit pool",
+    1 << 7: "the stack of free pages was too short",
     1 << 8: "(in the KV-streaming kernel)",
     1 << 9: "(in the projection's load pipeline)",
     1 << 10: "(in the projection's tensor-core pipeline)",
@@ -114,6 +116,85 @@ class NoAllocArgs(C.Structure):
     ]
 
 
+class Kv4PoolDesc(C.Structure):
+    _fields_ = [
+        ("k_codes", C.c_void_p),
+        ("k_scales", C.c_void_p),
+        ("v_codes", C.c_void_p),
+        ("v_scales", C.c_void_p),
+        ("n_slots", C.c_int64),
+        ("nh_kv", C.c_int),
+        ("page_size", C.c_int),
+        ("k_scale", C.c_float),
+        ("v_scale", C.c_float),
+        ("resolved", C.c_int),
+    ]
+
+
+class DecodeKv4Args(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int),
+        ("n_q", C.c_int),
+        ("nh_q", C.c_int),
+        ("q", C.c_void_p),
+        ("q_stride", C.c_int64),
+        ("out", C.c_void_p),
+        ("out_stride", C.c_int64),
+        ("seq_lens", C.c_void_p),
+        ("page_table", C.c_void_p),
+        ("pt_stride", C.c_int64),
+        ("pt_rows", C.c_int),
+        ("max_pages", C.c_int),
+        ("row_map", C.c_void_p),
+        ("softmax_scale", C.c_float),
+        ("lse_out", C.c_void_p),
+    ]
+
+
+class QkNormArgs(C.Structure):
+    _fields_ = [
+        ("n_tokens", C.c_int64),
+        ("nh_q", C.c_int),
+        ("nh_k", C.c_int),
+        ("q", C.c_void_p),
+        ("q_stride", C.c_int64),
+        ("k", C.c_void_p),
+        ("k_stride", C.c_int64),
+        ("q_out", C.c_void_p),
+        ("q_out_stride", C.c_int64),
+        ("k_out", C.c_void_p),
+        ("k_out_stride", C.c_int64),
+        ("q_weight", C.c_void_p),
+        ("k_weight", C.c_void_p),
+        ("q_weight_f32", C.c_int),
+        ("k_weight_f32", C.c_int),
+        ("q_weight_per_head", C.c_int),
+        ("k_weight_per_head", C.c_int),
+        ("positions", C.c_void_p),
+        ("positions_int64", C.c_int),
+        ("cos_sin", C.c_void_p),
+        ("max_pos", C.c_int),
+        ("eps", C.c_float),
+    ]
+
+
+class PagesArgs(C.Structure):
+    _fields_ = [
+        ("page_table", C.c_void_p),
+        ("pt_stride", C.c_int64),
+        ("pt_rows", C.c_int),
+        ("max_pages", C.c_int),
+        ("rows", C.c_void_p),
+        ("lens", C.c_void_p),
+        ("more", C.c_void_p),
+        ("batch", C.c_int),
+        ("page_size", C.c_int),
+        ("free_pages", C.c_void_p),
+        ("free_cap", C.c_int),
+        ("n_free", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); also the list of symbols include/directkv_b200.h declares.
 SIGNATURES = {
     "dkv_version": (C.c_int, []),
@@ -149,6 +230,14 @@ SIGNATURES = {
     "dkv_scatter_kv": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p,
                                  C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     "dkv_decode_noalloc": (C.c_int, [C.POINTER(NoAllocArgs), C.c_void_p]),
+    "dkv_kv4_pool_resolve": (C.c_int, [C.c_void_p, C.POINTER(Kv4PoolDesc)]),
+    "dkv_kv4_store": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64,
+                                C.c_void_p]),
+    "dkv_kv4_load": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "dkv_decode_kv4": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "dkv_qk_norm_rope": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "dkv_assign_pages": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "dkv_release_pages": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "dkv_stream_copy": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
 }
 

@@ -21,6 +21,10 @@
 #include "dkv_extend_pp.cuh"
 #include "dkv_extend.cuh"
 #include "dkv_proj.cuh"
+#include "dkv_kv4.cuh"
+#include "dkv_kv4_attn.cuh"
+#include "dkv_qk_norm.cuh"
+#include "dkv_pages.cuh"
 
 namespace {
 
@@ -128,6 +132,7 @@ struct LayerState {
 };
 
 constexpr int kMaxCounters = 4096;
+constexpr int kOpCounters = 64;           // behind them: tickets of the operators' kernels, zero between launches
 
 }  // namespace
 
@@ -863,8 +868,8 @@ int dkv_context_create(int device, dkv_context** out) {
     ctx->sm_count = prop.multiProcessorCount;
     cudaError_t e = cudaMalloc(&ctx->status, sizeof(unsigned int));
     if (e == cudaSuccess) e = cudaMemset(ctx->status, 0, sizeof(unsigned int));
-    if (e == cudaSuccess) e = cudaMalloc(&ctx->counters, kMaxCounters * sizeof(unsigned int));
-    if (e == cudaSuccess) e = cudaMemset(ctx->counters, 0, kMaxCounters * sizeof(unsigned int));
+    if (e == cudaSuccess) e = cudaMalloc(&ctx->counters, (kMaxCounters + kOpCounters) * sizeof(unsigned int));
+    if (e == cudaSuccess) e = cudaMemset(ctx->counters, 0, (kMaxCounters + kOpCounters) * sizeof(unsigned int));
     if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&ctx->side, cudaStreamNonBlocking);
     if (e == cudaSuccess) e = cudaEventCreateWithFlags(&ctx->ev_fork, cudaEventDisableTiming);
     if (e == cudaSuccess) e = cudaEventCreateWithFlags(&ctx->ev_join, cudaEventDisableTiming);
@@ -1022,7 +1027,7 @@ int dkv_read_status(dkv_context* ctx, unsigned int* status, int clear) {
     DKV_CUDA(cudaMemcpy(status, ctx->status, sizeof(unsigned int), cudaMemcpyDeviceToHost));
     if (clear && *status != 0) {
         DKV_CUDA(cudaMemset(ctx->status, 0, sizeof(unsigned int)));
-        DKV_CUDA(cudaMemset(ctx->counters, 0, kMaxCounters * sizeof(unsigned int)));
+        DKV_CUDA(cudaMemset(ctx->counters, 0, (kMaxCounters + kOpCounters) * sizeof(unsigned int)));
     }
     return DKV_OK;
 }
@@ -1911,3 +1916,5 @@ int dkv_stream_copy(dkv_context* ctx, void* dst, const void* src, int64_t bytes,
 }
 
 }  // extern "C"
+
+#include "dkv_ops_capi.cuh"

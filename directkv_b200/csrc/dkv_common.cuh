@@ -21,6 +21,8 @@ enum StatusBits : unsigned int {
     kStatusTmemTimeout   = 1u << 3,   // the MMA-completion barrier ran out of time
     kStatusExchangeOrder = 1u << 4,   // sequence-split exchange: a record of another step was found
     kStatusBadPage       = 1u << 5,   // a page-table index lay outside the table
+    kStatusNonFinite     = 1u << 6,   // an infinity or a not-a-number was stored to a 4-bit pool
+    kStatusOutOfPages    = 1u << 7,   // the stack of free pages was too short
     // Which kernel gave up waiting (set together with kStatusWaitTimeout / kStatusTmemTimeout).
     kStatusInStreaming   = 1u << 8,   // KV-streaming kernel: a tile's copy did not arrive
     kStatusInProjLoad    = 1u << 9,   // projection: the producer found no free stage

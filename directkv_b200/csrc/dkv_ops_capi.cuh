@@ -1,0 +1,258 @@
+// C entry points of the operators around a 4-bit paged cache: store, load and attention, head norms with rotation,
+// page tables.  Part of dkv_capi.cu (it uses that file's context and error helpers).
+#pragma once
+
+namespace {
+
+// Makes the context's device current for the launches of one call and puts the caller's back.
+struct DeviceScope {
+    int before = -1;
+    cudaError_t err;
+    explicit DeviceScope(int device) {
+        err = cudaGetDevice(&before);
+        if (err == cudaSuccess && before != device) err = cudaSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+#define DKV_ON_DEVICE(ctx)              \
+    DeviceScope device_scope((ctx)->device); \
+    DKV_CUDA(device_scope.err)
+
+bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+int log2_of(int v) {
+    int s = 0;
+    while ((1 << s) < v) ++s;
+    return s;
+}
+
+int check_kv4_pool(const dkv_context* ctx, const dkv_kv4_pool* pool) {
+    DKV_REQUIRE(pool->resolved == ctx->device + 1, "the 4-bit pool was not resolved for device %d (dkv_kv4_pool_resolve)", ctx->device);
+    return DKV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dkv_kv4_pool_resolve(dkv_context* ctx, dkv_kv4_pool* pool) {
+    DKV_REQUIRE(ctx != nullptr && pool != nullptr, "ctx / pool is NULL");
+    DKV_REQUIRE(pool->k_codes && pool->k_scales && pool->v_codes && pool->v_scales, "codes and scales must not be NULL");
+    DKV_REQUIRE(pool->n_slots > 0 && pool->n_slots <= INT32_MAX && pool->nh_kv > 0 && pool->nh_kv <= 65535,
+                "n_slots must be 1..2^31-1 and nh_kv 1..65535");
+    DKV_REQUIRE(pool->page_size >= 1 && (pool->page_size & (pool->page_size - 1)) == 0, "page_size (%d) must be a power of two", pool->page_size);
+    for (float s : {pool->k_scale, pool->v_scale}) {
+        int e = 0;
+        DKV_REQUIRE(s > 0.f && frexpf(s, &e) == 0.5f && e >= -23 && e <= 25, "pool scales must be powers of two from 2^-24 to 2^24");
+    }
+    DKV_REQUIRE(aligned(pool->k_codes, 16) && aligned(pool->v_codes, 16) && aligned(pool->k_scales, 8) && aligned(pool->v_scales, 8),
+                "codes must be 16-byte and scales 8-byte aligned");
+    DKV_ON_DEVICE(ctx);
+    dkv_kv4_pool r = *pool;
+    void** parts[4] = {&r.k_codes, &r.k_scales, &r.v_codes, &r.v_scales};
+    for (void** p : parts) {
+        cudaPointerAttributes attr;
+        DKV_CUDA(cudaPointerGetAttributes(&attr, *p));
+        DKV_REQUIRE(attr.type != cudaMemoryTypeDevice || attr.device == ctx->device, "a part of the 4-bit pool lives on device %d, not on %d",
+                    attr.device, ctx->device);
+        int rc = device_pointer_of(*p, p, "a 4-bit pool");
+        if (rc != DKV_OK) return rc;
+    }
+    r.resolved = ctx->device + 1;
+    *pool = r;
+    return DKV_OK;
+}
+
+static int kv4_rows(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, int64_t n_tokens) {
+    DKV_REQUIRE(ctx != nullptr && pool != nullptr, "ctx / pool is NULL");
+    int rc = check_kv4_pool(ctx, pool);
+    if (rc != DKV_OK) return rc;
+    DKV_REQUIRE(n_tokens >= 0 && n_tokens * pool->nh_kv <= (static_cast<int64_t>(INT32_MAX) - 1) * 32, "bad number of tokens");
+    DKV_REQUIRE(n_tokens == 0 || slots != nullptr, "slots must not be NULL");
+    return DKV_OK;
+}
+
+int dkv_kv4_store(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, int slots_int64, const void* k, int64_t k_stride,
+                  const void* v, int64_t v_stride, int64_t n_tokens, void* stream) {
+    int rc = kv4_rows(ctx, pool, slots, n_tokens);
+    if (rc != DKV_OK || n_tokens == 0) return rc;
+    DKV_REQUIRE(k != nullptr && v != nullptr && aligned(k, 16) && aligned(v, 16), "k / v must be 16-byte aligned device pointers");
+    const int64_t row = static_cast<int64_t>(pool->nh_kv) * 128;
+    DKV_REQUIRE(k_stride >= row && v_stride >= row && k_stride % 8 == 0 && v_stride % 8 == 0, "k / v strides too small or unaligned");
+    DKV_ON_DEVICE(ctx);
+    Kv4StoreParams p{};
+    p.src[0] = static_cast<const __nv_bfloat16*>(k), p.src[1] = static_cast<const __nv_bfloat16*>(v);
+    p.src_stride[0] = k_stride, p.src_stride[1] = v_stride;
+    p.codes[0] = static_cast<uint8_t*>(pool->k_codes), p.codes[1] = static_cast<uint8_t*>(pool->v_codes);
+    p.scales[0] = static_cast<uint8_t*>(pool->k_scales), p.scales[1] = static_cast<uint8_t*>(pool->v_scales);
+    p.inv_scale[0] = 1.f / pool->k_scale, p.inv_scale[1] = 1.f / pool->v_scale;
+    p.slots = slots, p.slots64 = slots_int64;
+    p.n_rows = n_tokens * pool->nh_kv;
+    p.nh = pool->nh_kv;
+    p.n_slots = pool->n_slots;
+    p.status = ctx->status;
+    kv4_store_kernel<<<dim3(static_cast<unsigned>((p.n_rows + 31) / 32), 2), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    DKV_CUDA(cudaGetLastError());
+    ctx->launches += 1;
+    return DKV_OK;
+}
+
+int dkv_kv4_load(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, int slots_int64, void* k, void* v, int64_t n_tokens,
+                 void* stream) {
+    int rc = kv4_rows(ctx, pool, slots, n_tokens);
+    if (rc != DKV_OK || n_tokens == 0) return rc;
+    DKV_REQUIRE(k != nullptr && v != nullptr && aligned(k, 16) && aligned(v, 16), "k / v must be 16-byte aligned device pointers");
+    DKV_ON_DEVICE(ctx);
+    Kv4LoadParams p{};
+    p.codes[0] = static_cast<const uint8_t*>(pool->k_codes), p.codes[1] = static_cast<const uint8_t*>(pool->v_codes);
+    p.scales[0] = static_cast<const uint8_t*>(pool->k_scales), p.scales[1] = static_cast<const uint8_t*>(pool->v_scales);
+    p.scale[0] = pool->k_scale, p.scale[1] = pool->v_scale;
+    p.dst[0] = static_cast<__nv_bfloat16*>(k), p.dst[1] = static_cast<__nv_bfloat16*>(v);
+    p.slots = slots, p.slots64 = slots_int64;
+    p.n_rows = n_tokens * pool->nh_kv;
+    p.nh = pool->nh_kv;
+    p.n_slots = pool->n_slots;
+    p.status = ctx->status;
+    kv4_load_kernel<<<dim3(static_cast<unsigned>((p.n_rows + 31) / 32), 2), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    DKV_CUDA(cudaGetLastError());
+    ctx->launches += 1;
+    return DKV_OK;
+}
+
+int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_kv4_args* a, void* stream) {
+    DKV_REQUIRE(ctx != nullptr && pool != nullptr && a != nullptr, "ctx / pool / args is NULL");
+    int rc = check_kv4_pool(ctx, pool);
+    if (rc != DKV_OK) return rc;
+    if (a->batch == 0) return DKV_OK;
+    DKV_REQUIRE(a->batch > 0 && a->batch <= 4096, "batch (%d) must be 0..4096", a->batch);
+    DKV_REQUIRE(a->n_q >= 1 && a->n_q <= 1024, "query tokens per request (%d) must be 1..1024", a->n_q);
+    DKV_REQUIRE(a->nh_q > 0 && a->nh_q % pool->nh_kv == 0, "nh_q (%d) must be a multiple of nh_kv (%d)", a->nh_q, pool->nh_kv);
+    DKV_REQUIRE(a->q && a->out && a->seq_lens && a->page_table, "q / out / seq_lens / page_table must not be NULL");
+    const int64_t row = static_cast<int64_t>(a->nh_q) * 128;
+    DKV_REQUIRE(a->q_stride >= row && a->q_stride % 8 == 0 && aligned(a->q, 16), "q must be 16-byte aligned with a token stride that is a multiple of 8");
+    DKV_REQUIRE(a->out_stride >= row && a->out_stride % 8 == 0 && aligned(a->out, 16),
+                "out must be 16-byte aligned with a token stride that is a multiple of 8");
+    DKV_REQUIRE(a->max_pages >= 0 && a->pt_stride >= 0 && a->pt_rows >= 0, "bad page table sizes");
+    DKV_REQUIRE(a->softmax_scale == a->softmax_scale, "softmax_scale is not a number");
+    DKV_ON_DEVICE(ctx);
+    Kv4AttnParams p{};
+    p.q = static_cast<const __nv_bfloat16*>(a->q);
+    p.q_stride = a->q_stride;
+    p.out = static_cast<__nv_bfloat16*>(a->out);
+    p.out_stride = a->out_stride;
+    p.lse = a->lse_out;
+    p.seq_lens = a->seq_lens;
+    p.page_table = a->page_table;
+    p.pt_stride = a->pt_stride;
+    p.pt_rows = a->pt_rows;
+    p.page_shift = log2_of(pool->page_size);
+    p.max_pages = std::min(a->max_pages, INT32_MAX >> p.page_shift);
+    p.row_map = a->row_map;
+    p.k_codes = static_cast<const uint8_t*>(pool->k_codes), p.v_codes = static_cast<const uint8_t*>(pool->v_codes);
+    p.k_scales = static_cast<const uint8_t*>(pool->k_scales), p.v_scales = static_cast<const uint8_t*>(pool->v_scales);
+    p.n_slots = pool->n_slots;
+    p.batch = a->batch, p.n_q = a->n_q, p.nh_q = a->nh_q, p.nh_kv = pool->nh_kv;
+    p.scale_log2 = a->softmax_scale * pool->k_scale * 1.4426950408889634f;
+    p.v_scale = pool->v_scale;
+    p.status = ctx->status;
+    kv4_attn_kernel<<<dim3(a->nh_q, a->n_q, a->batch), 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    DKV_CUDA(cudaGetLastError());
+    ctx->launches += 1;
+    return DKV_OK;
+}
+
+int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* a, void* stream) {
+    DKV_REQUIRE(ctx != nullptr && a != nullptr, "ctx / args is NULL");
+    DKV_REQUIRE(a->n_tokens >= 0 && a->nh_q >= 0 && a->nh_k >= 0 && a->nh_q <= 65535 && a->nh_k <= 65535, "bad sizes");
+    if (a->n_tokens == 0 || a->nh_q + a->nh_k == 0) return DKV_OK;
+    const int64_t rows = a->n_tokens * (a->nh_q + a->nh_k);
+    DKV_REQUIRE(rows <= (static_cast<int64_t>(INT32_MAX) - 1) * 16, "too many rows");
+    DKV_REQUIRE(a->cos_sin == nullptr || (a->positions != nullptr && a->max_pos > 0), "a rotation needs positions and a table");
+    DKV_REQUIRE(a->cos_sin == nullptr || aligned(a->cos_sin, 16), "cos_sin must be 16-byte aligned");
+    DKV_REQUIRE(a->eps >= 0.f, "eps must not be negative");
+    QkNormParams p{};
+    const void* x[2] = {a->q, a->k};
+    void* y[2] = {a->q_out, a->k_out};
+    const int64_t xs[2] = {a->q_stride, a->k_stride}, ys[2] = {a->q_out_stride, a->k_out_stride};
+    const int nh[2] = {a->nh_q, a->nh_k};
+    const void* w[2] = {a->q_weight, a->k_weight};
+    const int wf[2] = {a->q_weight_f32, a->k_weight_f32}, wp[2] = {a->q_weight_per_head, a->k_weight_per_head};
+    for (int i = 0; i < 2; ++i) {
+        p.heads[i] = nh[i];
+        if (nh[i] == 0) continue;
+        DKV_REQUIRE(x[i] != nullptr && y[i] != nullptr && aligned(x[i], 8) && aligned(y[i], 8), "q / k and their outputs must be 8-byte aligned device pointers");
+        DKV_REQUIRE(xs[i] >= static_cast<int64_t>(nh[i]) * 128 && xs[i] % 4 == 0 && ys[i] >= static_cast<int64_t>(nh[i]) * 128 && ys[i] % 4 == 0,
+                    "q / k token strides too small or not a multiple of 4");
+        DKV_REQUIRE(w[i] == nullptr || aligned(w[i], wf[i] ? 16 : 8), "norm weights must be 16-byte (fp32) or 8-byte (bf16) aligned");
+        p.x[i] = static_cast<const __nv_bfloat16*>(x[i]);
+        p.y[i] = static_cast<__nv_bfloat16*>(y[i]);
+        p.x_stride[i] = xs[i], p.y_stride[i] = ys[i];
+        p.weight[i] = w[i], p.weight_f32[i] = wf[i], p.weight_stride[i] = wp[i] ? 128 : 0;
+    }
+    p.positions = a->positions, p.pos64 = a->positions_int64;
+    p.cos_sin = a->cos_sin, p.max_pos = a->max_pos;
+    p.eps = a->eps;
+    p.n_tokens = a->n_tokens;
+    p.status = ctx->status;
+    DKV_ON_DEVICE(ctx);
+    qk_norm_rope_kernel<<<static_cast<unsigned>((rows + 15) / 16), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    DKV_CUDA(cudaGetLastError());
+    ctx->launches += 1;
+    return DKV_OK;
+}
+
+static int pages_common(dkv_context* ctx, const dkv_pages_args* a, PagesParams* p) {
+    DKV_REQUIRE(ctx != nullptr && a != nullptr, "ctx / args is NULL");
+    DKV_REQUIRE(a->batch >= 0 && a->batch <= kPagesMaxBatch, "batch (%d) must be 0..%d", a->batch, kPagesMaxBatch);
+    DKV_REQUIRE(a->page_size >= 1 && (a->page_size & (a->page_size - 1)) == 0, "page_size (%d) must be a power of two", a->page_size);
+    DKV_REQUIRE(a->page_table && a->free_pages && a->n_free && (a->batch == 0 || (a->lens && a->more)), "NULL argument");
+    DKV_REQUIRE(a->pt_rows >= 0 && a->max_pages >= 0 && a->pt_stride >= 0 && a->free_cap >= 0, "bad sizes");
+    p->page_table = a->page_table;
+    p->pt_stride = a->pt_stride;
+    p->pt_rows = a->pt_rows;
+    p->page_shift = log2_of(a->page_size);
+    p->max_pages = std::min(a->max_pages, INT32_MAX >> p->page_shift);
+    p->rows = a->rows, p->lens = a->lens, p->more = a->more;
+    p->batch = a->batch;
+    p->free_pages = a->free_pages, p->free_cap = a->free_cap, p->n_free = a->n_free;
+    p->status = ctx->status;
+    p->ticket = ctx->counters + kMaxCounters;
+    return DKV_OK;
+}
+
+int dkv_assign_pages(dkv_context* ctx, const dkv_pages_args* a, int32_t* slots, int32_t* positions, int64_t capacity, int32_t* seq_lens,
+                     int32_t* cu_new, void* stream) {
+    PagesParams p{};
+    int rc = pages_common(ctx, a, &p);
+    if (rc != DKV_OK) return rc;
+    DKV_REQUIRE(capacity >= 0 && capacity <= INT32_MAX && (capacity == 0 || slots != nullptr), "slots must hold 0..2^31-1 tokens");
+    DKV_REQUIRE(cu_new != nullptr && (a->batch == 0 || seq_lens != nullptr), "seq_lens / cu_new must not be NULL");
+    p.slots = slots, p.positions = positions, p.capacity = capacity, p.seq_lens = seq_lens, p.cu_new = cu_new;
+    DKV_ON_DEVICE(ctx);
+    const int64_t want = (capacity + kPagesThreads - 1) / kPagesThreads;
+    const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, ctx->sm_count * 2)));
+    pages_kernel<false><<<grid, kPagesThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    DKV_CUDA(cudaGetLastError());
+    ctx->launches += 1;
+    return DKV_OK;
+}
+
+int dkv_release_pages(dkv_context* ctx, const dkv_pages_args* a, void* stream) {
+    PagesParams p{};
+    int rc = pages_common(ctx, a, &p);
+    if (rc != DKV_OK || a->batch == 0) return rc;
+    DKV_ON_DEVICE(ctx);
+    const int64_t most = std::min<int64_t>(static_cast<int64_t>(a->batch) * p.max_pages, p.free_cap);
+    const int64_t want = (most + 4 * kPagesThreads - 1) / (4 * kPagesThreads);
+    const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, ctx->sm_count)));
+    pages_kernel<true><<<grid, kPagesThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    DKV_CUDA(cudaGetLastError());
+    ctx->launches += 1;
+    return DKV_OK;
+}
+
+}  // extern "C"

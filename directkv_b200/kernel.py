@@ -10,6 +10,7 @@ torch compute and no fallback.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Optional, Sequence
 
 import torch
@@ -370,6 +371,361 @@ def stream_copy(dst: torch.Tensor, src: torch.Tensor) -> None:
     _chk(dst.is_cuda and dst.numel() * dst.element_size() >= nbytes, "dst must be a CUDA tensor at least as large as src")
     ctx = get_context(dst.device.index)
     _lib.check(_lib.load().dkv_stream_copy(ctx.handle, _ptr(dst), _ptr(src), nbytes, _stream()))
+
+
+# ---------------------------------------------------------------------------
+# A paged cache held in 4 bits, and what a decode step over it needs beside the attention
+# ---------------------------------------------------------------------------
+KV4_BLOCK = 16          # consecutive dimensions that share a scale
+
+
+def _call(dev: int):
+    """Handle of the device's context and the raw handle of torch's current stream there."""
+    ctx = _lib._contexts.get(dev) or get_context(dev)
+    return ctx.handle, torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _on_device(dev: int, named) -> None:
+    for t, name in named:
+        if t is not None and (dev < 0 or t.get_device() != dev):
+            raise RuntimeError(f"{name} must be a CUDA tensor on the same device as the other tensors")
+
+
+def _int32_1d(t: torch.Tensor, n: int, name: str) -> None:
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.size(0) != n or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of {n} entries")
+
+
+def _heads_stride(t: torch.Tensor, name: str) -> int:
+    """Elements from token to token of ``[..., NH, 128]`` whose heads lie next to each other (a slice of a fused
+    projection's output is fine)."""
+    shape, st = t.shape, t.stride()
+    if t.dtype is not torch.bfloat16 or len(shape) < 3 or shape[-1] != HEAD_DIM or st[-1] != 1 or (st[-2] != HEAD_DIM and shape[-2] > 1):
+        raise RuntimeError(f"{name} must be bfloat16 [..., NH, {HEAD_DIM}] with the heads of a token next to each other")
+    row = shape[-2] * HEAD_DIM
+    if len(shape) == 3:
+        return st[0] if shape[0] > 1 else row
+    if len(shape) != 4 or (shape[0] > 1 and shape[1] > 1 and st[0] != shape[1] * st[1]):
+        raise RuntimeError(f"{name} must be 3D or 4D with evenly spaced tokens")
+    return st[1] if shape[1] > 1 else (st[0] if shape[0] > 1 else row)
+
+
+class KV4Pool:
+    """One layer's K and V pool in 4 bits (the format stands in include/directkv_b200.h at ``dkv_kv4_pool``).
+
+    ``k_codes`` / ``v_codes`` are uint8 ``[n_slots, NH_kv, 64]``, ``k_scales`` / ``v_scales`` uint8 ``[n_slots, NH_kv, 8]`` (e4m3
+    bytes), in device memory or page-locked host memory.  Token ``t`` of a request lies at slot
+    ``page_table[row, t // page_size] * page_size + t % page_size``.  ``k_scale`` / ``v_scale`` are powers of two that
+    the stored values are multiplied by; values above 2688 times the scale are cut off.
+    """
+
+    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "page_size", "k_scale", "v_scale", "n_slots", "nh_kv", "_descs")
+
+    def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
+                 page_size: int = 1, k_scale: float = 1.0, v_scale: float = 1.0):
+        _chk(k_codes.dim() == 3, "k_codes must be 3D [n_slots, NH_kv, 64]")
+        n_slots, nh = k_codes.size(0), k_codes.size(1)
+        for t, width, name in ((k_codes, HEAD_DIM // 2, "k_codes"), (v_codes, HEAD_DIM // 2, "v_codes"),
+                               (k_scales, HEAD_DIM // KV4_BLOCK, "k_scales"), (v_scales, HEAD_DIM // KV4_BLOCK, "v_scales")):
+            _chk(t.dtype == torch.uint8 and t.is_contiguous() and tuple(t.shape) == (n_slots, nh, width),
+                 f"{name} must be contiguous uint8 [{n_slots}, {nh}, {width}]")
+            _chk(t.device == k_codes.device, f"{name} must be on the device of k_codes")
+            _chk(t.is_cuda or t.is_pinned() or not torch.cuda.is_available(), f"{name} must be in pinned memory (or a CUDA tensor)")
+        _chk(page_size >= 1 and page_size & (page_size - 1) == 0, f"page_size ({page_size}) must be a power of two")
+        for s, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            _chk(2.0 ** -24 <= s <= 2.0 ** 24 and math.frexp(s)[0] == 0.5, f"{name} must be a power of two from 2^-24 to 2^24")
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
+        self.page_size, self.k_scale, self.v_scale = int(page_size), float(k_scale), float(v_scale)
+        self.n_slots, self.nh_kv = n_slots, nh
+        self._descs = {}
+
+    @classmethod
+    def empty(cls, n_slots: int, nh_kv: int, page_size: int = 1, device="cuda", k_scale: float = 1.0, v_scale: float = 1.0) -> "KV4Pool":
+        """A pool of zeros; ``device="cpu"`` puts it in page-locked host memory (beside the current GPU where the
+        machine has more than one memory node)."""
+        from .sglang_compat import pinned_zeros
+
+        def make(width):
+            if torch.device(device).type == "cpu":
+                return pinned_zeros((n_slots, nh_kv, width), torch.uint8)
+            return torch.zeros(n_slots, nh_kv, width, dtype=torch.uint8, device=device)
+
+        c, s = HEAD_DIM // 2, HEAD_DIM // KV4_BLOCK
+        return cls(make(c), make(s), make(c), make(s), page_size, k_scale, v_scale)
+
+    def nbytes(self) -> int:
+        return 2 * self.n_slots * self.nh_kv * (HEAD_DIM // 2 + HEAD_DIM // KV4_BLOCK)
+
+    def _ref(self, dev: int, handle):
+        """The C struct for one device, checked and resolved by the library on first use."""
+        ref = self._descs.get(dev)
+        if ref is None:
+            if self.k_codes.is_cuda and self.k_codes.get_device() != dev:
+                raise RuntimeError("the pool must be on the device of the other tensors")
+            d = _lib.Kv4PoolDesc(_ptr(self.k_codes), _ptr(self.k_scales), _ptr(self.v_codes), _ptr(self.v_scales), self.n_slots,
+                                 self.nh_kv, self.page_size, self.k_scale, self.v_scale, 0)
+            _lib.check(_lib.load().dkv_kv4_pool_resolve(handle, C.byref(d)))
+            ref = self._descs[dev] = C.byref(d)
+        return ref
+
+
+def _check_slots(slots: torch.Tensor) -> int:
+    if slots.dtype not in (torch.int32, torch.int64) or slots.dim() != 1 or not slots.is_contiguous():
+        raise RuntimeError("slots must be a contiguous 1D int32 or int64 tensor")
+    return slots.size(0)
+
+
+def store_kv4(pool: KV4Pool, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    """Quantises row ``i`` of ``k`` / ``v`` ``[n, NH_kv, 128]`` (bf16, tokens may be strided) into slot ``slots[i]``.
+
+    Slots outside the pool are not written and reported in the status word, and so are infinities (stored as the largest
+    value) and not-a-numbers (stored as zero).  Slots must be distinct, save for a padding slot that nobody attends.
+    """
+    n = _check_slots(slots)
+    if k.dim() != 3 or v.dim() != 3 or k.size(0) != n or v.size(0) != n or k.size(1) != pool.nh_kv or v.size(1) != pool.nh_kv:
+        raise RuntimeError(f"k and v must be [{n}, {pool.nh_kv}, {HEAD_DIM}]")
+    ks, vs = _heads_stride(k, "k"), _heads_stride(v, "v")
+    dev = k.get_device()
+    _on_device(dev, ((k, "k"), (v, "v"), (slots, "slots")))
+    if n == 0:
+        return
+    handle, stream = _call(dev)
+    rc = _lib.load().dkv_kv4_store(handle, pool._ref(dev, handle), slots.data_ptr(), slots.dtype is torch.int64, k.data_ptr(), ks,
+                                   v.data_ptr(), vs, n, stream)
+    if rc:
+        _lib.check(rc)
+
+
+def load_kv4(pool: KV4Pool, slots: torch.Tensor, k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None):
+    """The values of ``slots`` as bf16 ``(k, v)``, each ``[n, NH_kv, 128]``; exact.  A slot outside the pool gives zeros and
+    is reported in the status word."""
+    n = _check_slots(slots)
+    dev = slots.get_device()
+    _on_device(dev, ((slots, "slots"),))
+    shape = (n, pool.nh_kv, HEAD_DIM)
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
+    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
+        if t.dtype is not torch.bfloat16 or t.shape != shape or not t.is_contiguous():
+            raise RuntimeError(f"{name} must be contiguous bfloat16 [{n}, {pool.nh_kv}, {HEAD_DIM}]")
+    _on_device(dev, ((k_out, "k_out"), (v_out, "v_out")))
+    if n:
+        handle, stream = _call(dev)
+        rc = _lib.load().dkv_kv4_load(handle, pool._ref(dev, handle), slots.data_ptr(), slots.dtype is torch.int64, k_out.data_ptr(),
+                                      v_out.data_ptr(), n, stream)
+        if rc:
+            _lib.check(rc)
+    return k_out, v_out
+
+
+def decode_kv4(
+    q: torch.Tensor,                  # [B, NH_q, 128], [B, n_q, NH_q, 128] or [B, NH_q*128] bf16 CUDA (tokens may be strided)
+    pool: KV4Pool,
+    seq_lens: torch.Tensor,           # [B] int32 CUDA: stored tokens, the query tokens' own included
+    softmax_scale: float,
+    page_table: torch.Tensor,         # [rows, max_pages] int32 CUDA
+    row_map: Optional[torch.Tensor] = None,   # [B] int32 CUDA
+    out: Optional[torch.Tensor] = None,
+    lse_out: Optional[torch.Tensor] = None,   # [B, NH_q] or [B, n_q, NH_q] fp32
+) -> torch.Tensor:
+    """Decode attention over a 4-bit pool whose tokens are all stored (``store_kv4``).  Returns O with q's shape.
+
+    With ``n_q`` query tokens per request, token ``j`` attends the first ``seq_lens - n_q + 1 + j`` stored tokens (drafted
+    tokens under verification, a short chunk of a prompt).  A row that attends nothing is zero, its LSE -inf.
+    """
+    flat = q.dim() == 2
+    if flat and (q.size(1) % HEAD_DIM or q.size(1) == 0):
+        raise RuntimeError(f"q must be [B, NH_q*{HEAD_DIM}]")
+    q3 = q.view(q.size(0), -1, HEAD_DIM) if flat else q
+    qs = _heads_stride(q3, "q")
+    b, nh_q = q3.size(0), q3.size(-2)
+    n_q = q3.size(1) if q3.dim() == 4 else 1
+    if nh_q == 0 or nh_q % pool.nh_kv:
+        raise RuntimeError(f"q has {nh_q} heads, not a multiple of the pool's {pool.nh_kv}")
+    if b > 4096 or not 1 <= n_q <= 1024:
+        raise RuntimeError(f"{b} requests of {n_q} query tokens: at most 4096 of 1 to 1024")
+    _int32_1d(seq_lens, b, "seq_lens")
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 and page_table.size(1) > 1:
+        raise RuntimeError("page_table must be 2D int32 with unit inner stride")
+    if row_map is not None:
+        _int32_1d(row_map, b, "row_map")
+    elif page_table.size(0) < b:
+        raise RuntimeError(f"page_table has {page_table.size(0)} rows for {b} requests")
+    if lse_out is not None and (lse_out.dtype is not torch.float32 or lse_out.numel() != b * n_q * nh_q or not lse_out.is_contiguous()):
+        raise RuntimeError("lse_out must be contiguous fp32 with one entry per query row")
+    dev = q.get_device()
+    _on_device(dev, ((q, "q"), (seq_lens, "seq_lens"), (page_table, "page_table"), (row_map, "row_map"), (lse_out, "lse_out")))
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        os = nh_q * HEAD_DIM
+    else:
+        if out.shape != q.shape or out.get_device() != dev:
+            raise RuntimeError("out must have q's shape and device")
+        os = _heads_stride(out.view(b, -1, HEAD_DIM) if flat else out, "out")
+    if b == 0:
+        return out
+    handle, stream = _call(dev)
+    a = _lib.DecodeKv4Args(b, n_q, nh_q, q.data_ptr(), qs, out.data_ptr(), os, seq_lens.data_ptr(), page_table.data_ptr(),
+                           page_table.stride(0), page_table.size(0), page_table.size(1), _ptr(row_map), softmax_scale, _ptr(lse_out))
+    rc = _lib.load().dkv_decode_kv4(handle, pool._ref(dev, handle), C.byref(a), stream)
+    if rc:
+        _lib.check(rc)
+    return out
+
+
+def qk_norm_rope(
+    q: Optional[torch.Tensor],        # [T, NH_q, 128] bf16 CUDA (tokens may be strided: a slice of a fused projection)
+    k: Optional[torch.Tensor],        # [T, NH_kv, 128]
+    positions: Optional[torch.Tensor],     # [T] int32 or int64 CUDA
+    cos_sin: Optional[torch.Tensor],       # [max_pos, 128] fp32 CUDA = [cos | sin]; None: no rotation
+    q_weight: Optional[torch.Tensor] = None,   # [128] or [NH, 128], bf16 or fp32; None: no norm
+    k_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    q_out: Optional[torch.Tensor] = None,      # may be q itself (in place)
+    k_out: Optional[torch.Tensor] = None,
+):
+    """RMS norm of every query and key head and the Neox rotation at the tokens' positions, in one pass.
+
+    Returns ``(q_out, k_out)``; the norm of q or k is left out where it has no weight.  Computed in fp32 and rounded
+    once.  A position outside the table leaves its token unrotated and is reported in the status word.
+    """
+    lead = q if q is not None else k
+    if lead is None:
+        raise RuntimeError("q or k must be given")
+    n, dev = lead.size(0), lead.get_device()
+    args, keep = [], []
+    for x, y, w, name in ((q, q_out, q_weight, "q"), (k, k_out, k_weight, "k")):
+        if x is None:
+            keep.append(None)
+            args.append((0, None, 0, None, 0, None, 0, 0))
+            continue
+        if x.dim() != 3 or x.size(0) != n:
+            raise RuntimeError(f"{name} must be [{n}, NH, {HEAD_DIM}]")
+        xs, nh = _heads_stride(x, name), x.size(1)
+        if y is None:
+            y, ys = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device), nh * HEAD_DIM
+        else:
+            if y.shape != x.shape:
+                raise RuntimeError(f"{name}_out must have the shape of {name}")
+            ys = _heads_stride(y, f"{name}_out")
+        per_head = f32 = 0
+        if w is not None:
+            per_head, f32 = int(w.dim() == 2), int(w.dtype is torch.float32)
+            if (not f32 and w.dtype is not torch.bfloat16) or not w.is_contiguous() or w.size(-1) != HEAD_DIM or w.dim() > 2 or (per_head and w.size(0) != nh):
+                raise RuntimeError(f"{name}_weight must be contiguous bfloat16 or float32, [{HEAD_DIM}] or [{nh}, {HEAD_DIM}]")
+        _on_device(dev, ((x, name), (y, f"{name}_out"), (w, f"{name}_weight")))
+        keep.append(y)
+        args.append((nh, x.data_ptr(), xs, y.data_ptr(), ys, _ptr(w), f32, per_head))
+    max_pos = 0
+    if cos_sin is not None:
+        if cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or cos_sin.size(1) != HEAD_DIM or not cos_sin.is_contiguous() or cos_sin.size(0) == 0:
+            raise RuntimeError(f"cos_sin must be contiguous float32 [max_pos, {HEAD_DIM}]")
+        if positions is None or positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1 or positions.size(0) != n or not positions.is_contiguous():
+            raise RuntimeError(f"positions must be a contiguous int32 or int64 tensor of {n} entries")
+        _on_device(dev, ((cos_sin, "cos_sin"), (positions, "positions")))
+        max_pos = cos_sin.size(0)
+    if not eps >= 0.0:
+        raise RuntimeError("eps must not be negative")
+    if n == 0:
+        return tuple(keep)
+    (hq, qp, qs, qo, qos, qw, qf, qh), (hk, kp, ks, ko, kos, kw, kf, kh) = args
+    handle, stream = _call(dev)
+    a = _lib.QkNormArgs(n, hq, hk, qp, qs, kp, ks, qo, qos, ko, kos, qw, kw, qf, kf, qh, kh, _ptr(positions) if max_pos else None,
+                        bool(max_pos) and positions.dtype is torch.int64, _ptr(cos_sin), max_pos, eps)
+    rc = _lib.load().dkv_qk_norm_rope(handle, C.byref(a), stream)
+    if rc:
+        _lib.check(rc)
+    return tuple(keep)
+
+
+def _pages_args(page_table, lens, more, more_name, free_pages, n_free, page_size, rows):
+    b = lens.numel()
+    _int32_1d(lens, b, "lens")
+    _int32_1d(more, b, more_name)
+    if rows is not None:
+        _int32_1d(rows, b, "rows")
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 and page_table.size(1) > 1:
+        raise RuntimeError("page_table must be 2D int32 with unit inner stride")
+    if page_table.size(0) > 1 and page_table.stride(0) < page_table.size(1):
+        raise RuntimeError("the rows of page_table must not overlap")
+    if free_pages.dtype is not torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
+        raise RuntimeError("free_pages must be a contiguous 1D int32 tensor")
+    _int32_1d(n_free, 1, "n_free")
+    if b > 4096:
+        raise RuntimeError(f"{b} requests: at most 4096 per call")
+    if page_size < 1 or page_size & (page_size - 1):
+        raise RuntimeError(f"page_size ({page_size}) must be a power of two")
+    dev = page_table.get_device()
+    _on_device(dev, ((page_table, "page_table"), (lens, "lens"), (more, more_name), (free_pages, "free_pages"), (n_free, "n_free"), (rows, "rows")))
+    a = _lib.PagesArgs(page_table.data_ptr(), page_table.stride(0), page_table.size(0), page_table.size(1), _ptr(rows), lens.data_ptr(),
+                       more.data_ptr(), b, page_size, free_pages.data_ptr(), free_pages.size(0), n_free.data_ptr())
+    return dev, b, a
+
+
+def assign_pages(
+    page_table: torch.Tensor,         # [rows, max_pages] int32 CUDA, updated
+    lens: torch.Tensor,               # [B] int32 CUDA: tokens stored so far
+    new_lens: torch.Tensor,           # [B] int32 CUDA: tokens to come
+    free_pages: torch.Tensor,         # [N] int32 CUDA: a stack of page numbers, free_pages[:n_free] are free
+    n_free: torch.Tensor,             # [1] int32 CUDA, updated
+    page_size: int,
+    n_tokens: int,                    # room for the new tokens: their sum, or an upper bound of it
+    rows: Optional[torch.Tensor] = None,       # [B] int32 CUDA: row of the table of each request; None: row b
+    slots: Optional[torch.Tensor] = None,      # outputs (int32 CUDA), allocated where not given
+    positions: Optional[torch.Tensor] = None,
+    seq_lens: Optional[torch.Tensor] = None,   # may be ``lens`` itself
+    cu_new: Optional[torch.Tensor] = None,
+):
+    """Gives every request pages for its new tokens, on the GPU: no host copy of the lengths, capturable in a CUDA graph.
+
+    Returns ``(slots [n_tokens], positions [n_tokens], seq_lens [B], cu_new [B + 1])``: slot and position of each new token
+    packed in request order, the lengths with the new tokens, and the packed offsets.  Entries behind the last token are
+    left as they were.  Rows must be distinct.  The call takes effect as a whole or not at all: when the pages run out, or a
+    length does not fit the table or ``n_tokens``, everything is left as it was, the slots are -1 and the status
+    word says why.
+    """
+    dev, b, a = _pages_args(page_table, lens, new_lens, "new_lens", free_pages, n_free, page_size, rows)
+    if not 0 <= n_tokens < 2 ** 31:
+        raise RuntimeError(f"n_tokens ({n_tokens}) must be 0..2^31-1")
+    outs = []
+    for t, n, name in ((slots, n_tokens, "slots"), (positions, n_tokens, "positions"), (seq_lens, b, "seq_lens"), (cu_new, b + 1, "cu_new")):
+        if t is None:
+            t = torch.empty(n, dtype=torch.int32, device=page_table.device)
+        else:
+            _int32_1d(t, n, name)
+            _on_device(dev, ((t, name),))
+        outs.append(t)
+    handle, stream = _call(dev)
+    rc = _lib.load().dkv_assign_pages(handle, C.byref(a), outs[0].data_ptr(), outs[1].data_ptr(), n_tokens, outs[2].data_ptr(),
+                                      outs[3].data_ptr(), stream)
+    if rc:
+        _lib.check(rc)
+    return tuple(outs)
+
+
+def release_pages(
+    page_table: torch.Tensor,
+    lens: torch.Tensor,               # [B] int32 CUDA: tokens stored
+    keep_lens: torch.Tensor,          # [B] int32 CUDA: tokens that stay (0: all of the request's pages are freed)
+    free_pages: torch.Tensor,
+    n_free: torch.Tensor,
+    page_size: int,
+    rows: Optional[torch.Tensor] = None,
+) -> None:
+    """Puts the pages behind the tokens that stay back on the stack of free pages, on the GPU.
+
+    A release of exactly what the last ``assign_pages`` gave restores the stack.  The table's entries are left; nothing reads
+    them once the lengths are shorter.  As a whole or not at all, like ``assign_pages``.
+    """
+    dev, b, a = _pages_args(page_table, lens, keep_lens, "keep_lens", free_pages, n_free, page_size, rows)
+    if b == 0:
+        return
+    handle, stream = _call(dev)
+    rc = _lib.load().dkv_release_pages(handle, C.byref(a), stream)
+    if rc:
+        _lib.check(rc)
 
 
 # ---------------------------------------------------------------------------

@@ -43,6 +43,8 @@ extern "C" {
 #define DKV_STATUS_TMEM_TIMEOUT  (1u << 3)
 #define DKV_STATUS_EXCHANGE_ORDER (1u << 4)  /* dkv_decode_exchange: a record of another step arrived (calls of the ranks do not line up) */
 #define DKV_STATUS_BAD_PAGE      (1u << 5)  /* a length or row led outside the page table; the entry was not read */
+#define DKV_STATUS_NONFINITE     (1u << 6)  /* an infinity or a not-a-number was stored to a 4-bit pool (as the largest value, as zero) */
+#define DKV_STATUS_OUT_OF_PAGES  (1u << 7)  /* dkv_assign_pages: the stack of free pages was too short; nothing was assigned */
 /* Set together with a timeout bit: the kernel that gave up waiting. */
 #define DKV_STATUS_IN_STREAMING  (1u << 8)
 #define DKV_STATUS_IN_PROJ_LOAD  (1u << 9)
@@ -333,6 +335,133 @@ typedef struct {
 } dkv_noalloc_args;
 
 int dkv_decode_noalloc(const dkv_noalloc_args* args, void* stream);
+
+/*
+ * A KV pool held in 4 bits.  A row of 128 values is 8 blocks of 16 consecutive dimensions; with y = x / pool scale
+ *     s = e4m3(max |y| / 6), at least 2^-9, at most 448;  code = e2m1(y / s), nearest, ties to even;  x' = code * s * pool scale
+ * and takes 64 bytes of codes (dimension 2i in the low four bits of byte i, 2i + 1 in the high ones) and 8 bytes of
+ * scales instead of 256.  The four arrays lie in device memory or in pinned host memory.  Fill in everything but
+ * `resolved`, then call dkv_kv4_pool_resolve once per device: it checks the struct, replaces the pointers by the
+ * addresses the device uses, and marks it.  The arrays must stay valid while the struct is in use.
+ */
+typedef struct {
+    void*   k_codes;      /* [n_slots, nh_kv, 64] bytes, 16-byte aligned */
+    void*   k_scales;     /* [n_slots, nh_kv, 8] e4m3, 8-byte aligned, finite and not negative */
+    void*   v_codes;
+    void*   v_scales;
+    int64_t n_slots;      /* 1 .. 2^31 - 1 */
+    int     nh_kv;
+    int     page_size;    /* tokens per page, power of two >= 1 */
+    float   k_scale;      /* powers of two, 2^-24 .. 2^24 */
+    float   v_scale;
+    int     resolved;     /* set by dkv_kv4_pool_resolve; 0 before */
+} dkv_kv4_pool;
+
+int dkv_kv4_pool_resolve(dkv_context* ctx, dkv_kv4_pool* pool);
+
+/* The 4-bit counterpart of dkv_scatter_kv: row i of k / v ([n_tokens, nh_kv, 128] bf16 device, k_stride / v_stride
+ * elements from token to token) is quantised into slot slots[i] (int32 or int64, device).  A slot outside the
+ * pool is not written (DKV_STATUS_BAD_SLOT).  Two rows for one slot leave either of them or a mixture. */
+int dkv_kv4_store(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, int slots_int64, const void* k, int64_t k_stride,
+                  const void* v, int64_t v_stride, int64_t n_tokens, void* stream);
+
+/* Reads slots back: k / v [n_tokens, nh_kv, 128] bf16 device, contiguous; exact (see the format).  A slot outside the
+ * pool gives zeros (DKV_STATUS_BAD_SLOT). */
+int dkv_kv4_load(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, int slots_int64, void* k, void* v, int64_t n_tokens,
+                 void* stream);
+
+/*
+ * Decode attention over a 4-bit pool: dkv_decode with DKV_NEW_NONE for one or more query tokens per request.
+ * seq_lens[b] counts the stored tokens, the n_q query tokens' own included; query token j attends the first
+ * seq_lens[b] - n_q + 1 + j of them, and a row that attends nothing is zero with a log-sum-exp of -inf.
+ * Everything is read on the device, so the call can be captured and replayed with new lengths.  A page
+ * outside the pool counts as zeros, a length beyond the table is cut there, a row beyond the table (or a negative length)
+ * attends nothing; all three set DKV_STATUS_BAD_PAGE.
+ */
+typedef struct {
+    int            batch;        /* 0 .. 4096 */
+    int            n_q;          /* query tokens per request, 1 .. 1024 */
+    int            nh_q;
+    const void*    q;            /* bf16 device, token (b, j) at q + (b * n_q + j) * q_stride elements, [nh_q, 128] */
+    int64_t        q_stride;
+    void*          out;          /* likewise */
+    int64_t        out_stride;
+    const int32_t* seq_lens;     /* [batch] */
+    const int32_t* page_table;   /* [rows, pt_stride] */
+    int64_t        pt_stride;
+    int            pt_rows;      /* rows of the table, 0: unknown */
+    int            max_pages;    /* entries of a row that may be read */
+    const int32_t* row_map;      /* [batch] or NULL */
+    float          softmax_scale;
+    float*         lse_out;      /* [batch, n_q, nh_q] natural-log LSE, or NULL */
+} dkv_decode_kv4_args;
+
+int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_kv4_args* args, void* stream);
+
+/*
+ * RMS norm of every query and key head (x / sqrt(mean(x^2) + eps) * weight; weight NULL: no norm) and the Neox rotation at
+ * the tokens' positions (cos_sin NULL: none) in one pass, computed in fp32.  q [n_tokens, nh_q, 128], k
+ * [n_tokens, nh_k, 128] bf16 device with token strides in elements (multiples of 4); outputs likewise, in place when they are the
+ * inputs.  Weights are [128], or [heads, 128] with *_per_head, bf16 or fp32.  A position outside the table leaves the
+ * token unrotated (DKV_STATUS_BAD_POSITION).  nh_q or nh_k may be 0.
+ */
+typedef struct {
+    int64_t      n_tokens;
+    int          nh_q;
+    int          nh_k;
+    const void*  q;
+    int64_t      q_stride;
+    const void*  k;
+    int64_t      k_stride;
+    void*        q_out;
+    int64_t      q_out_stride;
+    void*        k_out;
+    int64_t      k_out_stride;
+    const void*  q_weight;
+    const void*  k_weight;
+    int          q_weight_f32;
+    int          k_weight_f32;
+    int          q_weight_per_head;
+    int          k_weight_per_head;
+    const void*  positions;      /* [n_tokens] int32 or int64 */
+    int          positions_int64;
+    const float* cos_sin;        /* [max_pos, 128] fp32 = [cos | sin] */
+    int          max_pos;
+    float        eps;
+} dkv_qk_norm_args;
+
+int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* args, void* stream);
+
+/*
+ * Page tables and slot maps on the GPU.  The free pages are a stack, free_pages[0 .. *n_free) of room for free_cap.
+ * dkv_assign_pages gives request b (row rows[b] of the table, or b) room for more[b] tokens behind its lens[b]: pages
+ * come off the top of the stack in request order, then page order, and are entered in the table; slots and positions
+ * [capacity] receive slot and position of every new token, packed in request order (entries behind the last one are
+ * left as they were); seq_lens[b] = lens[b] + more[b] (may be lens itself); cu_new [batch + 1] is the packed offset
+ * of every request.  dkv_release_pages puts the pages of the tokens [more[b], lens[b]) back on the stack - in the
+ * opposite order, so that a release of exactly the last assignment restores it - and leaves the table's entries.
+ * Rows must be distinct.  A call takes effect as a whole or not at all: a row, length or page beyond the table
+ * (DKV_STATUS_BAD_PAGE), too few free pages (DKV_STATUS_OUT_OF_PAGES) or more tokens than `capacity`, more pages than free_cap
+ * (DKV_STATUS_BAD_SLOT) leave stack, table and lengths as they were, with slots -1, positions 0 and cu_new 0.
+ */
+typedef struct {
+    int32_t*       page_table;   /* [pt_rows, pt_stride] */
+    int64_t        pt_stride;
+    int            pt_rows;
+    int            max_pages;    /* entries of a row */
+    const int32_t* rows;         /* [batch] or NULL */
+    const int32_t* lens;         /* [batch] */
+    const int32_t* more;         /* [batch] assign: new tokens; release: tokens that stay */
+    int            batch;        /* 0 .. 4096 */
+    int            page_size;    /* power of two */
+    int32_t*       free_pages;
+    int            free_cap;
+    int32_t*       n_free;       /* [1], read and written on the device */
+} dkv_pages_args;
+
+int dkv_assign_pages(dkv_context* ctx, const dkv_pages_args* args, int32_t* slots, int32_t* positions, int64_t capacity,
+                     int32_t* seq_lens, int32_t* cu_new, void* stream);
+int dkv_release_pages(dkv_context* ctx, const dkv_pages_args* args, void* stream);
 
 /* Measurement aid, not part of the drop-in surface (no counterpart in the reference): a device-side copy
  * kernel reading `bytes` from src (host-mapped or device) into dst (device) with plain vector loads, to find

@@ -1,0 +1,133 @@
+"""Argument checks of the 4-bit cache's operators, their C structs, and the plain forms the GPU tests compare with: no GPU."""
+
+import os
+import re
+
+import pytest
+import torch
+
+import kv4_ref as ref
+
+from directkv_b200 import _lib, kernel
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+BF = torch.bfloat16
+
+
+def _pool(n=32, nh=2, **kw):
+    return kernel.KV4Pool.empty(n, nh, device="cpu", **kw)
+
+
+def _i32(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+def test_struct_layouts_match_header_field_order():
+    text = open(os.path.join(ROOT, "include", "directkv_b200.h")).read()
+    for name, cls in (("dkv_kv4_pool", _lib.Kv4PoolDesc), ("dkv_decode_kv4_args", _lib.DecodeKv4Args), ("dkv_qk_norm_args", _lib.QkNormArgs),
+                      ("dkv_pages_args", _lib.PagesArgs)):
+        body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct \{([^}]*)\} " + name + ";", text).group(1), flags=re.S)
+        assert re.findall(r"([a-z_0-9]+)\s*;", body) == [f[0] for f in cls._fields_], name
+
+
+def test_plain_form_of_the_format():
+    """The format by hand: a block whose maximum is 6 has scale 1, and its values go to the nearest code."""
+    x = torch.zeros(1, 128, dtype=BF)
+    x[0, :8] = torch.tensor([6.0, 0.25, 0.75, -1.25, 2.5, 3.5, -5.0, 0.3])
+    codes, scales = ref.quantise(x)
+    assert scales[0, 0] == 0x38 and scales[0, 1] == 1
+    assert ref.values(codes, scales)[0, :8].tolist() == [6.0, 0.0, 1.0, -1.0, 2.0, 4.0, -4.0, 0.5]
+    assert codes[0, 0] == 0x07 and codes[0, 1] == 0xA2
+    # what the format holds it keeps
+    g = torch.Generator().manual_seed(0)
+    y = ref.values(*ref.quantise(torch.randn(50, 128, generator=g).to(BF)))
+    assert torch.equal(ref.values(*ref.quantise(y.to(BF))), y)
+    assert torch.equal(torch.arange(1, 127).to(torch.uint8).view(torch.float8_e4m3fn).double(), ref.E4M3[1:])
+
+
+def test_pool_checks():
+    c, s = torch.zeros(8, 2, 64, dtype=torch.uint8), torch.zeros(8, 2, 8, dtype=torch.uint8)
+    pool = kernel.KV4Pool(c, s, c.clone(), s.clone(), page_size=4, k_scale=0.25)
+    assert (pool.n_slots, pool.nh_kv, pool.nbytes()) == (8, 2, 8 * 2 * 144)
+    for kw in (dict(page_size=3), dict(page_size=0), dict(k_scale=3.0), dict(v_scale=0.0), dict(v_scale=-1.0), dict(k_scale=2.0 ** 25), dict(k_scale=float("nan"))):
+        with pytest.raises(RuntimeError, match="power of two"):
+            kernel.KV4Pool(c, s, c, s, **kw)
+    for args in ((c[:, :, :32], s, c, s), (c, s[:4], c, s), (c, s, c.float(), s), (c, s, c[::2], s), (c, c, c, s), (c[0], s, c, s)):
+        with pytest.raises(RuntimeError, match="k_codes|codes must|scales must"):
+            kernel.KV4Pool(*args)
+
+
+def test_store_and_load_refuse():
+    pool = _pool()
+    k = torch.zeros(3, 2, 128, dtype=BF)
+    ok = _i32(3)
+    for slots, kk, vv, why in ((_i32(2), k, k, "must be"), (ok.float(), k, k, "int32 or int64"), (_i32(6)[::2], k, k, "contiguous"), (_i32(3, 1), k, k, "1D"),
+                               (ok, k[:, :1], k, "must be"), (ok, k.float(), k, "bfloat16"), (ok, k, k.transpose(1, 2).contiguous().transpose(1, 2), "next to each other"),
+                               (ok, k[..., :64], k, "next to each other|must be"), (ok, k, k, "CUDA tensor")):
+        with pytest.raises(RuntimeError, match=why):
+            kernel.store_kv4(pool, slots, kk, vv)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        kernel.load_kv4(pool, ok)
+    with pytest.raises(RuntimeError, match="int32 or int64"):
+        kernel.load_kv4(pool, ok.short())
+
+
+def test_decode_refuses():
+    pool = _pool()
+    q = torch.zeros(2, 4, 128, dtype=BF)
+    lens, table = _i32(2), _i32(2, 3)
+    cases = [
+        (dict(q=q[:, :3]), "multiple of"), (dict(q=q.float()), "bfloat16"), (dict(q=torch.zeros(2, 500, dtype=BF)), "must be"),
+        (dict(q=torch.zeros(2, 2, 2, 4, 128, dtype=BF)), "3D or 4D"), (dict(q=torch.zeros(4, 3, 4, 128, dtype=BF)[::2, :2]), "evenly spaced"),
+        (dict(q=torch.zeros(2, 0, 4, 128, dtype=BF)), "at most"), (dict(q=torch.zeros(2, 1025, 4, 128, dtype=BF)), "at most"),
+        (dict(q=torch.zeros(4097, 4, 128, dtype=BF), seq_lens=_i32(4097), page_table=_i32(4097, 1)), "at most"),
+        (dict(seq_lens=_i32(3)), "seq_lens"), (dict(seq_lens=lens.long()), "seq_lens"), (dict(page_table=table.long()), "page_table"), (dict(page_table=_i32(6)), "page_table"),
+        (dict(page_table=_i32(3, 2).t()), "page_table"), (dict(page_table=_i32(1, 3)), "rows for 2"), (dict(row_map=_i32(1)), "row_map"), (dict(lse_out=torch.zeros(2, 3)), "lse_out"),
+        (dict(lse_out=torch.zeros(2, 4).double()), "lse_out"), ({}, "CUDA tensor"),
+    ]
+    for kw, why in cases:
+        a = dict(q=q, pool=pool, seq_lens=lens, softmax_scale=1.0, page_table=table)
+        a.update(kw)
+        with pytest.raises(RuntimeError, match=why):
+            kernel.decode_kv4(**a)
+
+
+def test_qk_norm_rope_refuses():
+    q, k, pos, cs, w = torch.zeros(3, 4, 128, dtype=BF), torch.zeros(3, 2, 128, dtype=BF), _i32(3), torch.zeros(9, 128), torch.ones(128, dtype=BF)
+    cuda = "CUDA tensor"
+    cases = [
+        (dict(q=None, k=None), "must be given"), (dict(q=q[:2]), "must be"), (dict(k=k[0]), "must be"), (dict(q=q.float()), "bfloat16"), (dict(q=q[..., ::2]), "next to each other"),
+        (dict(q_out=q[:, :2]), "shape of q"), (dict(q_out=q.float()), "bfloat16"), (dict(q_weight=w.half()), "q_weight|" + cuda), (dict(k_weight=torch.ones(3, 128, dtype=BF)), "k_weight|" + cuda),
+        (dict(q_weight=torch.ones(64, dtype=BF)), "q_weight"), ({}, cuda),
+    ]
+    for kw, why in cases:
+        a = dict(q=q, k=k, positions=pos, cos_sin=cs, q_weight=w, k_weight=w)
+        a.update(kw)
+        with pytest.raises(RuntimeError, match=why):
+            kernel.qk_norm_rope(**a)
+
+
+def test_pages_refuse():
+    table, lens, free, n = _i32(4, 3), _i32(2), _i32(8), _i32(1)
+    base = dict(page_table=table, lens=lens, new_lens=lens, free_pages=free, n_free=n, page_size=16, n_tokens=4)
+    cases = [
+        (dict(lens=lens.long()), "lens"), (dict(new_lens=_i32(3)), "new_lens"), (dict(rows=_i32(1)), "rows"), (dict(page_table=table.t()), "page_table"), (dict(page_table=_i32(4)), "page_table"),
+        (dict(page_table=_i32(1, 3).expand(4, 3)), "overlap"), (dict(free_pages=free.long()), "free_pages"), (dict(free_pages=free[::2]), "free_pages"), (dict(n_free=_i32(2)), "n_free"),
+        (dict(page_size=12), "power of two"), (dict(lens=_i32(4097), new_lens=_i32(4097)), "at most 4096"), ({}, "CUDA tensor"),
+    ]
+    for kw, why in cases:
+        with pytest.raises(RuntimeError, match=why):
+            kernel.assign_pages(**{**base, **kw})
+    rel = {k: v for k, v in base.items() if k not in ("new_lens", "n_tokens")}
+    for kw, why in (({}, "CUDA tensor"), (dict(keep_lens=_i32(1)), "keep_lens")):
+        with pytest.raises(RuntimeError, match=why):
+            kernel.release_pages(**{**rel, "keep_lens": lens, **kw})
+
+
+def test_plain_pages_restore_the_stack():
+    table = torch.zeros(2, 9, dtype=torch.int32)
+    p = ref.Pages(table, torch.arange(1, 20), 19, 4)
+    slots, pos, lens, cu = p.assign([0, 1], [0, 0], [5, 9])
+    assert slots[:5] == [76, 77, 78, 79, 72] and pos[5:] == list(range(9)) and cu == [0, 5, 14] and p.n == 14
+    p.release([0, 1], lens, [0, 0])
+    assert p.stack == list(range(1, 20)) and p.n == 19

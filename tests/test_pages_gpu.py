@@ -1,0 +1,214 @@
+"""Page tables and slot maps built on the GPU, against Python lists; and the operators of a decode step over a 4-bit cache in a row."""
+
+import pytest
+import torch
+
+import kv4_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+from directkv_b200 import kernel, workloads  # noqa: E402
+from directkv_b200._lib import get_context  # noqa: E402
+
+DEV = "cuda:0"
+BAD_SLOT, BAD_PAGE, OUT_OF_PAGES = 1 << 1, 1 << 5, 1 << 7
+
+
+@pytest.fixture(autouse=True)
+def _clean_status():
+    get_context(0).read_status(clear=True)
+    yield
+    get_context(0).read_status(clear=True)
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _setup(lens, page, spare_pages, max_pages, seed, n_rows=None):
+    g = torch.Generator().manual_seed(seed)
+    n_rows = n_rows or len(lens) + 2
+    rows = torch.randperm(n_rows, generator=g)[:len(lens)].tolist()
+    held = sum(-(-n // page) for n in lens)
+    order = (torch.randperm(held + spare_pages, generator=g) + 1).to(torch.int32)
+    table = torch.full((n_rows, max_pages), -7, dtype=torch.int32)
+    at = spare_pages
+    for r, n in zip(rows, lens):
+        c = -(-n // page)
+        table[r, :c] = order[at:at + c]
+        at += c
+    return rows, table, order, spare_pages
+
+
+def _same(state, table, free, n_free):
+    assert torch.equal(table.cpu(), state.table)
+    assert int(n_free) == state.n
+    assert free.cpu().tolist()[:state.n] == state.stack[:state.n]
+
+
+@pytest.mark.parametrize("page", [1, 2, 16, 128])
+@pytest.mark.parametrize("lens,new", [([0], [1]), ([5], [0]), ([0, 16, 15, 17, 1, 0], [1, 1, 1, 1, 1, 0]), ([0, 0, 0], [33, 0, 700]),
+                                      ([3, 200, 31, 0, 64], [5000, 1, 0, 77, 64])])
+def test_assign_and_release(page, lens, new):
+    need = sum(-(-(a + n) // page) - -(-a // page) for a, n in zip(lens, new))
+    max_pages = max(-(-(a + n) // page) for a, n in zip(lens, new)) + 1
+    rows, table, order, spare = _setup(lens, page, need + 3, max_pages, 11)
+    state = ref.Pages(table, order, spare, page)
+    t, free, n_free = table.to(DEV), order.to(DEV), _i32([spare])
+    room = sum(new) + 5
+    slots, positions = torch.full((room,), -9, dtype=torch.int32, device=DEV), torch.full((room,), -9, dtype=torch.int32, device=DEV)
+    got = kernel.assign_pages(t, _i32(lens), _i32(new), free, n_free, page, room, rows=_i32(rows), slots=slots, positions=positions)
+    want = state.assign(rows, lens, new)
+    total = sum(new)
+    assert got[0] is slots and got[1] is positions
+    assert slots.cpu().tolist() == want[0] + [-9] * 5 and positions.cpu().tolist() == want[1] + [-9] * 5
+    assert got[2].cpu().tolist() == want[2] and got[3].cpu().tolist() == want[3]
+    _same(state, t, free, n_free)
+    assert total == want[3][-1]
+    # the same tokens taken back: the stack is what it was before
+    kernel.release_pages(t, got[2], _i32(lens), free, n_free, page, rows=_i32(rows))
+    state.release(rows, want[2], lens)
+    _same(state, t, free, n_free)
+    assert int(n_free) == spare and torch.equal(free.cpu(), order)
+    # all pages of every request
+    room_list = torch.zeros(order.numel() + 4, dtype=torch.int32, device=DEV)
+    room_list[:order.numel()] = free
+    state.stack += [0] * 4
+    kernel.release_pages(t, _i32(lens), _i32([0] * len(lens)), room_list, n_free, page, rows=_i32(rows))
+    state.release(rows, lens, [0] * len(lens))
+    _same(state, t, room_list, n_free)
+    assert get_context(0).read_status() == 0
+
+
+def test_many_requests_and_tokens():
+    """More blocks than one and more requests than a block has threads; lengths updated in place, step after step."""
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 60, (1500,), generator=g).tolist()
+    page = 16
+    rows, table, order, spare = _setup(lens, page, 9000, 12, 12)
+    state = ref.Pages(table, order, spare, page)
+    t, free, n_free, lens_t = table.to(DEV), order.to(DEV), _i32([spare]), _i32(lens)
+    for step in range(3):
+        new = torch.randint(0, 40, (1500,), generator=g).tolist()
+        got = kernel.assign_pages(t, lens_t, _i32(new), free, n_free, page, sum(new), rows=_i32(rows), seq_lens=lens_t)
+        want = state.assign(rows, lens, new)
+        for x, y in zip(got, want):
+            assert x.cpu().tolist() == list(y)
+        lens = want[2]
+        _same(state, t, free, n_free)
+    keep = [n // 3 for n in lens]
+    kernel.release_pages(t, lens_t, _i32(keep), free, n_free, page, rows=_i32(rows))
+    state.release(rows, lens, keep)
+    _same(state, t, free, n_free)
+    assert get_context(0).read_status() == 0
+
+
+@pytest.mark.parametrize("what,status", [("pages", OUT_OF_PAGES), ("room", BAD_SLOT), ("row", BAD_PAGE), ("negative row", BAD_PAGE), ("table", BAD_PAGE),
+                                         ("negative", BAD_PAGE), ("stack", BAD_PAGE)])
+def test_assign_takes_effect_as_a_whole_or_not_at_all(what, status):
+    lens, new, page = [5, 30, 0], [20, 3, 40], 16
+    rows, table, order, spare = _setup(lens, page, 6, 4, 13)
+    n_tokens = sum(new)
+    if what == "pages":
+        spare = 3
+    if what == "room":
+        n_tokens -= 1
+    if what == "row":
+        rows[1] = 5
+    if what == "negative row":
+        rows[1] = -1
+    if what == "table":
+        new[2] = 65
+        n_tokens = sum(new)
+    if what == "negative":
+        new[0] = -1
+        n_tokens = 43
+    if what == "stack":
+        spare = order.numel() + 1
+    t, free, n_free = table.to(DEV), order.to(DEV), _i32([spare])
+    got = kernel.assign_pages(t, _i32(lens), _i32(new), free, n_free, page, n_tokens, rows=_i32(rows))
+    assert get_context(0).read_status() == status
+    assert torch.equal(t.cpu(), table) and torch.equal(free.cpu(), order) and int(n_free) == spare
+    assert (got[0] == -1).all() and (got[1] == 0).all() and got[2].cpu().tolist() == lens and not got[3].any()
+
+
+def test_release_takes_effect_as_a_whole_or_not_at_all():
+    lens, page = [50, 30, 1], 16
+    for what, keep, room, status in (("stack", [0, 0, 0], 6, BAD_SLOT), ("longer", [0, 31, 0], 20, BAD_PAGE), ("negative", [-1, 0, 0], 20, BAD_PAGE)):
+        rows, table, order, spare = _setup(lens, page, 2, 4, 14)
+        free = torch.zeros(room, dtype=torch.int32)
+        free[:2] = order[:2]
+        f, n_free = free.to(DEV), _i32([2])
+        kernel.release_pages(table.to(DEV), _i32(lens), _i32(keep), f, n_free, page, rows=_i32(rows))
+        assert get_context(0).read_status() == status, what
+        assert torch.equal(f.cpu(), free) and int(n_free) == 2
+
+
+def test_no_requests():
+    table, free, n_free = torch.zeros(2, 2, dtype=torch.int32, device=DEV), _i32([1, 2]), _i32([2])
+    got = kernel.assign_pages(table, _i32([]), _i32([]), free, n_free, 16, 0)
+    assert [x.numel() for x in got] == [0, 0, 0, 1] and int(got[3]) == 0 and int(n_free) == 2
+    kernel.release_pages(table, _i32([]), _i32([]), free, n_free, 16)
+
+
+def test_decode_steps_over_a_four_bit_cache():
+    """What a serving loop runs, captured once and replayed: pages and slots, head norms with rotation, store, attention.
+    Two graphs share the context's workspace and are replayed in turn; every step is checked against the plain forms."""
+    batch, nh_q, nh_kv, page, steps = 5, 8, 2, 4, 6
+    g = torch.Generator().manual_seed(21)
+    cs = workloads.build_cos_sin(64, 10000.0)
+    wq, wk = [(1 + 0.2 * torch.randn(128, generator=g)).to(torch.bfloat16) for _ in range(2)]
+    pool = kernel.KV4Pool.empty(200, nh_kv, page, DEV)
+    table, free, n_free = torch.zeros(batch, 12, dtype=torch.int32, device=DEV), torch.arange(1, 50, dtype=torch.int32, device=DEV), _i32([49])
+    state = ref.Pages(table.cpu(), free.cpu(), 49, page)
+    lens = torch.zeros(batch, dtype=torch.int32, device=DEV)
+    w = dict(cos_sin=cs.to(DEV), q_weight=wq.to(DEV), k_weight=wk.to(DEV))
+    n_q = {0: 1, 1: 3}                                   # one token per request, or three drafted ones
+    graphs, bufs = {}, {}
+    for i in n_q:
+        n = batch * n_q[i]
+        b = bufs[i] = dict(rows=torch.zeros(n, nh_q + 2 * nh_kv, 128, dtype=torch.bfloat16, device=DEV), new=_i32([n_q[i]] * batch),
+                           slots=torch.zeros(n, dtype=torch.int32, device=DEV), pos=torch.zeros(n, dtype=torch.int32, device=DEV),
+                           cu=torch.zeros(batch + 1, dtype=torch.int32, device=DEV), out=torch.zeros(batch, n_q[i], nh_q, 128, dtype=torch.bfloat16, device=DEV))
+
+        def step(b=b, m=n_q[i]):
+            q, k, v = b["rows"][:, :nh_q], b["rows"][:, nh_q:nh_q + nh_kv], b["rows"][:, nh_q + nh_kv:]
+            kernel.assign_pages(table, lens, b["new"], free, n_free, page, batch * m, slots=b["slots"], positions=b["pos"], seq_lens=lens, cu_new=b["cu"])
+            kernel.qk_norm_rope(q, k, b["pos"], w["cos_sin"], w["q_weight"], w["k_weight"], q_out=q, k_out=k)
+            kernel.store_kv4(pool, b["slots"], k, v)
+            kernel.decode_kv4(q.view(batch, m, nh_q, 128), pool, lens, 128 ** -0.5, table, out=b["out"])
+
+        # one eager step on a copy of the state sizes the workspace, then the capture
+        saved = [t.clone() for t in (table, free, n_free, lens)]
+        step()
+        torch.cuda.synchronize()
+        for t, s in zip((table, free, n_free, lens), saved):
+            t.copy_(s)
+        graphs[i] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graphs[i]):
+            step()
+    host = [0] * batch
+    kv = {b: [torch.zeros(0, nh_kv, 128, dtype=torch.float64) for _ in range(2)] for b in range(batch)}
+    for s in range(steps):
+        i = s % 2
+        m, b = n_q[i], bufs[i]
+        rows = torch.randn(batch * m, nh_q + 2 * nh_kv, 128, generator=g).to(torch.bfloat16)
+        b["rows"].copy_(rows)
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        slots, pos, host, cu = state.assign(range(batch), host, [m] * batch)
+        assert b["slots"].cpu().tolist() == slots and b["pos"].cpu().tolist() == pos and lens.cpu().tolist() == host
+        p = torch.tensor(pos)
+        for x, wt, got in ((rows[:, :nh_q], wq, b["rows"][:, :nh_q]), (rows[:, nh_q:nh_q + nh_kv], wk, b["rows"][:, nh_q:nh_q + nh_kv])):
+            y, e = ref.norm_rope(x, wt, p, cs, 1e-6)
+            assert ((got.cpu().double() - y).abs() <= e).all()
+        q, k, v = b["rows"][:, :nh_q].cpu(), b["rows"][:, nh_q:nh_q + nh_kv].cpu(), rows[:, nh_q + nh_kv:]
+        for r in range(batch):
+            at = slice(r * m, (r + 1) * m)
+            for j, x in enumerate((k, v)):
+                kv[r][j] = torch.cat([kv[r][j], ref.values(*ref.quantise(x[at]))])
+            o, _, e = ref.attend(q[at], kv[r][0], kv[r][1], host[r], 128 ** -0.5)
+            assert ((b["out"][r].cpu().double() - o).abs() <= e).all(), (s, r)
+    assert get_context(0).read_status() == 0
+    kernel.release_pages(table, lens, torch.zeros_like(lens), free, n_free, page)
+    assert int(n_free) == 49 and sorted(free.cpu().tolist()) == list(range(1, 50))
