@@ -149,6 +149,7 @@ struct dkv_context {
     int device = 0;
     int sm_count = 0;
     DevBuffer scratch;                  // per-call tables, partial records, new-token rows, split-K slices
+    DevBuffer kv4;                      // records and tile counts of the 4-bit attention
     DevBuffer stage;                    // extend over a host or paged pool: the requests' rows gathered in HBM
     std::vector<void*> retired;         // outgrown allocations that a captured graph may still use
     unsigned int* status = nullptr;     // device status word
@@ -925,6 +926,7 @@ int dkv_context_destroy(dkv_context* ctx) {
     if (ctx->ev_join) cudaEventDestroy(ctx->ev_join);
     if (ctx->scratch.ptr) cudaFree(ctx->scratch.ptr);
     if (ctx->stage.ptr) cudaFree(ctx->stage.ptr);
+    if (ctx->kv4.ptr) cudaFree(ctx->kv4.ptr);
     for (void* p : ctx->retired) cudaFree(p);
     if (ctx->ragged_host) cudaFreeHost(ctx->ragged_host);
     if (ctx->ragged_dev) cudaFree(ctx->ragged_dev);

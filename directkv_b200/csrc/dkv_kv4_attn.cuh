@@ -2,11 +2,32 @@
 //
 // out[b, j, h] = sum_t p_t v_t with p = softmax over t < len_b - n_q + 1 + j of scale * q[b, j, h] . k_t; a row that
 // attends nothing is zero with a log-sum-exp of -inf.
+//
+// One pass over the rows with a running maximum and sum.  The (query token, head) pairs that share a KV head are the
+// columns of two warp-level products (m16n8k16, fp16 in, fp32 out) per 16 tokens:
+//     S [16 tokens x 8 columns] = K Q^T            O^T [128 dims x 8 columns] += V^T P^T
+// so a row is decoded once for all of them.  Nothing is lost on the way in: code * block scale is exact in fp16, and a
+// query row is scaled by a power of two that brings its largest value to 2^14 before it becomes fp16 (undone in the
+// fp32 scores).  P is rounded to fp16 (2^-11, against bf16's 2^-8); scores, maximum, sum and O are fp32.
+//
+// What bounds it is bytes: 144 per token and KV head.  A warp brings its tokens in through its own ring of
+// cp.async copies (any page size, device or host pool alike: every lane looks its tokens' pages up itself), so warps
+// never wait for one another.  A block's warps take neighbouring heads of the same tokens, which makes the 64-byte
+// rows of a token one contiguous read.
 #pragma once
 
+#include "dkv_attn_mma.cuh"
 #include "dkv_kv4.cuh"
 
 namespace dkv {
+
+constexpr int kKv4Warps = 8;
+constexpr int kKv4Stages = 4;
+constexpr int kKv4StageBytes = 2 * 1024 + 2 * 128;       // 16 tokens: K codes, V codes, K scales, V scales
+constexpr int kKv4RingBytes = kKv4Stages * kKv4StageBytes;
+constexpr int kKv4MaxBatch = 4096;
+constexpr int kKv4RecFloats = 132;                       // O[128], m (log2 domain), l, 2 pad
+constexpr float kKv4Lag = 8.f;                           // the maximum follows once a score is 2^8 above it: P <= 2^8 in fp16
 
 struct Kv4AttnParams {
     const __nv_bfloat16* q;          // row (b, j) at q + (b * n_q + j) * q_stride, [nh_q, 128]
@@ -26,81 +47,497 @@ struct Kv4AttnParams {
     const uint8_t* v_scales;
     long long n_slots;
     int page_shift;
-    int batch, n_q, nh_q, nh_kv;
+    int batch, n_q, nh_q, nh_kv, group;
+    int cols;                        // n_q * group: columns of one KV head
+    int n_cc;                        // column chunks of 8 * NT
+    int hg, ts, n_hg;                // heads and token lanes of a block (hg * ts <= kKv4Warps), head groups
     float scale_log2;                // softmax scale * k_scale * log2(e)
     float v_scale;
+    float* rec;                      // [blocks, 2, hg, 8 * NT, kKv4RecFloats]
+    int* cum;                        // [batch + 1] tiles before each request
     unsigned int* status;
 };
 
-__device__ __forceinline__ void kv4_row4(const uint8_t* codes, const uint8_t* scales, long long at, int lane, float (&v)[4]) {
-    // Whole words go into the conversion: fed a 16-bit load, the compiled conversion took its bytes from the wrong place.
-    const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + at * 64 + (lane >> 1) * 4);
-    uint32_t h[4];
-    e2m1x8_to_f16(c, h);
-    const float s = e4m3_to_f32(scales[at * 8 + (lane >> 2)]);
-    const uint32_t h0 = lane & 1 ? h[2] : h[0], h1 = lane & 1 ? h[3] : h[1];
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-    v[0] = a.x * s, v[1] = a.y * s, v[2] = b.x * s, v[3] = b.y * s;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ldsf(uint32_t a) { return __uint_as_float(lds32(a)); }
+__device__ __forceinline__ void stsf(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
+
+__device__ __forceinline__ uint32_t hmul2_f16(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ uint32_t bit_select(uint32_t a, uint32_t b, uint32_t mask) {   // mask ? a : b
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xCA;" : "=r"(d) : "r"(mask), "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// One block per (request, query token, head); every warp takes every fourth token, lane l dimensions 4l..4l+3.
-__global__ void __launch_bounds__(128) kv4_attn_kernel(const Kv4AttnParams p) {
-    __shared__ float sm[4][130];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int h = blockIdx.x, j = blockIdx.y, b = blockIdx.z;
-    const int kvh = h / (p.nh_q / p.nh_kv);
-    long long row = p.row_map != nullptr ? p.row_map[b] : b;
-    int len = p.seq_lens[b];
+// The share of the flattened tile list that block i of n takes, and the block that has tile x.
+__device__ __forceinline__ long long kv4_share(long long total, int i, int n) { return total * i / n; }
+__device__ __forceinline__ int kv4_owner(long long total, long long x, int n) {
+    return static_cast<int>(((x + 1) * n - 1) / total);
+}
+__device__ __forceinline__ int kv4_blocks(long long total, int grid) { return total < grid ? static_cast<int>(total) : grid; }
+
+// A request's length as far as the table reaches, and its row; a length or row outside is reported.
+__device__ __forceinline__ int kv4_length(const Kv4AttnParams& p, int b, long long* row_out) {
+    const long long row = p.row_map != nullptr ? p.row_map[b] : b;
+    *row_out = row;
+    const int len = p.seq_lens[b];
     const long long room = static_cast<long long>(p.max_pages) << p.page_shift;
-    if (row < 0 || (p.pt_rows > 0 && row >= p.pt_rows) || len > room || len < 0) {
-        if (threadIdx.x == 0) atomicOr(p.status, kStatusBadPage);
-        len = row < 0 || (p.pt_rows > 0 && row >= p.pt_rows) || len < 0 ? 0 : static_cast<int>(room);
-    }
-    const int n = len - p.n_q + 1 + j;
-    const uint2 qw = *reinterpret_cast<const uint2*>(p.q + (static_cast<long long>(b) * p.n_q + j) * p.q_stride + h * 128 + lane * 4);
-    const float q[4] = {bf16lo(qw.x), bf16hi(qw.x), bf16lo(qw.y), bf16hi(qw.y)};
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int t = w; t < n; t += 4) {
-        const long long page = p.page_table[row * p.pt_stride + (t >> p.page_shift)];
-        const long long slot = (page << p.page_shift) + (t & ((1 << p.page_shift) - 1));
-        float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (slot >= 0 && slot < p.n_slots) {
-            kv4_row4(p.k_codes, p.k_scales, slot * p.nh_kv + kvh, lane, k);
-            kv4_row4(p.v_codes, p.v_scales, slot * p.nh_kv + kvh, lane, v);
-        } else if (lane == 0) {
-            atomicOr(p.status, kStatusBadPage);
+    if (row < 0 || (p.pt_rows > 0 && row >= p.pt_rows) || len < 0) return -1;
+    return len > room ? -2 : len;
+}
+__device__ __forceinline__ int kv4_clean_length(const Kv4AttnParams& p, int code) {
+    return code >= 0 ? code : (code == -2 ? static_cast<int>(static_cast<long long>(p.max_pages) << p.page_shift) : 0);
+}
+
+template <int NT>
+struct Kv4State {
+    float o[8][NT][4];
+    float m[NT][2], l[NT][2];
+};
+
+template <int NT>
+__global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4AttnParams p) {
+    constexpr int C = 8 * NT;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int sh_scan[kKv4Warps];
+    int* cum = reinterpret_cast<int*>(smem + kKv4Warps * kKv4RingBytes);
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int g = lane >> 2, c = lane & 3;
+
+    // Tiles (of 16 * ts tokens) before every request; a request without tokens has one, which writes its zeros.
+    if (threadIdx.x == 0) cum[0] = 0;
+    int before = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += kKv4Warps * 32) {
+        const int b = b0 + threadIdx.x;
+        int n = 0;
+        if (b < p.batch) {
+            long long row;
+            const int code = kv4_length(p, b, &row);
+            if (code < 0 && blockIdx.x == 0) atomicOr(p.status, kStatusBadPage);
+            const int len = kv4_clean_length(p, code);
+            n = max(1, static_cast<int>((static_cast<long long>(len) + 16 * p.ts - 1) / (16 * p.ts)));
         }
-        float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+        int inc = n;
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= p.scale_log2;
-        const float m2 = fmaxf(m, s), c = exp2f(m - m2), e = exp2f(s - m2);
-        l = l * c + e;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = o[i] * c + e * v[i];
-        m = m2;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += x;
+        }
+        if (lane == 31) sh_scan[w] = inc;
+        __syncthreads();
+        int base = before;
+        for (int i = 0; i < w; ++i) base += sh_scan[i];
+        if (b < p.batch) cum[b + 1] = base + inc;
+        for (int i = 0; i < kKv4Warps; ++i) before += sh_scan[i];
+        __syncthreads();
     }
+    if (blockIdx.x == 0)
+        for (int b = threadIdx.x; b <= p.batch; b += blockDim.x) p.cum[b] = cum[b];
+    const int per_tile = p.n_hg * p.n_cc;
+    const long long total = static_cast<long long>(before) * per_tile;
+    const int blocks = kv4_blocks(total, gridDim.x);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (static_cast<int>(blockIdx.x) >= blocks) return;
+    const long long x0 = kv4_share(total, blockIdx.x, blocks), x1 = kv4_share(total, blockIdx.x + 1, blocks);
+
+    const int hl = w % p.hg, tl = w / p.hg;
+    const bool active = tl < p.ts;
+    const uint32_t ring = smem_u32(smem) + w * kKv4RingBytes;
+    const int tau = (g >> 1) + 4 * (g & 1);          // token of this lane's rows of the score tile: tau and tau + 8
+    const int page_mask = (1 << p.page_shift) - 1;
+    Kv4State<NT> st;
+
+    for (long long x = x0; x < x1;) {
+        // Segment: one request, head group and column chunk.
+        const int y = static_cast<int>(x / per_tile);
+        int lo = 0, hi = p.batch - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (cum[mid] <= y) lo = mid;
+            else hi = mid - 1;
+        }
+        const int b = lo;
+        const int tiles = cum[b + 1] - cum[b];
+        const long long r = x - static_cast<long long>(cum[b]) * per_tile;
+        const int seg = static_cast<int>(r / tiles), tile0 = static_cast<int>(r - static_cast<long long>(seg) * tiles);
+        const int n_tiles = static_cast<int>(min(static_cast<long long>(tiles - tile0), x1 - x));
+        const int hgi = seg / p.n_cc, cc = seg - hgi * p.n_cc;
+        const bool whole = n_tiles == tiles;
+        const int kvh = hgi * p.hg + hl;
+        long long row;
+        const int len = kv4_clean_length(p, kv4_length(p, b, &row));
+        const int* table = p.page_table + row * p.pt_stride;
+
+        if (active) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sm[w][lane * 4 + i] = o[i];
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) st.o[i][n][k] = 0.f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) st.m[n][0] = st.m[n][1] = -INFINITY, st.l[n][0] = st.l[n][1] = 0.f;
+
+            // ---- copies: this lane brings 16 bytes of K and V of tokens tau and tau + 8, and 8 bytes of scales
+            auto lookup = [&](int t) { return t < len ? __ldg(table + (t >> p.page_shift)) : -1; };
+            auto slot_of = [&](int t, int page) -> long long {
+                if (t >= len) return -1;
+                const long long s = (static_cast<long long>(page) << p.page_shift) + (t & page_mask);
+                if (page < 0 || s >= p.n_slots) {
+                    atomicOr(p.status, kStatusBadPage);
+                    return -1;
+                }
+                return s;
+            };
+            auto token0 = [&](int i) { return ((tile0 + i) * p.ts + tl) * 16 + tau; };
+            auto issue = [&](int i, int pa, int pb) {
+                const uint32_t s = ring + (i % kKv4Stages) * kKv4StageBytes;
+                const int t = token0(i);
+                const long long sa = slot_of(t, pa), sb = slot_of(t + 8, pb);
+                const long long ra = sa < 0 ? 0 : sa * p.nh_kv + kvh, rb = sb < 0 ? 0 : sb * p.nh_kv + kvh;
+                const uint32_t na = sa < 0 ? 0u : 16u, nb = sb < 0 ? 0u : 16u;
+                cp_async16(s + lane * 16, p.k_codes + ra * 64 + c * 16, na);
+                cp_async16(s + 512 + lane * 16, p.k_codes + rb * 64 + c * 16, nb);
+                const uint32_t vq = s + 1024 + tau * 64 + ((c ^ ((g >> 1) & 2)) << 4);      // 16-byte pieces of rows 2, 3 mod 4 change places
+                cp_async16(vq, p.v_codes + ra * 64 + c * 16, na);
+                cp_async16(vq + 512, p.v_codes + rb * 64 + c * 16, nb);
+                const uint8_t* sc = (c & 2) ? p.v_scales : p.k_scales;
+                cp_async8(s + 2048 + (c & 2) * 64 + (tau + (c & 1) * 8) * 8, sc + ((c & 1) ? rb : ra) * 8, ((c & 1) ? nb : na) >> 1);
+            };
+            int pa = lookup(token0(0)), pb = lookup(token0(0) + 8);
+#pragma unroll
+            for (int i = 0; i < kKv4Stages - 1; ++i) {
+                if (i < n_tiles) issue(i, pa, pb);
+                cp_async_commit();
+                pa = lookup(token0(i + 1)), pb = lookup(token0(i + 1) + 8);
+            }
+
+            // ---- queries: column g of each 8, dimensions 32 c .. 32 c + 31, as fp16 scaled by a power of two
+            uint32_t qf[NT][8][2];
+            float mul[NT][2];
+            int limit[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int col = cc * C + n * 8 + g;
+                uint4 v[4];
+                uint32_t top = 0;
+                if (col < p.cols) {
+                    const int j = col / p.group, h = kvh * p.group + (col - j * p.group);
+                    const uint4* src = reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(b) * p.n_q + j) * p.q_stride + h * 128 + c * 32);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = __ldg(src + i);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    top = max(max(max(top, (v[i].x & 0x7fffu)), max((v[i].x >> 16) & 0x7fffu, v[i].y & 0x7fffu)),
+                              max(max((v[i].y >> 16) & 0x7fffu, v[i].z & 0x7fffu),
+                                  max((v[i].z >> 16) & 0x7fffu, max(v[i].w & 0x7fffu, (v[i].w >> 16) & 0x7fffu))));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                int e = static_cast<int>(top >> 7);                                 // biased exponent of the largest value
+                e = e == 255 ? 127 + 14 : max(e, 127 + 14 - 100);                   // not finite: as it is; tiny rows: at most 2^100
+                const float f = __uint_as_float(static_cast<uint32_t>(127 + 14 - e + 127) << 23);
+                const float undo = __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    qf[n][2 * i][0] = pack_f16x2(bf16lo(v[i].x) * f, bf16hi(v[i].x) * f);
+                    qf[n][2 * i][1] = pack_f16x2(bf16lo(v[i].y) * f, bf16hi(v[i].y) * f);
+                    qf[n][2 * i + 1][0] = pack_f16x2(bf16lo(v[i].z) * f, bf16hi(v[i].z) * f);
+                    qf[n][2 * i + 1][1] = pack_f16x2(bf16lo(v[i].w) * f, bf16hi(v[i].w) * f);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    mul[n][k] = __shfl_sync(0xffffffffu, undo, (2 * c + k) * 4) * p.scale_log2;
+                    limit[n][k] = len - p.n_q + 1 + min((cc * C + n * 8 + 2 * c + k) / p.group, p.n_q - 1);
+                }
+            }
+            const int full = len - p.n_q + 1;             // tokens that every column attends
+
+            for (int i = 0; i < n_tiles; ++i) {
+                cp_async_wait<kKv4Stages - 2>();
+                __syncwarp();
+                if (i + kKv4Stages - 1 < n_tiles) issue(i + kKv4Stages - 1, pa, pb);
+                cp_async_commit();
+                pa = lookup(token0(i + kKv4Stages)), pb = lookup(token0(i + kKv4Stages) + 8);
+                const uint32_t s = ring + (i % kKv4Stages) * kKv4StageBytes;
+                const int t0 = ((tile0 + i) * p.ts + tl) * 16;
+                if (t0 >= len) continue;
+
+                // ---- scores
+                float sc[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+                {
+                    const uint4 ka = lds128(s + lane * 16), kb = lds128(s + 512 + lane * 16);
+                    const uint32_t wa = lds32(s + 2048 + tau * 8 + (c >> 1) * 4), wb = lds32(s + 2048 + 64 + tau * 8 + (c >> 1) * 4);
+                    const uint32_t ha = e4m3x2_to_f16((wa >> ((c & 1) * 16)) & 0xffffu), hb = e4m3x2_to_f16((wb >> ((c & 1) * 16)) & 0xffffu);
+                    const uint32_t aw[4] = {ka.x, ka.y, ka.z, ka.w}, bw[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t sa = __byte_perm(ha, ha, k < 2 ? 0x1010 : 0x3232), sb = __byte_perm(hb, hb, k < 2 ? 0x1010 : 0x3232);
+                        uint32_t a[4], bq[4];
+                        e2m1x8_to_f16(aw[k], a);
+                        e2m1x8_to_f16(bw[k], bq);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) a[u] = hmul2_f16(a[u], sa), bq[u] = hmul2_f16(bq[u], sb);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma_f16(sc[n], a[0], bq[0], a[1], bq[1], qf[n][2 * k][0], qf[n][2 * k][1]);
+                            mma_f16(sc[n], a[2], bq[2], a[3], bq[3], qf[n][2 * k + 1][0], qf[n][2 * k + 1][1]);
+                        }
+                    }
+                }
+                bool rise = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) sc[n][k] *= mul[n][k & 1];
+                    if (t0 + 16 > full) {                 // a token that some column does not attend
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (t0 + tau + (k >> 1) * 8 >= limit[n][k & 1]) sc[n][k] = -INFINITY;
+                    }
+                    rise |= fmaxf(sc[n][0], sc[n][2]) > st.m[n][0] + kKv4Lag;
+                    rise |= fmaxf(sc[n][1], sc[n][3]) > st.m[n][1] + kKv4Lag;
+                }
+                if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            float top = fmaxf(sc[n][k], sc[n][k + 2]);
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                            const float m2 = fmaxf(st.m[n][k], top);
+                            const float f = m2 == st.m[n][k] ? 1.f : ex2_approx(st.m[n][k] - m2);
+                            st.m[n][k] = m2;
+                            st.l[n][k] *= f;
+#pragma unroll
+                            for (int d = 0; d < 8; ++d) st.o[d][n][k] *= f, st.o[d][n][k + 2] *= f;
+                        }
+                }
+                uint32_t pf[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float m0 = st.m[n][0] == -INFINITY ? 0.f : st.m[n][0], m1 = st.m[n][1] == -INFINITY ? 0.f : st.m[n][1];
+                    const float e0 = ex2_approx(sc[n][0] - m0), e1 = ex2_approx(sc[n][1] - m1), e2 = ex2_approx(sc[n][2] - m0), e3 = ex2_approx(sc[n][3] - m1);
+                    st.l[n][0] += e0 + e2;
+                    st.l[n][1] += e1 + e3;
+                    // Rows of the score tile become the k index of the second product: tokens c, c + 4 and c + 8, c + 12 of lane c.
+                    pf[n][0] = movmatrix_trans(pack_f16x2(e0, e1));
+                    pf[n][1] = movmatrix_trans(pack_f16x2(e2, e3));
+                }
+
+                // ---- O^T += V^T P^T: this lane has dimensions 16 g .. 16 g + 15 of tokens c, c + 4, c + 8, c + 12
+                {
+                    const uint32_t vp = s + 1024 + c * 64 + (((g >> 1) ^ (c & 2)) << 4) + (g & 1) * 8;
+                    const uint2 v0 = lds64(vp), v1 = lds64(vp + 256), v2 = lds64(vp + 512), v3 = lds64(vp + 768);
+                    const uint32_t sp = s + 2048 + 128 + c * 8 + g;
+                    const uint32_t sa = e4m3x2_to_f16(lds8(sp) | (lds8(sp + 32) << 8)), sb = e4m3x2_to_f16(lds8(sp + 64) | (lds8(sp + 96) << 8));
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t w0 = half ? v0.y : v0.x, w1 = half ? v1.y : v1.x, w2 = half ? v2.y : v2.x, w3 = half ? v3.y : v3.x;
+                        uint32_t a[2][4], bq[2][4];       // [even / odd dimensions][pair]
+                        e2m1x8_to_f16(bit_select(w0, w1 << 4, 0x0f0f0f0fu), a[0]);
+                        e2m1x8_to_f16(bit_select(w0 >> 4, w1, 0x0f0f0f0fu), a[1]);
+                        e2m1x8_to_f16(bit_select(w2, w3 << 4, 0x0f0f0f0fu), bq[0]);
+                        e2m1x8_to_f16(bit_select(w2 >> 4, w3, 0x0f0f0f0fu), bq[1]);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                const uint32_t a0 = hmul2_f16(a[q][2 * u], sa), a1 = hmul2_f16(a[q][2 * u + 1], sa);
+                                const uint32_t a2 = hmul2_f16(bq[q][2 * u], sb), a3 = hmul2_f16(bq[q][2 * u + 1], sb);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) mma_f16(st.o[half * 4 + q * 2 + u][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+                            }
+                    }
+                }
+            }
+            cp_async_wait<0>();
+            __syncwarp();
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    st.l[n][k] += __shfl_xor_sync(0xffffffffu, st.l[n][k], 4);
+                    st.l[n][k] += __shfl_xor_sync(0xffffffffu, st.l[n][k], 8);
+                    st.l[n][k] += __shfl_xor_sync(0xffffffffu, st.l[n][k], 16);
+                }
+        }
+        // ---- join the token lanes of a head (its ring is free by now)
+        if (p.ts > 1) {
+            if (active && tl > 0) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) stsf(ring + (((i * NT + n) * 4 + k) * 32 + lane) * 4, st.o[i][n][k]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        stsf(ring + ((32 * NT + n * 4 + k) * 32 + lane) * 4, st.m[n][k]);
+                        stsf(ring + ((32 * NT + n * 4 + 2 + k) * 32 + lane) * 4, st.l[n][k]);
+                    }
+            }
+            __syncthreads();
+            if (active && tl == 0) {
+                for (int t = 1; t < p.ts; ++t) {
+                    const uint32_t from = smem_u32(smem) + (t * p.hg + hl) * kKv4RingBytes;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const float om = ldsf(from + ((32 * NT + n * 4 + k) * 32 + lane) * 4), ol = ldsf(from + ((32 * NT + n * 4 + 2 + k) * 32 + lane) * 4);
+                            const float m2 = fmaxf(st.m[n][k], om);
+                            const float fa = st.m[n][k] == m2 ? 1.f : ex2_approx(st.m[n][k] - m2), fb = om == m2 ? 1.f : ex2_approx(om - m2);
+                            st.m[n][k] = m2;
+                            st.l[n][k] = st.l[n][k] * fa + ol * fb;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                st.o[i][n][k] = st.o[i][n][k] * fa + ldsf(from + (((i * NT + n) * 4 + k) * 32 + lane) * 4) * fb;
+                                st.o[i][n][k + 2] = st.o[i][n][k + 2] * fa + ldsf(from + (((i * NT + n) * 4 + k + 2) * 32 + lane) * 4) * fb;
+                            }
+                        }
+                }
+            }
+            __syncthreads();
+        }
+        if (active && tl == 0) {
+            // Dimension 16 g + d of column 2 c + k sits in st.o[(d >> 3) * 4 + (d & 1) * 2 + ((d >> 2) & 1)][n][k + (d & 2)].
+            const int slot = tile0 == 0 ? 1 : 0;          // of this block's two records: the segment that began before it, or the one that goes on
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int cl = n * 8 + 2 * c + k, col = cc * C + cl;
+                    if (col >= p.cols) continue;
+                    float v[16];
+#pragma unroll
+                    for (int d = 0; d < 16; ++d) v[d] = st.o[(d >> 3) * 4 + (d & 1) * 2 + ((d >> 2) & 1)][n][k + (d & 2)];
+                    const float l = st.l[n][k], m = st.m[n][k];
+                    if (whole) {
+                        const int j = col / p.group, h = kvh * p.group + (col - j * p.group);
+                        const long long at = static_cast<long long>(b) * p.n_q + j;
+                        const float inv = l == 0.f ? 0.f : p.v_scale / l;          // a not-a-number goes through
+                        uint4* dst = reinterpret_cast<uint4*>(p.out + at * p.out_stride + h * 128 + g * 16);
+                        dst[0] = make_uint4(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
+                                            pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
+                        dst[1] = make_uint4(pack_bf16x2(v[8] * inv, v[9] * inv), pack_bf16x2(v[10] * inv, v[11] * inv),
+                                            pack_bf16x2(v[12] * inv, v[13] * inv), pack_bf16x2(v[14] * inv, v[15] * inv));
+                        if (p.lse != nullptr && g == 0)
+                            p.lse[at * p.nh_q + h] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+                    } else {
+                        float* rec = p.rec + (((static_cast<long long>(blockIdx.x) * 2 + slot) * p.hg + hl) * C + cl) * kKv4RecFloats;
+                        float4* dst = reinterpret_cast<float4*>(rec + g * 16);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        if (g == 0) *reinterpret_cast<float2*>(rec + 128) = make_float2(m, l);
+                    }
+                }
+        }
+        x += n_tiles;
+    }
+}
+
+// Joins the records of the segments that more than one block had a part of: one block of 4 warps per output row.
+template <int NT>
+__global__ void __launch_bounds__(128) kv4_merge_kernel(const Kv4AttnParams p, int grid) {
+    constexpr int C = 8 * NT;
+    __shared__ float sm[4][130];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int h = blockIdx.x % p.nh_q, j = (blockIdx.x / p.nh_q) % p.n_q, b = blockIdx.x / (p.nh_q * p.n_q);
+    const int first = p.cum[b], tiles = p.cum[b + 1] - first, per_tile = p.n_hg * p.n_cc;
+    const long long total = static_cast<long long>(p.cum[p.batch]) * per_tile;
+    const int blocks = kv4_blocks(total, grid);
+    const int kvh = h / p.group, col = j * p.group + (h - kvh * p.group);
+    const int hgi = kvh / p.hg, hl = kvh - hgi * p.hg, cc = col / C, cl = col - cc * C;
+    const long long s0 = static_cast<long long>(first) * per_tile + static_cast<long long>(hgi * p.n_cc + cc) * tiles;
+    const int i0 = kv4_owner(total, s0, blocks), i1 = kv4_owner(total, s0 + tiles - 1, blocks);
+    if (i0 == i1) return;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = i0 + w; i <= i1; i += 4) {
+        // The segment's first block has it as the one that goes on behind its share; for the others it began before theirs.
+        const float* rec = p.rec + (((static_cast<long long>(i) * 2 + (i == i0 ? 1 : 0)) * p.hg + hl) * C + cl) * kKv4RecFloats;
+        const float4 v = *reinterpret_cast<const float4*>(rec + lane * 4);
+        const float2 ml = *reinterpret_cast<const float2*>(rec + 128);
+        const float m2 = fmaxf(m, ml.x);
+        const float fa = m == m2 ? 1.f : ex2_approx(m - m2), fb = ml.x == m2 ? 1.f : ex2_approx(ml.x - m2);
+        m = m2;
+        l = l * fa + ml.y * fb;
+        o.x = o.x * fa + v.x * fb, o.y = o.y * fa + v.y * fb, o.z = o.z * fa + v.z * fb, o.w = o.w * fa + v.w * fb;
+    }
+    *reinterpret_cast<float2*>(&sm[w][lane * 4]) = make_float2(o.x, o.y);
+    *reinterpret_cast<float2*>(&sm[w][lane * 4 + 2]) = make_float2(o.z, o.w);
     if (lane == 0) sm[w][128] = m, sm[w][129] = l;
     __syncthreads();
-    if (w != 0) return;
-    float top = -INFINITY;
+    const int d = threadIdx.x;
+    float top = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
     for (int i = 0; i < 4; ++i) top = fmaxf(top, sm[i][128]);
-    float total = 0.f, r[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if (sm[i][129] == 0.f) continue;
-        const float c = exp2f(sm[i][128] - top);
-        total += sm[i][129] * c;
-        for (int d = 0; d < 4; ++d) r[d] += sm[i][lane * 4 + d] * c;
+        const float f = sm[i][128] == top ? 1.f : ex2_approx(sm[i][128] - top);
+        sum += sm[i][129] * f;
+        acc += sm[i][d] * f;
     }
-    const float inv = total > 0.f ? p.v_scale / total : (total == 0.f ? 0.f : NAN);
+    const float inv = sum == 0.f ? 0.f : p.v_scale / sum;
     const long long at = static_cast<long long>(b) * p.n_q + j;
-    *reinterpret_cast<uint2*>(p.out + at * p.out_stride + h * 128 + lane * 4) =
-        make_uint2(pack_bf16x2(r[0] * inv, r[1] * inv), pack_bf16x2(r[2] * inv, r[3] * inv));
-    if (p.lse != nullptr && lane == 0)
-        p.lse[at * p.nh_q + h] = total > 0.f ? top * 0.6931471805599453f + logf(total) : (total == 0.f ? -INFINITY : NAN);
+    p.out[at * p.out_stride + h * 128 + d] = __float2bfloat16_rn(acc * inv);
+    if (p.lse != nullptr && d == 0) p.lse[at * p.nh_q + h] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
 }
 
 }  // namespace dkv

@@ -35,6 +35,53 @@ int check_kv4_pool(const dkv_context* ctx, const dkv_kv4_pool* pool) {
     return DKV_OK;
 }
 
+// Heads and token lanes of a block: as many of the 8 warps as the number of heads allows (7 will do), and of the shapes
+// that use them the one with the most heads side by side, whose rows of a token are one contiguous read.
+void kv4_block_shape(int nh_kv, int* hg, int* ts) {
+    int best = 0;
+    for (int h = 1; h <= kKv4Warps; ++h) {
+        if (nh_kv % h != 0) continue;
+        const int t = kKv4Warps / h, used = std::min(h * t, 7);
+        if (used >= best) best = used, *hg = h, *ts = t;
+    }
+}
+
+constexpr size_t kKv4CumBytes = (kKv4MaxBatch + 1) * sizeof(int) / 256 * 256 + 256;
+
+int kv4_grid(const dkv_context* ctx) { return ctx->sm_count * 2; }
+
+// One size for every call, so that any call (or registering a pool) makes room for all of them.
+size_t kv4_workspace(const dkv_context* ctx) {
+    return kKv4CumBytes + static_cast<size_t>(kv4_grid(ctx)) * 2 * kKv4Warps * 16 * kKv4RecFloats * sizeof(float);
+}
+
+template <int NT>
+int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
+    p.n_cc = (p.cols + 8 * NT - 1) / (8 * NT);
+    const int grid = kv4_grid(ctx);
+    const size_t smem = kKv4Warps * kKv4RingBytes + (p.batch + 1) * sizeof(int);
+    kv4_attn_kernel<NT><<<grid, kKv4Warps * 32, smem, st>>>(p);
+    DKV_CUDA(cudaGetLastError());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.n_q * p.nh_q);
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    DKV_CUDA(cudaLaunchKernelEx(&cfg, kv4_merge_kernel<NT>, p, grid));
+    ctx->launches += 2;
+    return DKV_OK;
+}
+
+template <int NT>
+cudaError_t kv4_set_attr() {
+    return cudaFuncSetAttribute(kv4_attn_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kKv4Warps * kKv4RingBytes + (kKv4MaxBatch + 1) * static_cast<int>(sizeof(int)));
+}
+
 }  // namespace
 
 extern "C" {
@@ -62,6 +109,10 @@ int dkv_kv4_pool_resolve(dkv_context* ctx, dkv_kv4_pool* pool) {
         int rc = device_pointer_of(*p, p, "a 4-bit pool");
         if (rc != DKV_OK) return rc;
     }
+    DKV_CUDA(kv4_set_attr<1>());
+    DKV_CUDA(kv4_set_attr<2>());
+    int rc = ensure_buffer(ctx, &ctx->kv4, kv4_workspace(ctx), false, "workspace of the 4-bit attention");
+    if (rc != DKV_OK) return rc;
     r.resolved = ctx->device + 1;
     *pool = r;
     return DKV_OK;
@@ -128,7 +179,7 @@ int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_
     int rc = check_kv4_pool(ctx, pool);
     if (rc != DKV_OK) return rc;
     if (a->batch == 0) return DKV_OK;
-    DKV_REQUIRE(a->batch > 0 && a->batch <= 4096, "batch (%d) must be 0..4096", a->batch);
+    DKV_REQUIRE(a->batch > 0 && a->batch <= kKv4MaxBatch, "batch (%d) must be 0..%d", a->batch, kKv4MaxBatch);
     DKV_REQUIRE(a->n_q >= 1 && a->n_q <= 1024, "query tokens per request (%d) must be 1..1024", a->n_q);
     DKV_REQUIRE(a->nh_q > 0 && a->nh_q % pool->nh_kv == 0, "nh_q (%d) must be a multiple of nh_kv (%d)", a->nh_q, pool->nh_kv);
     DKV_REQUIRE(a->q && a->out && a->seq_lens && a->page_table, "q / out / seq_lens / page_table must not be NULL");
@@ -156,13 +207,22 @@ int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_
     p.k_scales = static_cast<const uint8_t*>(pool->k_scales), p.v_scales = static_cast<const uint8_t*>(pool->v_scales);
     p.n_slots = pool->n_slots;
     p.batch = a->batch, p.n_q = a->n_q, p.nh_q = a->nh_q, p.nh_kv = pool->nh_kv;
+    p.group = a->nh_q / pool->nh_kv;
+    p.cols = a->n_q * p.group;
     p.scale_log2 = a->softmax_scale * pool->k_scale * 1.4426950408889634f;
     p.v_scale = pool->v_scale;
     p.status = ctx->status;
-    kv4_attn_kernel<<<dim3(a->nh_q, a->n_q, a->batch), 128, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    DKV_CUDA(cudaGetLastError());
-    ctx->launches += 1;
-    return DKV_OK;
+    DKV_REQUIRE(static_cast<int64_t>(a->batch) * a->n_q * a->nh_q <= INT32_MAX, "too many query rows");
+    DKV_REQUIRE((static_cast<int64_t>(p.max_pages) << p.page_shift) / 16 * a->batch < INT32_MAX, "%d requests of up to %lld tokens are too many for one call",
+                a->batch, static_cast<long long>(p.max_pages) << p.page_shift);
+    kv4_block_shape(pool->nh_kv, &p.hg, &p.ts);
+    p.n_hg = pool->nh_kv / p.hg;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    rc = ensure_buffer(ctx, &ctx->kv4, kv4_workspace(ctx), stream_is_capturing(st), "workspace of the 4-bit attention");
+    if (rc != DKV_OK) return rc;
+    p.cum = reinterpret_cast<int*>(ctx->kv4.ptr);
+    p.rec = reinterpret_cast<float*>(ctx->kv4.ptr + kKv4CumBytes);
+    return p.cols <= 8 ? launch_kv4_attn<1>(ctx, p, st) : launch_kv4_attn<2>(ctx, p, st);
 }
 
 int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* a, void* stream) {
