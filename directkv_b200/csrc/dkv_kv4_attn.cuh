@@ -22,11 +22,14 @@
 namespace dkv {
 
 constexpr int kKv4Warps = 8;
-constexpr int kKv4Stages = 4;
-constexpr int kKv4StageBytes = 2 * 1024 + 2 * 128;       // 16 tokens: K codes, V codes, K scales, V scales
+constexpr int kKv4Tile = 32;                             // tokens a warp takes in one step, as two halves of 16
+constexpr int kKv4Stages = 2;
+constexpr int kKv4HalfBytes = 2 * 1024 + 2 * 128;        // 16 tokens: K codes, V codes, K scales, V scales
+constexpr int kKv4StageBytes = 2 * kKv4HalfBytes;
 constexpr int kKv4RingBytes = kKv4Stages * kKv4StageBytes;
 constexpr int kKv4MaxBatch = 4096;
 constexpr int kKv4RecFloats = 132;                       // O[128], m (log2 domain), l, 2 pad
+constexpr float kKv4Low = -3e38f;                        // the running maximum before the first token
 constexpr float kKv4Lag = 8.f;                           // the maximum follows once a score is 2^8 above it: P <= 2^8 in fp16
 
 struct Kv4AttnParams {
@@ -47,6 +50,7 @@ struct Kv4AttnParams {
     const uint8_t* v_scales;
     long long n_slots;
     int page_shift;
+    int n_pages;                     // pages that begin inside the pool
     int batch, n_q, nh_q, nh_kv, group;
     int cols;                        // n_q * group: columns of one KV head
     int n_cc;                        // column chunks of 8 * NT
@@ -69,29 +73,6 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint32_t lds8(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ float ldsf(uint32_t a) { return __uint_as_float(lds32(a)); }
-__device__ __forceinline__ void stsf(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
-
 __device__ __forceinline__ uint32_t hmul2_f16(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -108,7 +89,7 @@ __device__ __forceinline__ uint32_t bit_select(uint32_t a, uint32_t b, uint32_t 
     return d;
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -140,7 +121,8 @@ struct Kv4State {
     float m[NT][2], l[NT][2];
 };
 
-template <int NT>
+// WIDE: pages of 16 tokens and more, so that 16 tokens lie in one page and one table entry serves the whole warp.
+template <int NT, bool WIDE>
 __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4AttnParams p) {
     constexpr int C = 8 * NT;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -149,7 +131,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int g = lane >> 2, c = lane & 3;
 
-    // Tiles (of 16 * ts tokens) before every request; a request without tokens has one, which writes its zeros.
+    // Tiles (of 32 * ts tokens) before every request; a request without tokens has one, which writes its zeros.
     if (threadIdx.x == 0) cum[0] = 0;
     int before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += kKv4Warps * 32) {
@@ -160,7 +142,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
             const int code = kv4_length(p, b, &row);
             if (code < 0 && blockIdx.x == 0) atomicOr(p.status, kStatusBadPage);
             const int len = kv4_clean_length(p, code);
-            n = max(1, static_cast<int>((static_cast<long long>(len) + 16 * p.ts - 1) / (16 * p.ts)));
+            n = max(1, static_cast<int>((static_cast<long long>(len) + kKv4Tile * p.ts - 1) / (kKv4Tile * p.ts)));
         }
         int inc = n;
 #pragma unroll
@@ -187,7 +169,8 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
 
     const int hl = w % p.hg, tl = w / p.hg;
     const bool active = tl < p.ts;
-    const uint32_t ring = smem_u32(smem) + w * kKv4RingBytes;
+    uint8_t* const ring_ptr = smem + w * kKv4RingBytes;
+    const uint32_t ring = smem_u32(ring_ptr);
     const int tau = (g >> 1) + 4 * (g & 1);          // token of this lane's rows of the score tile: tau and tau + 8
     const int page_mask = (1 << p.page_shift) - 1;
     Kv4State<NT> st;
@@ -221,41 +204,71 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
 #pragma unroll
                     for (int k = 0; k < 4; ++k) st.o[i][n][k] = 0.f;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) st.m[n][0] = st.m[n][1] = -INFINITY, st.l[n][0] = st.l[n][1] = 0.f;
+            for (int n = 0; n < NT; ++n) st.m[n][0] = st.m[n][1] = kKv4Low, st.l[n][0] = st.l[n][1] = 0.f;
 
-            // ---- copies: this lane brings 16 bytes of K and V of tokens tau and tau + 8, and 8 bytes of scales
-            auto lookup = [&](int t) { return t < len ? __ldg(table + (t >> p.page_shift)) : -1; };
-            auto slot_of = [&](int t, int page) -> long long {
-                if (t >= len) return -1;
-                const long long s = (static_cast<long long>(page) << p.page_shift) + (t & page_mask);
-                if (page < 0 || s >= p.n_slots) {
-                    atomicOr(p.status, kStatusBadPage);
-                    return -1;
-                }
-                return s;
-            };
-            auto token0 = [&](int i) { return ((tile0 + i) * p.ts + tl) * 16 + tau; };
-            auto issue = [&](int i, int pa, int pb) {
-                const uint32_t s = ring + (i % kKv4Stages) * kKv4StageBytes;
-                const int t = token0(i);
-                const long long sa = slot_of(t, pa), sb = slot_of(t + 8, pb);
-                const long long ra = sa < 0 ? 0 : sa * p.nh_kv + kvh, rb = sb < 0 ? 0 : sb * p.nh_kv + kvh;
-                const uint32_t na = sa < 0 ? 0u : 16u, nb = sb < 0 ? 0u : 16u;
-                cp_async16(s + lane * 16, p.k_codes + ra * 64 + c * 16, na);
-                cp_async16(s + 512 + lane * 16, p.k_codes + rb * 64 + c * 16, nb);
-                const uint32_t vq = s + 1024 + tau * 64 + ((c ^ ((g >> 1) & 2)) << 4);      // 16-byte pieces of rows 2, 3 mod 4 change places
-                cp_async16(vq, p.v_codes + ra * 64 + c * 16, na);
-                cp_async16(vq + 512, p.v_codes + rb * 64 + c * 16, nb);
-                const uint8_t* sc = (c & 2) ? p.v_scales : p.k_scales;
-                cp_async8(s + 2048 + (c & 2) * 64 + (tau + (c & 1) * 8) * 8, sc + ((c & 1) ? rb : ra) * 8, ((c & 1) ? nb : na) >> 1);
-            };
-            int pa = lookup(token0(0)), pb = lookup(token0(0) + 8);
+            // ---- copies: of every 16 tokens this lane brings 16 bytes of K and V of tokens tau and tau + 8, and 8 bytes of scales
+            const uint8_t* k_lane = p.k_codes + kvh * 64 + c * 16;
+            const uint8_t* v_lane = p.v_codes + kvh * 64 + c * 16;
+            const uint8_t* s_lane = ((c & 2) ? p.v_scales : p.k_scales) + kvh * 8;
+            const long long code_row = static_cast<long long>(p.nh_kv) * 64;
+            const uint32_t k_dst = ring + lane * 16;
+            const uint32_t v_dst = ring + 1024 + tau * 64 + ((c ^ ((g >> 1) & 2)) << 4);     // 16-byte pieces of rows 2, 3 mod 4 change places
+            const uint32_t s_dst = ring + 2048 + (c & 2) * 64 + (tau + (c & 1) * 8) * 8;
+            auto token0 = [&](int i) { return ((tile0 + i) * p.ts + tl) * kKv4Tile; };
+            // Table entries of a step: WIDE one for each half, else one for each of the lane's tokens.
+            int entry[WIDE ? 2 : 4];
+            auto lookup = [&](int i) {
+                const int t0 = token0(i) + (WIDE ? 0 : tau);
 #pragma unroll
-            for (int i = 0; i < kKv4Stages - 1; ++i) {
-                if (i < n_tiles) issue(i, pa, pb);
-                cp_async_commit();
-                pa = lookup(token0(i + 1)), pb = lookup(token0(i + 1) + 8);
-            }
+                for (int u = 0; u < (WIDE ? 2 : 4); ++u) {
+                    const int t = t0 + u * (WIDE ? 16 : 8);
+                    entry[u] = i < n_tiles && t < len ? __ldg(table + (t >> p.page_shift)) : 0;
+                }
+            };
+            auto issue = [&](int i) {
+                const int t0 = token0(i);
+                const uint32_t at = (i % kKv4Stages) * kKv4StageBytes;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int th = t0 + half * 16;
+                    if (th >= len) break;
+                    unsigned slot[2];
+                    bool ok[2], outside = false;
+                    if constexpr (WIDE) {
+                        const int e = entry[half];
+                        const bool known = static_cast<unsigned>(e) < static_cast<unsigned>(p.n_pages);
+                        const unsigned first = known ? (static_cast<unsigned>(e) << p.page_shift) + (th & page_mask) : 0u;
+                        const int room = known ? static_cast<int>(max(min(p.n_slots - first, 16ll), 0ll)) : 0;
+                        const int want = min(len - th, 16);
+                        outside = room < want;
+                        const int n = min(room, want);
+                        ok[0] = tau < n, ok[1] = tau + 8 < n;
+                        slot[0] = first + tau, slot[1] = first + tau + 8;
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int t = th + tau + u * 8, e = entry[half * 2 + u];
+                            const bool known = static_cast<unsigned>(e) < static_cast<unsigned>(p.n_pages);
+                            slot[u] = known ? (static_cast<unsigned>(e) << p.page_shift) + (t & page_mask) : 0u;
+                            ok[u] = known && t < len && slot[u] < p.n_slots;
+                            outside |= t < len && !ok[u];
+                        }
+                    }
+                    if (outside) atomicOr(p.status, kStatusBadPage);
+                    const uint32_t n0 = ok[0] ? 16u : 0u, n1 = ok[1] ? 16u : 0u;
+                    const long long r0 = ok[0] ? slot[0] * code_row : 0, r1 = ok[1] ? slot[1] * code_row : 0;
+                    const uint32_t h = at + half * kKv4HalfBytes;
+                    cp_async16(k_dst + h, k_lane + r0, n0);
+                    cp_async16(k_dst + h + 512, k_lane + r1, n1);
+                    cp_async16(v_dst + h, v_lane + r0, n0);
+                    cp_async16(v_dst + h + 512, v_lane + r1, n1);
+                    cp_async8(s_dst + h, s_lane + (((c & 1) ? r1 : r0) >> 3), ((c & 1) ? n1 : n0) >> 1);
+                }
+            };
+            lookup(0);
+            issue(0);
+            cp_async_commit();
+            lookup(1);
 
             // ---- queries: column g of each 8, dimensions 32 c .. 32 c + 31, as fp16 scaled by a power of two
             uint32_t qf[NT][8][2];
@@ -296,28 +309,33 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     mul[n][k] = __shfl_sync(0xffffffffu, undo, (2 * c + k) * 4) * p.scale_log2;
+                    if (mul[n][k] == 0.f) mul[n][k] = 1e-30f;                       // scores of zero all the same; masks need a sign
                     limit[n][k] = len - p.n_q + 1 + min((cc * C + n * 8 + 2 * c + k) / p.group, p.n_q - 1);
                 }
             }
             const int full = len - p.n_q + 1;             // tokens that every column attends
 
             for (int i = 0; i < n_tiles; ++i) {
-                cp_async_wait<kKv4Stages - 2>();
+                cp_async_wait<0>();
                 __syncwarp();
-                if (i + kKv4Stages - 1 < n_tiles) issue(i + kKv4Stages - 1, pa, pb);
+                if (i + 1 < n_tiles) issue(i + 1);
                 cp_async_commit();
-                pa = lookup(token0(i + kKv4Stages)), pb = lookup(token0(i + kKv4Stages) + 8);
-                const uint32_t s = ring + (i % kKv4Stages) * kKv4StageBytes;
-                const int t0 = ((tile0 + i) * p.ts + tl) * 16;
+                lookup(i + 2);
+                const uint8_t* s0 = ring_ptr + (i % kKv4Stages) * kKv4StageBytes;
+                const int t0 = token0(i);
                 if (t0 >= len) continue;
+                const int halves = t0 + 16 < len ? 2 : 1;
 
                 // ---- scores
-                float sc[NT][4];
+                float sc[2][NT][4];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-                {
-                    const uint4 ka = lds128(s + lane * 16), kb = lds128(s + 512 + lane * 16);
-                    const uint32_t wa = lds32(s + 2048 + tau * 8 + (c >> 1) * 4), wb = lds32(s + 2048 + 64 + tau * 8 + (c >> 1) * 4);
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) sc[half][n][0] = sc[half][n][1] = sc[half][n][2] = sc[half][n][3] = 0.f;
+                    if (half >= halves) break;
+                    const uint8_t* s = s0 + half * kKv4HalfBytes;
+                    const uint4 ka = *reinterpret_cast<const uint4*>(s + lane * 16), kb = *reinterpret_cast<const uint4*>(s + 512 + lane * 16);
+                    const uint32_t wa = *reinterpret_cast<const uint32_t*>(s + 2048 + tau * 8 + (c >> 1) * 4), wb = *reinterpret_cast<const uint32_t*>(s + 2048 + 64 + tau * 8 + (c >> 1) * 4);
                     const uint32_t ha = e4m3x2_to_f16((wa >> ((c & 1) * 16)) & 0xffffu), hb = e4m3x2_to_f16((wb >> ((c & 1) * 16)) & 0xffffu);
                     const uint32_t aw[4] = {ka.x, ka.y, ka.z, ka.w}, bw[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
@@ -330,30 +348,38 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                         for (int u = 0; u < 4; ++u) a[u] = hmul2_f16(a[u], sa), bq[u] = hmul2_f16(bq[u], sb);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma_f16(sc[n], a[0], bq[0], a[1], bq[1], qf[n][2 * k][0], qf[n][2 * k][1]);
-                            mma_f16(sc[n], a[2], bq[2], a[3], bq[3], qf[n][2 * k + 1][0], qf[n][2 * k + 1][1]);
+                            mma_f16(sc[half][n], a[0], bq[0], a[1], bq[1], qf[n][2 * k][0], qf[n][2 * k][1]);
+                            mma_f16(sc[half][n], a[2], bq[2], a[3], bq[3], qf[n][2 * k + 1][0], qf[n][2 * k + 1][1]);
                         }
                     }
                 }
+                if (t0 + kKv4Tile > full) {               // a token that some column does not attend: its score becomes -inf
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (t0 + half * 16 + tau + (k >> 1) * 8 >= limit[n][k & 1]) sc[half][n][k] = copysignf(INFINITY, -mul[n][k & 1]);
+                }
+                float e[2][NT][4];
                 bool rise = false;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) sc[n][k] *= mul[n][k & 1];
-                    if (t0 + 16 > full) {                 // a token that some column does not attend
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (t0 + tau + (k >> 1) * 8 >= limit[n][k & 1]) sc[n][k] = -INFINITY;
-                    }
-                    rise |= fmaxf(sc[n][0], sc[n][2]) > st.m[n][0] + kKv4Lag;
-                    rise |= fmaxf(sc[n][1], sc[n][3]) > st.m[n][1] + kKv4Lag;
-                }
+                        for (int k = 0; k < 4; ++k) {
+                            e[half][n][k] = fmaf(sc[half][n][k], mul[n][k & 1], -st.m[n][k & 1]);
+                            rise |= e[half][n][k] > kKv4Lag;
+                        }
                 if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            float top = fmaxf(sc[n][k], sc[n][k + 2]);
+                            const float u = mul[n][k];
+                            float top = fmaxf(fmaxf(sc[0][n][k] * u, sc[0][n][k + 2] * u), fmaxf(sc[1][n][k] * u, sc[1][n][k + 2] * u));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -363,29 +389,34 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                             st.l[n][k] *= f;
 #pragma unroll
                             for (int d = 0; d < 8; ++d) st.o[d][n][k] *= f, st.o[d][n][k + 2] *= f;
+#pragma unroll
+                            for (int half = 0; half < 2; ++half)
+                                e[half][n][k] = fmaf(sc[half][n][k], u, -m2), e[half][n][k + 2] = fmaf(sc[half][n][k + 2], u, -m2);
                         }
                 }
-                uint32_t pf[NT][2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float m0 = st.m[n][0] == -INFINITY ? 0.f : st.m[n][0], m1 = st.m[n][1] == -INFINITY ? 0.f : st.m[n][1];
-                    const float e0 = ex2_approx(sc[n][0] - m0), e1 = ex2_approx(sc[n][1] - m1), e2 = ex2_approx(sc[n][2] - m0), e3 = ex2_approx(sc[n][3] - m1);
-                    st.l[n][0] += e0 + e2;
-                    st.l[n][1] += e1 + e3;
-                    // Rows of the score tile become the k index of the second product: tokens c, c + 4 and c + 8, c + 12 of lane c.
-                    pf[n][0] = movmatrix_trans(pack_f16x2(e0, e1));
-                    pf[n][1] = movmatrix_trans(pack_f16x2(e2, e3));
-                }
+                for (int half = 0; half < 2; ++half) {
+                    if (half >= halves) break;
+                    uint32_t pf[NT][2];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float e0 = ex2_approx(e[half][n][0]), e1 = ex2_approx(e[half][n][1]), e2 = ex2_approx(e[half][n][2]), e3 = ex2_approx(e[half][n][3]);
+                        st.l[n][0] += e0 + e2;
+                        st.l[n][1] += e1 + e3;
+                        // Rows of the score tile become the k index of the second product: tokens c, c + 4 and c + 8, c + 12 of lane c.
+                        pf[n][0] = movmatrix_trans(pack_f16x2(e0, e1));
+                        pf[n][1] = movmatrix_trans(pack_f16x2(e2, e3));
+                    }
 
-                // ---- O^T += V^T P^T: this lane has dimensions 16 g .. 16 g + 15 of tokens c, c + 4, c + 8, c + 12
-                {
-                    const uint32_t vp = s + 1024 + c * 64 + (((g >> 1) ^ (c & 2)) << 4) + (g & 1) * 8;
-                    const uint2 v0 = lds64(vp), v1 = lds64(vp + 256), v2 = lds64(vp + 512), v3 = lds64(vp + 768);
-                    const uint32_t sp = s + 2048 + 128 + c * 8 + g;
-                    const uint32_t sa = e4m3x2_to_f16(lds8(sp) | (lds8(sp + 32) << 8)), sb = e4m3x2_to_f16(lds8(sp + 64) | (lds8(sp + 96) << 8));
+                    // ---- O^T += V^T P^T: this lane has dimensions 16 g .. 16 g + 15 of tokens c, c + 4, c + 8, c + 12
+                    const uint8_t* s = s0 + half * kKv4HalfBytes;
+                    const uint8_t* vp = s + 1024 + c * 64 + (((g >> 1) ^ (c & 2)) << 4) + (g & 1) * 8;
+                    const uint2 v0 = *reinterpret_cast<const uint2*>(vp), v1 = *reinterpret_cast<const uint2*>(vp + 256), v2 = *reinterpret_cast<const uint2*>(vp + 512), v3 = *reinterpret_cast<const uint2*>(vp + 768);
+                    const uint8_t* sp = s + 2048 + 128 + c * 8 + g;
+                    const uint32_t sa = e4m3x2_to_f16(sp[0] | (static_cast<uint32_t>(sp[32]) << 8)), sb = e4m3x2_to_f16(sp[64] | (static_cast<uint32_t>(sp[96]) << 8));
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint32_t w0 = half ? v0.y : v0.x, w1 = half ? v1.y : v1.x, w2 = half ? v2.y : v2.x, w3 = half ? v3.y : v3.x;
+                    for (int word = 0; word < 2; ++word) {
+                        const uint32_t w0 = word ? v0.y : v0.x, w1 = word ? v1.y : v1.x, w2 = word ? v2.y : v2.x, w3 = word ? v3.y : v3.x;
                         uint32_t a[2][4], bq[2][4];       // [even / odd dimensions][pair]
                         e2m1x8_to_f16(bit_select(w0, w1 << 4, 0x0f0f0f0fu), a[0]);
                         e2m1x8_to_f16(bit_select(w0 >> 4, w1, 0x0f0f0f0fu), a[1]);
@@ -398,7 +429,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                                 const uint32_t a0 = hmul2_f16(a[q][2 * u], sa), a1 = hmul2_f16(a[q][2 * u + 1], sa);
                                 const uint32_t a2 = hmul2_f16(bq[q][2 * u], sb), a3 = hmul2_f16(bq[q][2 * u + 1], sb);
 #pragma unroll
-                                for (int n = 0; n < NT; ++n) mma_f16(st.o[half * 4 + q * 2 + u][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+                                for (int n = 0; n < NT; ++n) mma_f16(st.o[word * 4 + q * 2 + u][n], a0, a1, a2, a3, pf[n][0], pf[n][1]);
                             }
                     }
                 }
@@ -422,32 +453,32 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) stsf(ring + (((i * NT + n) * 4 + k) * 32 + lane) * 4, st.o[i][n][k]);
+                        for (int k = 0; k < 4; ++k) reinterpret_cast<float*>(ring_ptr)[(((i * NT + n) * 4 + k) * 32 + lane)] = st.o[i][n][k];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        stsf(ring + ((32 * NT + n * 4 + k) * 32 + lane) * 4, st.m[n][k]);
-                        stsf(ring + ((32 * NT + n * 4 + 2 + k) * 32 + lane) * 4, st.l[n][k]);
+                        reinterpret_cast<float*>(ring_ptr)[((32 * NT + n * 4 + k) * 32 + lane)] = st.m[n][k];
+                        reinterpret_cast<float*>(ring_ptr)[((32 * NT + n * 4 + 2 + k) * 32 + lane)] = st.l[n][k];
                     }
             }
             __syncthreads();
             if (active && tl == 0) {
                 for (int t = 1; t < p.ts; ++t) {
-                    const uint32_t from = smem_u32(smem) + (t * p.hg + hl) * kKv4RingBytes;
+                    const float* from = reinterpret_cast<const float*>(smem + (t * p.hg + hl) * kKv4RingBytes);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            const float om = ldsf(from + ((32 * NT + n * 4 + k) * 32 + lane) * 4), ol = ldsf(from + ((32 * NT + n * 4 + 2 + k) * 32 + lane) * 4);
+                            const float om = from[((32 * NT + n * 4 + k) * 32 + lane)], ol = from[((32 * NT + n * 4 + 2 + k) * 32 + lane)];
                             const float m2 = fmaxf(st.m[n][k], om);
                             const float fa = st.m[n][k] == m2 ? 1.f : ex2_approx(st.m[n][k] - m2), fb = om == m2 ? 1.f : ex2_approx(om - m2);
                             st.m[n][k] = m2;
                             st.l[n][k] = st.l[n][k] * fa + ol * fb;
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                st.o[i][n][k] = st.o[i][n][k] * fa + ldsf(from + (((i * NT + n) * 4 + k) * 32 + lane) * 4) * fb;
-                                st.o[i][n][k + 2] = st.o[i][n][k + 2] * fa + ldsf(from + (((i * NT + n) * 4 + k + 2) * 32 + lane) * 4) * fb;
+                                st.o[i][n][k] = st.o[i][n][k] * fa + from[(((i * NT + n) * 4 + k) * 32 + lane)] * fb;
+                                st.o[i][n][k + 2] = st.o[i][n][k + 2] * fa + from[(((i * NT + n) * 4 + k + 2) * 32 + lane)] * fb;
                             }
                         }
                 }
@@ -491,11 +522,14 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
     }
 }
 
-// Joins the records of the segments that more than one block had a part of: one block of 4 warps per output row.
-template <int NT>
-__global__ void __launch_bounds__(128) kv4_merge_kernel(const Kv4AttnParams p, int grid) {
+// Joins the records of the segments that more than one block had a part of: one block of NW warps per output row.  The
+// weights of all parts come first (one load of maximum and sum per thread), so that the loads of O depend on nothing.
+template <int NT, int NW>
+__global__ void __launch_bounds__(NW * 32) kv4_merge_kernel(const Kv4AttnParams p, int grid) {
     constexpr int C = 8 * NT;
-    __shared__ float sm[4][130];
+    extern __shared__ __align__(16) uint8_t smem[];
+    float2* ml = reinterpret_cast<float2*>(smem);                         // [grid]
+    __shared__ float part[NW][128];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int h = blockIdx.x % p.nh_q, j = (blockIdx.x / p.nh_q) % p.n_q, b = blockIdx.x / (p.nh_q * p.n_q);
@@ -505,35 +539,35 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const Kv4AttnParams p, i
     const int kvh = h / p.group, col = j * p.group + (h - kvh * p.group);
     const int hgi = kvh / p.hg, hl = kvh - hgi * p.hg, cc = col / C, cl = col - cc * C;
     const long long s0 = static_cast<long long>(first) * per_tile + static_cast<long long>(hgi * p.n_cc + cc) * tiles;
-    const int i0 = kv4_owner(total, s0, blocks), i1 = kv4_owner(total, s0 + tiles - 1, blocks);
-    if (i0 == i1) return;
-    float m = -INFINITY, l = 0.f;
+    const int i0 = kv4_owner(total, s0, blocks), n = kv4_owner(total, s0 + tiles - 1, blocks) - i0 + 1;
+    if (n == 1) return;
+    // The segment's first block has it as the one that goes on behind its share; for the others it began before theirs.
+    const long long step = 2ll * p.hg * C * kKv4RecFloats;
+    const float* rec0 = p.rec + ((static_cast<long long>(i0) * 2 * p.hg + hl) * C + cl) * kKv4RecFloats;
+    const long long goes_on = static_cast<long long>(p.hg) * C * kKv4RecFloats;
+    for (int i = threadIdx.x; i < n; i += NW * 32) ml[i] = *reinterpret_cast<const float2*>(rec0 + i * step + (i == 0 ? goes_on : 0) + 128);
+    __syncthreads();
+    float top = kKv4Low, sum = 0.f;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, ml[i].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i = lane; i < n; i += 32) sum += ml[i].y * ex2_approx(ml[i].x - top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = i0 + w; i <= i1; i += 4) {
-        // The segment's first block has it as the one that goes on behind its share; for the others it began before theirs.
-        const float* rec = p.rec + (((static_cast<long long>(i) * 2 + (i == i0 ? 1 : 0)) * p.hg + hl) * C + cl) * kKv4RecFloats;
-        const float4 v = *reinterpret_cast<const float4*>(rec + lane * 4);
-        const float2 ml = *reinterpret_cast<const float2*>(rec + 128);
-        const float m2 = fmaxf(m, ml.x);
-        const float fa = m == m2 ? 1.f : ex2_approx(m - m2), fb = ml.x == m2 ? 1.f : ex2_approx(ml.x - m2);
-        m = m2;
-        l = l * fa + ml.y * fb;
-        o.x = o.x * fa + v.x * fb, o.y = o.y * fa + v.y * fb, o.z = o.z * fa + v.z * fb, o.w = o.w * fa + v.w * fb;
+#pragma unroll 4
+    for (int i = w; i < n; i += NW) {
+        const float4 v = *reinterpret_cast<const float4*>(rec0 + i * step + (i == 0 ? goes_on : 0) + lane * 4);
+        const float f = ex2_approx(ml[i].x - top);
+        o.x += v.x * f, o.y += v.y * f, o.z += v.z * f, o.w += v.w * f;
     }
-    *reinterpret_cast<float2*>(&sm[w][lane * 4]) = make_float2(o.x, o.y);
-    *reinterpret_cast<float2*>(&sm[w][lane * 4 + 2]) = make_float2(o.z, o.w);
-    if (lane == 0) sm[w][128] = m, sm[w][129] = l;
+    *reinterpret_cast<float4*>(&part[w][lane * 4]) = o;
     __syncthreads();
     const int d = threadIdx.x;
-    float top = -INFINITY, sum = 0.f, acc = 0.f;
+    if (d >= 128) return;
+    float acc = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = fmaxf(top, sm[i][128]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float f = sm[i][128] == top ? 1.f : ex2_approx(sm[i][128] - top);
-        sum += sm[i][129] * f;
-        acc += sm[i][d] * f;
-    }
+    for (int i = 0; i < NW; ++i) acc += part[i][d];
     const float inv = sum == 0.f ? 0.f : p.v_scale / sum;
     const long long at = static_cast<long long>(b) * p.n_q + j;
     p.out[at * p.out_stride + h * 128 + d] = __float2bfloat16_rn(acc * inv);

@@ -60,25 +60,30 @@ int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
     p.n_cc = (p.cols + 8 * NT - 1) / (8 * NT);
     const int grid = kv4_grid(ctx);
     const size_t smem = kKv4Warps * kKv4RingBytes + (p.batch + 1) * sizeof(int);
-    kv4_attn_kernel<NT><<<grid, kKv4Warps * 32, smem, st>>>(p);
+    if (p.page_shift >= 4) kv4_attn_kernel<NT, true><<<grid, kKv4Warps * 32, smem, st>>>(p);
+    else kv4_attn_kernel<NT, false><<<grid, kKv4Warps * 32, smem, st>>>(p);
     DKV_CUDA(cudaGetLastError());
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.n_q * p.nh_q);
-    cfg.blockDim = dim3(128);
+    // Few rows: many blocks had a part of each.
+    const bool few = cfg.gridDim.x <= static_cast<unsigned>(2 * ctx->sm_count);
+    cfg.blockDim = dim3(few ? 512 : 128);
+    cfg.dynamicSmemBytes = grid * sizeof(float2);
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    DKV_CUDA(cudaLaunchKernelEx(&cfg, kv4_merge_kernel<NT>, p, grid));
+    if (few) DKV_CUDA(cudaLaunchKernelEx(&cfg, kv4_merge_kernel<NT, 16>, p, grid));
+    else DKV_CUDA(cudaLaunchKernelEx(&cfg, kv4_merge_kernel<NT, 4>, p, grid));
     ctx->launches += 2;
     return DKV_OK;
 }
 
-template <int NT>
+template <int NT, bool WIDE>
 cudaError_t kv4_set_attr() {
-    return cudaFuncSetAttribute(kv4_attn_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(kv4_attn_kernel<NT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 kKv4Warps * kKv4RingBytes + (kKv4MaxBatch + 1) * static_cast<int>(sizeof(int)));
 }
 
@@ -109,8 +114,10 @@ int dkv_kv4_pool_resolve(dkv_context* ctx, dkv_kv4_pool* pool) {
         int rc = device_pointer_of(*p, p, "a 4-bit pool");
         if (rc != DKV_OK) return rc;
     }
-    DKV_CUDA(kv4_set_attr<1>());
-    DKV_CUDA(kv4_set_attr<2>());
+    DKV_CUDA((kv4_set_attr<1, false>()));
+    DKV_CUDA((kv4_set_attr<1, true>()));
+    DKV_CUDA((kv4_set_attr<2, false>()));
+    DKV_CUDA((kv4_set_attr<2, true>()));
     int rc = ensure_buffer(ctx, &ctx->kv4, kv4_workspace(ctx), false, "workspace of the 4-bit attention");
     if (rc != DKV_OK) return rc;
     r.resolved = ctx->device + 1;
@@ -206,6 +213,7 @@ int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_
     p.k_codes = static_cast<const uint8_t*>(pool->k_codes), p.v_codes = static_cast<const uint8_t*>(pool->v_codes);
     p.k_scales = static_cast<const uint8_t*>(pool->k_scales), p.v_scales = static_cast<const uint8_t*>(pool->v_scales);
     p.n_slots = pool->n_slots;
+    p.n_pages = static_cast<int>((pool->n_slots + pool->page_size - 1) / pool->page_size);
     p.batch = a->batch, p.n_q = a->n_q, p.nh_q = a->nh_q, p.nh_kv = pool->nh_kv;
     p.group = a->nh_q / pool->nh_kv;
     p.cols = a->n_q * p.group;
