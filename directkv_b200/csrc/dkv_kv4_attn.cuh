@@ -207,68 +207,69 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
             for (int n = 0; n < NT; ++n) st.m[n][0] = st.m[n][1] = kKv4Low, st.l[n][0] = st.l[n][1] = 0.f;
 
             // ---- copies: of every 16 tokens this lane brings 16 bytes of K and V of tokens tau and tau + 8, and 8 bytes of scales
-            const uint8_t* k_lane = p.k_codes + kvh * 64 + c * 16;
-            const uint8_t* v_lane = p.v_codes + kvh * 64 + c * 16;
-            const uint8_t* s_lane = ((c & 2) ? p.v_scales : p.k_scales) + kvh * 8;
             const long long code_row = static_cast<long long>(p.nh_kv) * 64;
+            const uint8_t* k_lane = p.k_codes + kvh * 64 + c * 16 + (WIDE ? tau * code_row : 0);
+            const uint8_t* v_lane = p.v_codes + kvh * 64 + c * 16 + (WIDE ? tau * code_row : 0);
+            const int s_tau = tau + (c & 1) * 8;
+            const uint8_t* s_lane = ((c & 2) ? p.v_scales : p.k_scales) + kvh * 8 + (WIDE ? s_tau * (code_row >> 3) : 0);
             const uint32_t k_dst = ring + lane * 16;
             const uint32_t v_dst = ring + 1024 + tau * 64 + ((c ^ ((g >> 1) & 2)) << 4);     // 16-byte pieces of rows 2, 3 mod 4 change places
-            const uint32_t s_dst = ring + 2048 + (c & 2) * 64 + (tau + (c & 1) * 8) * 8;
+            const uint32_t s_dst = ring + 2048 + (c & 2) * 64 + s_tau * 8;
             auto token0 = [&](int i) { return ((tile0 + i) * p.ts + tl) * kKv4Tile; };
-            // Table entries of a step: WIDE one for each half, else one for each of the lane's tokens.
-            int entry[WIDE ? 2 : 4];
-            auto lookup = [&](int i) {
-                const int t0 = token0(i) + (WIDE ? 0 : tau);
-#pragma unroll
-                for (int u = 0; u < (WIDE ? 2 : 4); ++u) {
-                    const int t = t0 + u * (WIDE ? 16 : 8);
-                    entry[u] = i < n_tiles && t < len ? __ldg(table + (t >> p.page_shift)) : 0;
+            // Slots, looked up by the lanes together and handed round: WIDE the first slot of a half (lane l of a batch of
+            // 16 steps has half l), else every token's (lane l of a step has token l).  -1: behind the length, or no page.
+            int now = -1, next;
+            auto look = [&](int i) {
+                const int step = WIDE ? i + (lane >> 1) : i;
+                const int t = token0(step) + (WIDE ? (lane & 1) * 16 : lane);
+                int slot = -1;
+                if (step < n_tiles && t < len) {
+                    const int e = __ldg(table + (t >> p.page_shift));
+                    if (static_cast<unsigned>(e) < static_cast<unsigned>(p.n_pages)) slot = (e << p.page_shift) + (t & page_mask);
+                    else atomicOr(p.status, kStatusBadPage);
                 }
+                return slot;
             };
             auto issue = [&](int i) {
-                const int t0 = token0(i);
-                const uint32_t at = (i % kKv4Stages) * kKv4StageBytes;
+                if (!WIDE || (i & 15) == 0) {
+                    now = next;
+                    next = look(i + (WIDE ? 16 : 1));
+                }
+                const uint32_t at = (i & (kKv4Stages - 1)) * kKv4StageBytes;
+                const int left = len - token0(i);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int th = t0 + half * 16;
-                    if (th >= len) break;
-                    unsigned slot[2];
-                    bool ok[2], outside = false;
-                    if constexpr (WIDE) {
-                        const int e = entry[half];
-                        const bool known = static_cast<unsigned>(e) < static_cast<unsigned>(p.n_pages);
-                        const unsigned first = known ? (static_cast<unsigned>(e) << p.page_shift) + (th & page_mask) : 0u;
-                        const int room = known ? static_cast<int>(max(min(p.n_slots - first, 16ll), 0ll)) : 0;
-                        const int want = min(len - th, 16);
-                        outside = room < want;
-                        const int n = min(room, want);
-                        ok[0] = tau < n, ok[1] = tau + 8 < n;
-                        slot[0] = first + tau, slot[1] = first + tau + 8;
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const int t = th + tau + u * 8, e = entry[half * 2 + u];
-                            const bool known = static_cast<unsigned>(e) < static_cast<unsigned>(p.n_pages);
-                            slot[u] = known ? (static_cast<unsigned>(e) << p.page_shift) + (t & page_mask) : 0u;
-                            ok[u] = known && t < len && slot[u] < p.n_slots;
-                            outside |= t < len && !ok[u];
-                        }
-                    }
-                    if (outside) atomicOr(p.status, kStatusBadPage);
-                    const uint32_t n0 = ok[0] ? 16u : 0u, n1 = ok[1] ? 16u : 0u;
-                    const long long r0 = ok[0] ? slot[0] * code_row : 0, r1 = ok[1] ? slot[1] * code_row : 0;
+                    if (half * 16 >= left) break;
                     const uint32_t h = at + half * kKv4HalfBytes;
-                    cp_async16(k_dst + h, k_lane + r0, n0);
-                    cp_async16(k_dst + h + 512, k_lane + r1, n1);
-                    cp_async16(v_dst + h, v_lane + r0, n0);
-                    cp_async16(v_dst + h + 512, v_lane + r1, n1);
-                    cp_async8(s_dst + h, s_lane + (((c & 1) ? r1 : r0) >> 3), ((c & 1) ? n1 : n0) >> 1);
+                    uint32_t n0, n1;
+                    const uint8_t *k0, *k1, *v0, *v1, *sp;
+                    if constexpr (WIDE) {
+                        // A page lies in the pool as a whole: rows behind the length may be addressed, but are not read.
+                        const int slot = __shfl_sync(0xffffffffu, now, (2 * i + half) & 31);
+                        const int n = slot < 0 ? 0 : left - half * 16;
+                        const long long first = static_cast<long long>(max(slot, 0)) * code_row;
+                        n0 = tau < n ? 16u : 0u, n1 = tau + 8 < n ? 16u : 0u;
+                        k0 = k_lane + first, k1 = k0 + 8 * code_row;
+                        v0 = v_lane + first, v1 = v0 + 8 * code_row;
+                        sp = s_lane + (first >> 3);
+                    } else {
+                        const int a = __shfl_sync(0xffffffffu, now, half * 16 + tau), b8 = __shfl_sync(0xffffffffu, now, half * 16 + tau + 8);
+                        n0 = a < 0 ? 0u : 16u, n1 = b8 < 0 ? 0u : 16u;
+                        const long long ra = max(a, 0) * code_row, rb = max(b8, 0) * code_row;
+                        k0 = k_lane + ra, k1 = k_lane + rb;
+                        v0 = v_lane + ra, v1 = v_lane + rb;
+                        sp = s_lane + (((c & 1) ? rb : ra) >> 3);
+                    }
+                    cp_async16(k_dst + h, k0, n0);
+                    cp_async16(k_dst + h + 512, k1, n1);
+                    cp_async16(v_dst + h, v0, n0);
+                    cp_async16(v_dst + h + 512, v1, n1);
+                    cp_async8(s_dst + h, sp, ((c & 1) ? n1 : n0) >> 1);
                 }
             };
-            lookup(0);
+            next = look(0);
             issue(0);
             cp_async_commit();
-            lookup(1);
 
             // ---- queries: column g of each 8, dimensions 32 c .. 32 c + 31, as fp16 scaled by a power of two
             uint32_t qf[NT][8][2];
@@ -320,8 +321,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                 __syncwarp();
                 if (i + 1 < n_tiles) issue(i + 1);
                 cp_async_commit();
-                lookup(i + 2);
-                const uint8_t* s0 = ring_ptr + (i % kKv4Stages) * kKv4StageBytes;
+                const uint8_t* s0 = ring_ptr + (i & (kKv4Stages - 1)) * kKv4StageBytes;
                 const int t0 = token0(i);
                 if (t0 >= len) continue;
                 const int halves = t0 + 16 < len ? 2 : 1;
@@ -363,17 +363,16 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                                 if (t0 + half * 16 + tau + (k >> 1) * 8 >= limit[n][k & 1]) sc[half][n][k] = copysignf(INFINITY, -mul[n][k & 1]);
                 }
                 float e[2][NT][4];
-                bool rise = false;
+                float high = kKv4Low;
 #pragma unroll
-                for (int half = 0; half < 2; ++half)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            e[half][n][k] = fmaf(sc[half][n][k], mul[n][k & 1], -st.m[n][k & 1]);
-                            rise |= e[half][n][k] > kKv4Lag;
-                        }
-                if (__any_sync(0xffffffffu, rise)) {
+                    for (int k = 0; k < 4; ++k) {
+                        e[0][n][k] = fmaf(sc[0][n][k], mul[n][k & 1], -st.m[n][k & 1]);
+                        e[1][n][k] = fmaf(sc[1][n][k], mul[n][k & 1], -st.m[n][k & 1]);
+                        high = fmax3(high, e[0][n][k], e[1][n][k]);
+                    }
+                if (__any_sync(0xffffffffu, high > kKv4Lag)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll

@@ -66,7 +66,8 @@ int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.n_q * p.nh_q);
     // Few rows: many blocks had a part of each.
-    const bool few = cfg.gridDim.x <= static_cast<unsigned>(2 * ctx->sm_count);
+    const int64_t most_parts = (static_cast<int64_t>(p.max_pages) << p.page_shift) / (kKv4Tile * p.ts) + 1;
+    const bool few = cfg.gridDim.x <= static_cast<unsigned>(2 * ctx->sm_count) && most_parts > 16;
     cfg.blockDim = dim3(few ? 512 : 128);
     cfg.dynamicSmemBytes = grid * sizeof(float2);
     cfg.stream = st;
@@ -97,6 +98,7 @@ int dkv_kv4_pool_resolve(dkv_context* ctx, dkv_kv4_pool* pool) {
     DKV_REQUIRE(pool->n_slots > 0 && pool->n_slots <= INT32_MAX && pool->nh_kv > 0 && pool->nh_kv <= 65535,
                 "n_slots must be 1..2^31-1 and nh_kv 1..65535");
     DKV_REQUIRE(pool->page_size >= 1 && (pool->page_size & (pool->page_size - 1)) == 0, "page_size (%d) must be a power of two", pool->page_size);
+    DKV_REQUIRE(pool->n_slots % pool->page_size == 0, "n_slots (%lld) must be a multiple of page_size (%d)", (long long)pool->n_slots, pool->page_size);
     for (float s : {pool->k_scale, pool->v_scale}) {
         int e = 0;
         DKV_REQUIRE(s > 0.f && frexpf(s, &e) == 0.5f && e >= -23 && e <= 25, "pool scales must be powers of two from 2^-24 to 2^24");
@@ -213,7 +215,7 @@ int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_
     p.k_codes = static_cast<const uint8_t*>(pool->k_codes), p.v_codes = static_cast<const uint8_t*>(pool->v_codes);
     p.k_scales = static_cast<const uint8_t*>(pool->k_scales), p.v_scales = static_cast<const uint8_t*>(pool->v_scales);
     p.n_slots = pool->n_slots;
-    p.n_pages = static_cast<int>((pool->n_slots + pool->page_size - 1) / pool->page_size);
+    p.n_pages = static_cast<int>(pool->n_slots / pool->page_size);
     p.batch = a->batch, p.n_q = a->n_q, p.nh_q = a->nh_q, p.nh_kv = pool->nh_kv;
     p.group = a->nh_q / pool->nh_kv;
     p.cols = a->n_q * p.group;

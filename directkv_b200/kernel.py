@@ -432,6 +432,7 @@ class KV4Pool:
             _chk(t.device == k_codes.device, f"{name} must be on the device of k_codes")
             _chk(t.is_cuda or t.is_pinned() or not torch.cuda.is_available(), f"{name} must be in pinned memory (or a CUDA tensor)")
         _chk(page_size >= 1 and page_size & (page_size - 1) == 0, f"page_size ({page_size}) must be a power of two")
+        _chk(n_slots > 0 and n_slots % page_size == 0, f"the number of slots ({n_slots}) must be a positive multiple of page_size ({page_size})")
         for s, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
             _chk(2.0 ** -24 <= s <= 2.0 ** 24 and math.frexp(s)[0] == 0.5, f"{name} must be a power of two from 2^-24 to 2^24")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales

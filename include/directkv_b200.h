@@ -349,7 +349,7 @@ typedef struct {
     void*   k_scales;     /* [n_slots, nh_kv, 8] e4m3, 8-byte aligned, finite and not negative */
     void*   v_codes;
     void*   v_scales;
-    int64_t n_slots;      /* 1 .. 2^31 - 1 */
+    int64_t n_slots;      /* 1 .. 2^31 - 1, a multiple of page_size */
     int     nh_kv;
     int     page_size;    /* tokens per page, power of two >= 1 */
     float   k_scale;      /* powers of two, 2^-24 .. 2^24 */
