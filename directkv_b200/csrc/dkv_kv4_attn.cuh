@@ -88,6 +88,12 @@ __device__ __forceinline__ uint32_t bit_select(uint32_t a, uint32_t b, uint32_t 
     asm("lop3.b32 %0, %1, %2, %3, 0xCA;" : "=r"(d) : "r"(mask), "r"(a), "r"(b));
     return d;
 }
+// The same with zeros to add to.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -207,11 +213,11 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
             for (int n = 0; n < NT; ++n) st.m[n][0] = st.m[n][1] = kKv4Low, st.l[n][0] = st.l[n][1] = 0.f;
 
             // ---- copies: of every 16 tokens this lane brings 16 bytes of K and V of tokens tau and tau + 8, and 8 bytes of scales
-            const long long code_row = static_cast<long long>(p.nh_kv) * 64;
-            const uint8_t* k_lane = p.k_codes + kvh * 64 + c * 16 + (WIDE ? tau * code_row : 0);
-            const uint8_t* v_lane = p.v_codes + kvh * 64 + c * 16 + (WIDE ? tau * code_row : 0);
+            const unsigned code_row = p.nh_kv * 64, scale_row = p.nh_kv * 8;                 // bytes per token
+            const uint8_t* k_lane = p.k_codes + kvh * 64 + c * 16 + (WIDE ? tau * code_row : 0u);
+            const uint8_t* v_lane = p.v_codes + kvh * 64 + c * 16 + (WIDE ? tau * code_row : 0u);
             const int s_tau = tau + (c & 1) * 8;
-            const uint8_t* s_lane = ((c & 2) ? p.v_scales : p.k_scales) + kvh * 8 + (WIDE ? s_tau * (code_row >> 3) : 0);
+            const uint8_t* s_lane = ((c & 2) ? p.v_scales : p.k_scales) + kvh * 8 + (WIDE ? s_tau * scale_row : 0);
             const uint32_t k_dst = ring + lane * 16;
             const uint32_t v_dst = ring + 1024 + tau * 64 + ((c ^ ((g >> 1) & 2)) << 4);     // 16-byte pieces of rows 2, 3 mod 4 change places
             const uint32_t s_dst = ring + 2048 + (c & 2) * 64 + s_tau * 8;
@@ -238,8 +244,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                 const uint32_t at = (i & (kKv4Stages - 1)) * kKv4StageBytes;
                 const int left = len - token0(i);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (half * 16 >= left) break;
+                for (int half = 0; half < 2; ++half) {        // a half behind the length is filled with zeros
                     const uint32_t h = at + half * kKv4HalfBytes;
                     uint32_t n0, n1;
                     const uint8_t *k0, *k1, *v0, *v1, *sp;
@@ -247,18 +252,20 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                         // A page lies in the pool as a whole: rows behind the length may be addressed, but are not read.
                         const int slot = __shfl_sync(0xffffffffu, now, (2 * i + half) & 31);
                         const int n = slot < 0 ? 0 : left - half * 16;
-                        const long long first = static_cast<long long>(max(slot, 0)) * code_row;
+                        const unsigned first = static_cast<unsigned>(max(slot, 0));
+                        const unsigned long long at_codes = static_cast<unsigned long long>(first) * code_row;
                         n0 = tau < n ? 16u : 0u, n1 = tau + 8 < n ? 16u : 0u;
-                        k0 = k_lane + first, k1 = k0 + 8 * code_row;
-                        v0 = v_lane + first, v1 = v0 + 8 * code_row;
-                        sp = s_lane + (first >> 3);
+                        k0 = k_lane + at_codes, k1 = k0 + 8 * code_row;
+                        v0 = v_lane + at_codes, v1 = v0 + 8 * code_row;
+                        sp = s_lane + static_cast<unsigned long long>(first) * scale_row;
                     } else {
                         const int a = __shfl_sync(0xffffffffu, now, half * 16 + tau), b8 = __shfl_sync(0xffffffffu, now, half * 16 + tau + 8);
                         n0 = a < 0 ? 0u : 16u, n1 = b8 < 0 ? 0u : 16u;
-                        const long long ra = max(a, 0) * code_row, rb = max(b8, 0) * code_row;
+                        const unsigned ua = static_cast<unsigned>(max(a, 0)), ub = static_cast<unsigned>(max(b8, 0));
+                        const unsigned long long ra = static_cast<unsigned long long>(ua) * code_row, rb = static_cast<unsigned long long>(ub) * code_row;
                         k0 = k_lane + ra, k1 = k_lane + rb;
                         v0 = v_lane + ra, v1 = v_lane + rb;
-                        sp = s_lane + (((c & 1) ? rb : ra) >> 3);
+                        sp = s_lane + static_cast<unsigned long long>((c & 1) ? ub : ua) * scale_row;
                     }
                     cp_async16(k_dst + h, k0, n0);
                     cp_async16(k_dst + h + 512, k1, n1);
@@ -324,19 +331,15 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                 const uint8_t* s0 = ring_ptr + (i & (kKv4Stages - 1)) * kKv4StageBytes;
                 const int t0 = token0(i);
                 if (t0 >= len) continue;
-                const int halves = t0 + 16 < len ? 2 : 1;
 
                 // ---- scores
                 float sc[2][NT][4];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) sc[half][n][0] = sc[half][n][1] = sc[half][n][2] = sc[half][n][3] = 0.f;
-                    if (half >= halves) break;
                     const uint8_t* s = s0 + half * kKv4HalfBytes;
                     const uint4 ka = *reinterpret_cast<const uint4*>(s + lane * 16), kb = *reinterpret_cast<const uint4*>(s + 512 + lane * 16);
-                    const uint32_t wa = *reinterpret_cast<const uint32_t*>(s + 2048 + tau * 8 + (c >> 1) * 4), wb = *reinterpret_cast<const uint32_t*>(s + 2048 + 64 + tau * 8 + (c >> 1) * 4);
-                    const uint32_t ha = e4m3x2_to_f16((wa >> ((c & 1) * 16)) & 0xffffu), hb = e4m3x2_to_f16((wb >> ((c & 1) * 16)) & 0xffffu);
+                    const uint32_t ha = e4m3x2_to_f16(*reinterpret_cast<const uint16_t*>(s + 2048 + tau * 8 + c * 2));
+                    const uint32_t hb = e4m3x2_to_f16(*reinterpret_cast<const uint16_t*>(s + 2048 + 64 + tau * 8 + c * 2));
                     const uint32_t aw[4] = {ka.x, ka.y, ka.z, ka.w}, bw[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -348,7 +351,8 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                         for (int u = 0; u < 4; ++u) a[u] = hmul2_f16(a[u], sa), bq[u] = hmul2_f16(bq[u], sb);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma_f16(sc[half][n], a[0], bq[0], a[1], bq[1], qf[n][2 * k][0], qf[n][2 * k][1]);
+                            if (k == 0) mma_f16_first(sc[half][n], a[0], bq[0], a[1], bq[1], qf[n][0][0], qf[n][0][1]);
+                            else mma_f16(sc[half][n], a[0], bq[0], a[1], bq[1], qf[n][2 * k][0], qf[n][2 * k][1]);
                             mma_f16(sc[half][n], a[2], bq[2], a[3], bq[3], qf[n][2 * k + 1][0], qf[n][2 * k + 1][1]);
                         }
                     }
@@ -395,7 +399,6 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                 }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    if (half >= halves) break;
                     uint32_t pf[NT][2];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
