@@ -21,13 +21,20 @@
 
 namespace dkv {
 
-constexpr int kKv4Warps = 8;
 constexpr int kKv4Tile = 32;                             // tokens a warp takes in one step, as two halves of 16
 constexpr int kKv4Stages = 2;
 constexpr int kKv4HalfBytes = 2 * 1024 + 2 * 128;        // 16 tokens: K codes, V codes, K scales, V scales
 constexpr int kKv4StageBytes = 2 * kKv4HalfBytes;
-constexpr int kKv4RingBytes = kKv4Stages * kKv4StageBytes;
-constexpr int kKv4MaxBatch = 4096;
+// Warps of a block and blocks per SM: 16 warps per SM with 8 columns (query fragments in registers), 12 with 16 (in shared
+// memory; 16 drafts of up to 4096 tokens: 36 us, against 48 us as 16 warps that spill).
+template <int NT>
+constexpr int kKv4Warps = NT == 1 ? 8 : 4;
+template <int NT>
+constexpr int kKv4BlocksPerSm = NT == 1 ? 2 : 3;
+template <int NT>
+constexpr int kKv4WarpBytes = kKv4Stages * kKv4StageBytes + (NT == 1 ? 0 : NT * 2048);
+constexpr int kKv4MaxBatch = 4096;                       // of a call
+constexpr int kKv4LaunchBatch = 1024;                    // of a launch: what leaves room for the blocks that share an SM
 constexpr int kKv4RecFloats = 132;                       // O[128], m (log2 domain), l, 2 pad
 constexpr float kKv4Low = -3e38f;                        // the running maximum before the first token
 constexpr float kKv4Lag = 8.f;                           // the maximum follows once a score is 2^8 above it: P <= 2^8 in fp16
@@ -43,7 +50,8 @@ struct Kv4AttnParams {
     long long pt_stride;
     int pt_rows;                     // 0: unknown
     int max_pages;                   // entries of a row that may be read
-    const int* row_map;              // [batch] or nullptr
+    const int* row_map;              // [batch] or nullptr: row b + row0
+    int row0;
     const uint8_t* k_codes;          // [n_slots, nh_kv, 64]
     const uint8_t* k_scales;         // [n_slots, nh_kv, 8]
     const uint8_t* v_codes;
@@ -54,7 +62,7 @@ struct Kv4AttnParams {
     int batch, n_q, nh_q, nh_kv, group;
     int cols;                        // n_q * group: columns of one KV head
     int n_cc;                        // column chunks of 8 * NT
-    int hg, ts, n_hg;                // heads and token lanes of a block (hg * ts <= kKv4Warps), head groups
+    int hg, ts, n_hg;                // heads and token lanes of a block (hg * ts <= kKv4Warps<NT>), head groups
     float scale_log2;                // softmax scale * k_scale * log2(e)
     float v_scale;
     float* rec;                      // [blocks, 2, hg, 8 * NT, kKv4RecFloats]
@@ -67,6 +75,12 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
 }
 __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -110,7 +124,7 @@ __device__ __forceinline__ int kv4_blocks(long long total, int grid) { return to
 
 // A request's length as far as the table reaches, and its row; a length or row outside is reported.
 __device__ __forceinline__ int kv4_length(const Kv4AttnParams& p, int b, long long* row_out) {
-    const long long row = p.row_map != nullptr ? p.row_map[b] : b;
+    const long long row = p.row_map != nullptr ? p.row_map[b] : b + p.row0;
     *row_out = row;
     const int len = p.seq_lens[b];
     const long long room = static_cast<long long>(p.max_pages) << p.page_shift;
@@ -129,18 +143,18 @@ struct Kv4State {
 
 // WIDE: pages of 16 tokens and more, so that 16 tokens lie in one page and one table entry serves the whole warp.
 template <int NT, bool WIDE>
-__global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4AttnParams p) {
-    constexpr int C = 8 * NT;
+__global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_attn_kernel(const Kv4AttnParams p) {
+    constexpr int C = 8 * NT, W = kKv4Warps<NT>;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int sh_scan[kKv4Warps];
-    int* cum = reinterpret_cast<int*>(smem + kKv4Warps * kKv4RingBytes);
+    __shared__ int sh_scan[W];
+    int* cum = reinterpret_cast<int*>(smem + W * kKv4WarpBytes<NT>);
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int g = lane >> 2, c = lane & 3;
 
     // Tiles (of 32 * ts tokens) before every request; a request without tokens has one, which writes its zeros.
     if (threadIdx.x == 0) cum[0] = 0;
     int before = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += kKv4Warps * 32) {
+    for (int b0 = 0; b0 < p.batch; b0 += W * 32) {
         const int b = b0 + threadIdx.x;
         int n = 0;
         if (b < p.batch) {
@@ -161,7 +175,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
         int base = before;
         for (int i = 0; i < w; ++i) base += sh_scan[i];
         if (b < p.batch) cum[b + 1] = base + inc;
-        for (int i = 0; i < kKv4Warps; ++i) before += sh_scan[i];
+        for (int i = 0; i < W; ++i) before += sh_scan[i];
         __syncthreads();
     }
     if (blockIdx.x == 0)
@@ -175,7 +189,8 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
 
     const int hl = w % p.hg, tl = w / p.hg;
     const bool active = tl < p.ts;
-    uint8_t* const ring_ptr = smem + w * kKv4RingBytes;
+    uint8_t* const ring_ptr = smem + w * kKv4WarpBytes<NT>;
+    uint4* const q_smem = reinterpret_cast<uint4*>(ring_ptr + kKv4Stages * kKv4StageBytes) + lane;
     const uint32_t ring = smem_u32(ring_ptr);
     const int tau = (g >> 1) + 4 * (g & 1);          // token of this lane's rows of the score tile: tau and tau + 8
     const int page_mask = (1 << p.page_shift) - 1;
@@ -216,6 +231,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
             const unsigned code_row = p.nh_kv * 64, scale_row = p.nh_kv * 8;                 // bytes per token
             const uint8_t* k_lane = p.k_codes + kvh * 64 + c * 16 + (WIDE ? tau * code_row : 0u);
             const uint8_t* v_lane = p.v_codes + kvh * 64 + c * 16 + (WIDE ? tau * code_row : 0u);
+            const unsigned long long row8 = 8ull * code_row;
             const int s_tau = tau + (c & 1) * 8;
             const uint8_t* s_lane = ((c & 2) ? p.v_scales : p.k_scales) + kvh * 8 + (WIDE ? s_tau * scale_row : 0);
             const uint32_t k_dst = ring + lane * 16;
@@ -242,36 +258,51 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                     next = look(i + (WIDE ? 16 : 1));
                 }
                 const uint32_t at = (i & (kKv4Stages - 1)) * kKv4StageBytes;
+                const uint32_t kd = k_dst + at, vd = v_dst + at, sd = s_dst + at;
                 const int left = len - token0(i);
+                if constexpr (WIDE) {
+                    // A page lies in the pool as a whole: rows behind the length may be addressed, but are not read.
+                    const int s0 = __shfl_sync(0xffffffffu, now, (2 * i) & 31), s1 = __shfl_sync(0xffffffffu, now, (2 * i + 1) & 31);
+                    const bool plain = left >= kKv4Tile && (s0 | s1) >= 0;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {        // a half behind the length is filled with zeros
-                    const uint32_t h = at + half * kKv4HalfBytes;
-                    uint32_t n0, n1;
-                    const uint8_t *k0, *k1, *v0, *v1, *sp;
-                    if constexpr (WIDE) {
-                        // A page lies in the pool as a whole: rows behind the length may be addressed, but are not read.
-                        const int slot = __shfl_sync(0xffffffffu, now, (2 * i + half) & 31);
-                        const int n = slot < 0 ? 0 : left - half * 16;
-                        const unsigned first = static_cast<unsigned>(max(slot, 0));
-                        const unsigned long long at_codes = static_cast<unsigned long long>(first) * code_row;
-                        n0 = tau < n ? 16u : 0u, n1 = tau + 8 < n ? 16u : 0u;
-                        k0 = k_lane + at_codes, k1 = k0 + 8 * code_row;
-                        v0 = v_lane + at_codes, v1 = v0 + 8 * code_row;
-                        sp = s_lane + static_cast<unsigned long long>(first) * scale_row;
-                    } else {
+                    for (int half = 0; half < 2; ++half) {        // a half behind the length is filled with zeros
+                        const int slot = half ? s1 : s0;
+                        const unsigned first = plain ? slot : max(slot, 0);
+                        const unsigned long long codes = static_cast<unsigned long long>(first) * code_row;
+                        const uint8_t *k0 = k_lane + codes, *v0 = v_lane + codes, *k1 = k0 + row8, *v1 = v0 + row8;
+                        const uint8_t* sp = s_lane + static_cast<unsigned long long>(first) * scale_row;
+                        const uint32_t h = half * kKv4HalfBytes;
+                        if (plain) {
+                            cp_async16(kd + h, k0);
+                            cp_async16(kd + h + 512, k1);
+                            cp_async16(vd + h, v0);
+                            cp_async16(vd + h + 512, v1);
+                            cp_async8(sd + h, sp);
+                        } else {
+                            const int n = slot < 0 ? 0 : left - half * 16;
+                            const uint32_t n0 = tau < n ? 16u : 0u, n1 = tau + 8 < n ? 16u : 0u;
+                            cp_async16(kd + h, k0, n0);
+                            cp_async16(kd + h + 512, k1, n1);
+                            cp_async16(vd + h, v0, n0);
+                            cp_async16(vd + h + 512, v1, n1);
+                            cp_async8(sd + h, sp, ((c & 1) ? n1 : n0) >> 1);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
                         const int a = __shfl_sync(0xffffffffu, now, half * 16 + tau), b8 = __shfl_sync(0xffffffffu, now, half * 16 + tau + 8);
-                        n0 = a < 0 ? 0u : 16u, n1 = b8 < 0 ? 0u : 16u;
+                        const uint32_t n0 = a < 0 ? 0u : 16u, n1 = b8 < 0 ? 0u : 16u;
                         const unsigned ua = static_cast<unsigned>(max(a, 0)), ub = static_cast<unsigned>(max(b8, 0));
                         const unsigned long long ra = static_cast<unsigned long long>(ua) * code_row, rb = static_cast<unsigned long long>(ub) * code_row;
-                        k0 = k_lane + ra, k1 = k_lane + rb;
-                        v0 = v_lane + ra, v1 = v_lane + rb;
-                        sp = s_lane + static_cast<unsigned long long>((c & 1) ? ub : ua) * scale_row;
+                        const uint8_t* sp = s_lane + static_cast<unsigned long long>((c & 1) ? ub : ua) * scale_row;
+                        const uint32_t h = half * kKv4HalfBytes;
+                        cp_async16(kd + h, k_lane + ra, n0);
+                        cp_async16(kd + h + 512, k_lane + rb, n1);
+                        cp_async16(vd + h, v_lane + ra, n0);
+                        cp_async16(vd + h + 512, v_lane + rb, n1);
+                        cp_async8(sd + h, sp, ((c & 1) ? n1 : n0) >> 1);
                     }
-                    cp_async16(k_dst + h, k0, n0);
-                    cp_async16(k_dst + h + 512, k1, n1);
-                    cp_async16(v_dst + h, v0, n0);
-                    cp_async16(v_dst + h + 512, v1, n1);
-                    cp_async8(s_dst + h, sp, ((c & 1) ? n1 : n0) >> 1);
                 }
             };
             next = look(0);
@@ -279,9 +310,8 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
             cp_async_commit();
 
             // ---- queries: column g of each 8, dimensions 32 c .. 32 c + 31, as fp16 scaled by a power of two
-            uint32_t qf[NT][8][2];
+            uint32_t qf[NT == 1 ? 16 : 1];
             float mul[NT][2];
-            int limit[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int col = cc * C + n * 8 + g;
@@ -298,9 +328,8 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    top = max(max(max(top, (v[i].x & 0x7fffu)), max((v[i].x >> 16) & 0x7fffu, v[i].y & 0x7fffu)),
-                              max(max((v[i].y >> 16) & 0x7fffu, v[i].z & 0x7fffu),
-                                  max((v[i].z >> 16) & 0x7fffu, max(v[i].w & 0x7fffu, (v[i].w >> 16) & 0x7fffu))));
+                    top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu), __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
+                top = max(top & 0xffffu, top >> 16);
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 int e = static_cast<int>(top >> 7);                                 // biased exponent of the largest value
@@ -309,16 +338,15 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                 const float undo = __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    qf[n][2 * i][0] = pack_f16x2(bf16lo(v[i].x) * f, bf16hi(v[i].x) * f);
-                    qf[n][2 * i][1] = pack_f16x2(bf16lo(v[i].y) * f, bf16hi(v[i].y) * f);
-                    qf[n][2 * i + 1][0] = pack_f16x2(bf16lo(v[i].z) * f, bf16hi(v[i].z) * f);
-                    qf[n][2 * i + 1][1] = pack_f16x2(bf16lo(v[i].w) * f, bf16hi(v[i].w) * f);
+                    const uint4 h = make_uint4(pack_f16x2(bf16lo(v[i].x) * f, bf16hi(v[i].x) * f), pack_f16x2(bf16lo(v[i].y) * f, bf16hi(v[i].y) * f),
+                                               pack_f16x2(bf16lo(v[i].z) * f, bf16hi(v[i].z) * f), pack_f16x2(bf16lo(v[i].w) * f, bf16hi(v[i].w) * f));
+                    if constexpr (NT == 1) qf[4 * i] = h.x, qf[4 * i + 1] = h.y, qf[4 * i + 2] = h.z, qf[4 * i + 3] = h.w;
+                    else q_smem[(n * 4 + i) * 32] = h;       // read back by this lane alone
                 }
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     mul[n][k] = __shfl_sync(0xffffffffu, undo, (2 * c + k) * 4) * p.scale_log2;
                     if (mul[n][k] == 0.f) mul[n][k] = 1e-30f;                       // scores of zero all the same; masks need a sign
-                    limit[n][k] = len - p.n_q + 1 + min((cc * C + n * 8 + 2 * c + k) / p.group, p.n_q - 1);
                 }
             }
             const int full = len - p.n_q + 1;             // tokens that every column attends
@@ -351,9 +379,12 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                         for (int u = 0; u < 4; ++u) a[u] = hmul2_f16(a[u], sa), bq[u] = hmul2_f16(bq[u], sb);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            if (k == 0) mma_f16_first(sc[half][n], a[0], bq[0], a[1], bq[1], qf[n][0][0], qf[n][0][1]);
-                            else mma_f16(sc[half][n], a[0], bq[0], a[1], bq[1], qf[n][2 * k][0], qf[n][2 * k][1]);
-                            mma_f16(sc[half][n], a[2], bq[2], a[3], bq[3], qf[n][2 * k + 1][0], qf[n][2 * k + 1][1]);
+                            uint4 q;
+                            if constexpr (NT == 1) q = make_uint4(qf[4 * k], qf[4 * k + 1], qf[4 * k + 2], qf[4 * k + 3]);
+                            else q = q_smem[(n * 4 + k) * 32];
+                            if (k == 0) mma_f16_first(sc[half][n], a[0], bq[0], a[1], bq[1], q.x, q.y);
+                            else mma_f16(sc[half][n], a[0], bq[0], a[1], bq[1], q.x, q.y);
+                            mma_f16(sc[half][n], a[2], bq[2], a[3], bq[3], q.z, q.w);
                         }
                     }
                 }
@@ -364,7 +395,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
-                                if (t0 + half * 16 + tau + (k >> 1) * 8 >= limit[n][k & 1]) sc[half][n][k] = copysignf(INFINITY, -mul[n][k & 1]);
+                                if (t0 + half * 16 + tau + (k >> 1) * 8 >= full + min((cc * C + n * 8 + 2 * c + (k & 1)) / p.group, p.n_q - 1)) sc[half][n][k] = copysignf(INFINITY, -mul[n][k & 1]);
                 }
                 float e[2][NT][4];
                 float high = kKv4Low;
@@ -467,7 +498,7 @@ __global__ void __launch_bounds__(kKv4Warps * 32, 2) kv4_attn_kernel(const Kv4At
             __syncthreads();
             if (active && tl == 0) {
                 for (int t = 1; t < p.ts; ++t) {
-                    const float* from = reinterpret_cast<const float*>(smem + (t * p.hg + hl) * kKv4RingBytes);
+                    const float* from = reinterpret_cast<const float*>(smem + (t * p.hg + hl) * kKv4WarpBytes<NT>);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll

@@ -35,33 +35,44 @@ int check_kv4_pool(const dkv_context* ctx, const dkv_kv4_pool* pool) {
     return DKV_OK;
 }
 
-// Heads and token lanes of a block: as many of the 8 warps as the number of heads allows (7 will do), and of the shapes
-// that use them the one with the most heads side by side, whose rows of a token are one contiguous read.
-void kv4_block_shape(int nh_kv, int* hg, int* ts) {
+// Heads and token lanes of a block: as many of its warps as the number of heads allows, and of the shapes that use
+// them the one with the most heads side by side, whose rows of a token are one contiguous read.
+void kv4_block_shape(int nh_kv, int warps, int* hg, int* ts) {
     int best = 0;
-    for (int h = 1; h <= kKv4Warps; ++h) {
+    for (int h = 1; h <= warps; ++h) {
         if (nh_kv % h != 0) continue;
-        const int t = kKv4Warps / h, used = std::min(h * t, 7);
-        if (used >= best) best = used, *hg = h, *ts = t;
+        const int t = warps / h;
+        if (h * t >= best) best = h * t, *hg = h, *ts = t;
     }
 }
 
-constexpr size_t kKv4CumBytes = (kKv4MaxBatch + 1) * sizeof(int) / 256 * 256 + 256;
+constexpr size_t kKv4CumBytes = (kKv4LaunchBatch + 1) * sizeof(int) / 256 * 256 + 256;
 
-int kv4_grid(const dkv_context* ctx) { return ctx->sm_count * 2; }
+template <int NT>
+int kv4_grid(const dkv_context* ctx) {
+    return ctx->sm_count * kKv4BlocksPerSm<NT>;
+}
 
 // One size for every call, so that any call (or registering a pool) makes room for all of them.
 size_t kv4_workspace(const dkv_context* ctx) {
-    return kKv4CumBytes + static_cast<size_t>(kv4_grid(ctx)) * 2 * kKv4Warps * 16 * kKv4RecFloats * sizeof(float);
+    const size_t cols = std::max(kv4_grid<1>(ctx) * kKv4Warps<1> * 8, kv4_grid<2>(ctx) * kKv4Warps<2> * 16);
+    return kKv4CumBytes + cols * 2 * kKv4RecFloats * sizeof(float);
+}
+
+template <int NT>
+constexpr int kv4_smem(int batch) {
+    return kKv4Warps<NT> * kKv4WarpBytes<NT> + (batch + 1) * static_cast<int>(sizeof(int));
 }
 
 template <int NT>
 int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
+    kv4_block_shape(p.nh_kv, kKv4Warps<NT>, &p.hg, &p.ts);
+    p.n_hg = p.nh_kv / p.hg;
     p.n_cc = (p.cols + 8 * NT - 1) / (8 * NT);
-    const int grid = kv4_grid(ctx);
-    const size_t smem = kKv4Warps * kKv4RingBytes + (p.batch + 1) * sizeof(int);
-    if (p.page_shift >= 4) kv4_attn_kernel<NT, true><<<grid, kKv4Warps * 32, smem, st>>>(p);
-    else kv4_attn_kernel<NT, false><<<grid, kKv4Warps * 32, smem, st>>>(p);
+    const int grid = kv4_grid<NT>(ctx);
+    const size_t smem = kv4_smem<NT>(p.batch);
+    if (p.page_shift >= 4) kv4_attn_kernel<NT, true><<<grid, kKv4Warps<NT> * 32, smem, st>>>(p);
+    else kv4_attn_kernel<NT, false><<<grid, kKv4Warps<NT> * 32, smem, st>>>(p);
     DKV_CUDA(cudaGetLastError());
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.n_q * p.nh_q);
@@ -84,8 +95,7 @@ int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
 
 template <int NT, bool WIDE>
 cudaError_t kv4_set_attr() {
-    return cudaFuncSetAttribute(kv4_attn_kernel<NT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kKv4Warps * kKv4RingBytes + (kKv4MaxBatch + 1) * static_cast<int>(sizeof(int)));
+    return cudaFuncSetAttribute(kv4_attn_kernel<NT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kv4_smem<NT>(kKv4LaunchBatch));
 }
 
 }  // namespace
@@ -225,14 +235,23 @@ int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_
     DKV_REQUIRE(static_cast<int64_t>(a->batch) * a->n_q * a->nh_q <= INT32_MAX, "too many query rows");
     DKV_REQUIRE((static_cast<int64_t>(p.max_pages) << p.page_shift) / 16 * a->batch < INT32_MAX, "%d requests of up to %lld tokens are too many for one call",
                 a->batch, static_cast<long long>(p.max_pages) << p.page_shift);
-    kv4_block_shape(pool->nh_kv, &p.hg, &p.ts);
-    p.n_hg = pool->nh_kv / p.hg;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     rc = ensure_buffer(ctx, &ctx->kv4, kv4_workspace(ctx), stream_is_capturing(st), "workspace of the 4-bit attention");
     if (rc != DKV_OK) return rc;
     p.cum = reinterpret_cast<int*>(ctx->kv4.ptr);
     p.rec = reinterpret_cast<float*>(ctx->kv4.ptr + kKv4CumBytes);
-    return p.cols <= 8 ? launch_kv4_attn<1>(ctx, p, st) : launch_kv4_attn<2>(ctx, p, st);
+    for (int b0 = 0; b0 < a->batch && rc == DKV_OK; b0 += kKv4LaunchBatch) {
+        Kv4AttnParams part = p;
+        part.batch = std::min(a->batch - b0, kKv4LaunchBatch);
+        part.row0 = b0;
+        part.seq_lens += b0;
+        if (part.row_map) part.row_map += b0;
+        part.q += static_cast<int64_t>(b0) * p.n_q * p.q_stride;
+        part.out += static_cast<int64_t>(b0) * p.n_q * p.out_stride;
+        if (part.lse) part.lse += static_cast<int64_t>(b0) * p.n_q * p.nh_q;
+        rc = p.cols <= 8 ? launch_kv4_attn<1>(ctx, part, st) : launch_kv4_attn<2>(ctx, part, st);
+    }
+    return rc;
 }
 
 int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* a, void* stream) {

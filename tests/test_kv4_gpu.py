@@ -217,6 +217,8 @@ def test_one_long_request_and_a_batch_of_short_ones():
     _check(c, *_run(c))
     c = _case([1 + i % 37 for i in range(300)], 4, 2, 4, 1, 521)
     _check(c, *_run(c))
+    c = _case([i % 23 for i in range(2000)], 2, 2, 16, 1, 522)
+    _check(c, *_run(c))
 
 
 def test_row_map_strides_and_2d_queries():
