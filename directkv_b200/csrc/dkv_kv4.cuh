@@ -68,104 +68,164 @@ __device__ __forceinline__ uint32_t f32_to_e4m3(float v) {
     return r & 0xffu;
 }
 
-struct Kv4StoreParams {
-    const __nv_bfloat16* src[2];     // K rows, V rows: [n, nh, 128], token stride in elements
-    long long src_stride[2];
-    uint8_t* codes[2];
-    uint8_t* scales[2];
-    float inv_scale[2];              // 1 / pool scale
+// 32 bytes in one instruction; 32-byte aligned.
+__device__ __forceinline__ void ld_global_v8(const void* p, uint32_t (&w)[8]) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// To 16 significant bits, to nearest.
+__device__ __forceinline__ float snap16(float x) { return __uint_as_float((__float_as_uint(x) + 0x80u) & 0xffffff00u); }
+
+struct Kv4RowsParams {
+    const __nv_bfloat16 *k, *v;      // store: [n, nh, 128], token strides in elements
+    long long k_stride, v_stride;
+    __nv_bfloat16 *k_out, *v_out;    // load: [n, nh, 128] contiguous
+    uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+    float k_scale, v_scale;          // store: 1 / pool scale; load: pool scale
     const void* slots;               // [n] int32 or int64
     int slots64;
-    long long n_rows;                // n * nh
+    int wide;                        // the bf16 rows are 32-byte aligned
+    long long n;
     int nh;
+    int per_block;                   // tokens of a block
     long long n_slots;
     unsigned int* status;
 };
 
-__device__ __forceinline__ long long kv4_slot(const void* slots, int slots64, long long i) {
-    return slots64 ? static_cast<const long long*>(slots)[i] : static_cast<long long>(static_cast<const int*>(slots)[i]);
+__device__ __forceinline__ long long kv4_slot(const Kv4RowsParams& p, long long i) {
+    return p.slots64 ? static_cast<const long long*>(p.slots)[i] : static_cast<long long>(static_cast<const int*>(p.slots)[i]);
 }
 
-// One thread per block of 16 dimensions (8 threads per row), K rows first, then V rows.
-__global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4StoreParams p) {
-    const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int which = blockIdx.y;
-    const long long row = i >> 3;
-    if (row >= p.n_rows) return;
-    const int blk = static_cast<int>(i & 7);
-    const long long tok = row / p.nh;
-    const int head = static_cast<int>(row - tok * p.nh);
-    const long long slot = kv4_slot(p.slots, p.slots64, tok);
-    if (slot < 0 || slot >= p.n_slots) {
-        if (blk == 0) atomicOr(p.status, kStatusBadSlot);
-        return;
+// Quantises 16 bf16 values.  Returns whether one of them is not finite.
+//
+// y / s decides between codes at borders of 2 significant bits times s (4 bits), and max|y| / 6 between scales at borders of
+// 5 bits: a bf16 value (8 bits) lies on such a border or is at least 2^-8 of it away.  So a product with the rounded
+// reciprocal (off by less than 2^-21), snapped to 16 bits, is on a border only where the true quotient is, and on the
+// right side of it otherwise: the result is that of exact arithmetic, without a division per value.
+__device__ __forceinline__ bool kv4_quantise(const uint32_t (&w)[8], float inv_scale, uint2* codes, uint32_t* scale) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = __vmaxu2(m, w[j] & 0x7fff7fffu);
+    m = max(m & 0xffffu, m >> 16);
+    const bool odd = m >= 0x7f80u;
+    float y[16];
+    float top;
+    if (!odd) {
+        top = fminf(__uint_as_float(m << 16) * inv_scale, 2688.f);
+    } else {                                              // infinities count as the largest value, not-a-numbers as zero
+        top = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float x = (j & 1) ? bf16hi(w[j >> 1]) : bf16lo(w[j >> 1]);
+            top = fmaxf(top, x == x ? fminf(fabsf(x) * inv_scale, 2688.f) : 0.f);
+        }
     }
-    const uint4* src = reinterpret_cast<const uint4*>(p.src[which] + tok * p.src_stride[which] + head * 128 + blk * 16);
-    const uint4 lo = src[0], hi = src[1];
-    const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    float y[16], top = 0.f;
-    bool odd = false;                 // a value that is not finite
+    uint32_t sb = f32_to_e4m3(snap16(top * (1.f / 6.f)));
+    sb = max(sb, 1u);                                     // 2^-9 at least: the reciprocal exists
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e4m3_to_f32(sb)));
+    const float f = r * inv_scale;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         const float x = (j & 1) ? bf16hi(w[j >> 1]) : bf16lo(w[j >> 1]);
-        odd |= !(fabsf(x) <= 3.4e38f);
-        y[j] = x == x ? fminf(fmaxf(x * p.inv_scale[which], -2688.f), 2688.f) : 0.f;
-        top = fmaxf(top, fabsf(y[j]));
+        y[j] = snap16(x * f);
     }
-    if (odd) atomicOr(p.status, kStatusNonFinite);
-    // __fdiv_rn: a quotient that lies exactly between two scales (or two codes) must come out exactly there.
-    uint32_t sb = f32_to_e4m3(__fdiv_rn(top, 6.f));
-    sb = sb == 0 ? 1u : sb;           // 2^-9: never a division by zero below
-    const float s = e4m3_to_f32(sb);
+    if (odd) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) y[j] = __fdiv_rn(y[j], s);
-    const long long at = (slot * p.nh + head) * 8 + blk;
-    reinterpret_cast<uint2*>(p.codes[which])[at] = make_uint2(f32_to_e2m1x8(y), f32_to_e2m1x8(y + 8));
-    p.scales[which][at] = static_cast<uint8_t>(sb);
+        for (int j = 0; j < 16; ++j) {
+            const float x = (j & 1) ? bf16hi(w[j >> 1]) : bf16lo(w[j >> 1]);
+            y[j] = x == x ? snap16(fminf(fmaxf(x, -1e30f), 1e30f) * f) : 0.f;
+            if (!(fabsf(x) <= 3.4e38f) && x == x) y[j] = copysignf(6.f, x);
+        }
+    }
+    *codes = make_uint2(f32_to_e2m1x8(y), f32_to_e2m1x8(y + 8));
+    *scale = sb;
+    return odd;
 }
 
-struct Kv4LoadParams {
-    const uint8_t* codes[2];
-    const uint8_t* scales[2];
-    float scale[2];                  // pool scale
-    __nv_bfloat16* dst[2];           // [n, nh, 128] contiguous
-    const void* slots;
-    int slots64;
-    long long n_rows;
-    int nh;
-    long long n_slots;
-    unsigned int* status;
-};
-
-__global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4LoadParams p) {
-    const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int which = blockIdx.y;
-    const long long row = i >> 3;
-    if (row >= p.n_rows) return;
-    const int blk = static_cast<int>(i & 7);
-    const long long tok = row / p.nh;
-    const int head = static_cast<int>(row - tok * p.nh);
-    const long long slot = kv4_slot(p.slots, p.slots64, tok);
-    uint2 c = make_uint2(0u, 0u);
-    float s = 0.f;
-    if (slot >= 0 && slot < p.n_slots) {
-        const long long at = (slot * p.nh + head) * 8 + blk;
-        c = reinterpret_cast<const uint2*>(p.codes[which])[at];
-        s = e4m3_to_f32(p.scales[which][at]) * p.scale[which];
-    } else if (blk == 0) {
-        atomicOr(p.status, kStatusBadSlot);
+__device__ __forceinline__ void kv4_read16(const __nv_bfloat16* src, int wide, uint32_t (&w)[8]) {
+    if (wide) {
+        ld_global_v8(src, w);
+    } else {
+        const uint4 a = reinterpret_cast<const uint4*>(src)[0], b = reinterpret_cast<const uint4*>(src)[1];
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
     }
+}
+
+// A thread takes one block of 16 dimensions of K and the same one of V.
+__global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowsParams p) {
+    const int units = p.nh * 8;                           // blocks of 16 per token
+    for (int i = threadIdx.x; i < p.per_block * units; i += 256) {
+        const int t = i / units, u = i - t * units;
+        const long long tok = static_cast<long long>(blockIdx.x) * p.per_block + t;
+        if (tok >= p.n) return;
+        const long long slot = kv4_slot(p, tok);
+        uint32_t kw[8], vw[8];
+        kv4_read16(p.k + tok * p.k_stride + u * 16, p.wide, kw);
+        kv4_read16(p.v + tok * p.v_stride + u * 16, p.wide, vw);
+        if (slot < 0 || slot >= p.n_slots) {
+            if (u == 0) atomicOr(p.status, kStatusBadSlot);
+            continue;
+        }
+        uint2 kc, vc;
+        uint32_t ks, vs;
+        bool odd = kv4_quantise(kw, p.k_scale, &kc, &ks);
+        odd |= kv4_quantise(vw, p.v_scale, &vc, &vs);
+        const long long at = slot * units + u;
+        reinterpret_cast<uint2*>(p.k_codes)[at] = kc;
+        reinterpret_cast<uint2*>(p.v_codes)[at] = vc;
+        p.k_scales[at] = static_cast<uint8_t>(ks);
+        p.v_scales[at] = static_cast<uint8_t>(vs);
+        if (odd) atomicOr(p.status, kStatusNonFinite);
+    }
+}
+
+__device__ __forceinline__ void kv4_write16(__nv_bfloat16* dst, uint2 codes, uint32_t scale, float pool_scale, int wide) {
     uint32_t h[8], o[8];
-    e2m1x8_to_f16(c.x, reinterpret_cast<uint32_t(&)[4]>(h[0]));
-    e2m1x8_to_f16(c.y, reinterpret_cast<uint32_t(&)[4]>(h[4]));
+    e2m1x8_to_f16(codes.x, reinterpret_cast<uint32_t(&)[4]>(h[0]));
+    e2m1x8_to_f16(codes.y, reinterpret_cast<uint32_t(&)[4]>(h[4]));
+    const float s = e4m3_to_f32(scale) * pool_scale;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
         o[j] = pack_bf16x2(f.x * s, f.y * s);
     }
-    uint4* dst = reinterpret_cast<uint4*>(p.dst[which] + row * 128 + blk * 16);
-    dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    if (wide) {
+        st_global_v8(dst, o);
+    } else {
+        reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+}
+
+__global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowsParams p) {
+    const int units = p.nh * 8;
+    for (int i = threadIdx.x; i < p.per_block * units; i += 256) {
+        const int t = i / units, u = i - t * units;
+        const long long tok = static_cast<long long>(blockIdx.x) * p.per_block + t;
+        if (tok >= p.n) return;
+        const long long slot = kv4_slot(p, tok);
+        uint2 kc = make_uint2(0u, 0u), vc = make_uint2(0u, 0u);
+        uint32_t ks = 0, vs = 0;
+        if (slot >= 0 && slot < p.n_slots) {
+            const long long at = slot * units + u;
+            kc = reinterpret_cast<const uint2*>(p.k_codes)[at];
+            vc = reinterpret_cast<const uint2*>(p.v_codes)[at];
+            ks = p.k_scales[at], vs = p.v_scales[at];
+        } else if (u == 0) {
+            atomicOr(p.status, kStatusBadSlot);
+        }
+        const long long at = (tok * units + u) * 16;
+        kv4_write16(p.k_out + at, kc, ks, p.k_scale, p.wide);
+        kv4_write16(p.v_out + at, vc, vs, p.v_scale, p.wide);
+    }
 }
 
 }  // namespace dkv

@@ -141,9 +141,22 @@ static int kv4_rows(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slot
     DKV_REQUIRE(ctx != nullptr && pool != nullptr, "ctx / pool is NULL");
     int rc = check_kv4_pool(ctx, pool);
     if (rc != DKV_OK) return rc;
-    DKV_REQUIRE(n_tokens >= 0 && n_tokens * pool->nh_kv <= (static_cast<int64_t>(INT32_MAX) - 1) * 32, "bad number of tokens");
+    DKV_REQUIRE(n_tokens >= 0 && n_tokens <= INT32_MAX, "n_tokens must be 0..2^31-1");
     DKV_REQUIRE(n_tokens == 0 || slots != nullptr, "slots must not be NULL");
     return DKV_OK;
+}
+
+static Kv4RowsParams kv4_rows_params(const dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, int slots64, int64_t n) {
+    Kv4RowsParams p{};
+    p.k_codes = static_cast<uint8_t*>(pool->k_codes), p.v_codes = static_cast<uint8_t*>(pool->v_codes);
+    p.k_scales = static_cast<uint8_t*>(pool->k_scales), p.v_scales = static_cast<uint8_t*>(pool->v_scales);
+    p.slots = slots, p.slots64 = slots64;
+    p.n = n;
+    p.nh = pool->nh_kv;
+    p.per_block = std::max(1, 256 / (pool->nh_kv * 8));
+    p.n_slots = pool->n_slots;
+    p.status = ctx->status;
+    return p;
 }
 
 int dkv_kv4_store(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, int slots_int64, const void* k, int64_t k_stride,
@@ -153,19 +166,13 @@ int dkv_kv4_store(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots,
     DKV_REQUIRE(k != nullptr && v != nullptr && aligned(k, 16) && aligned(v, 16), "k / v must be 16-byte aligned device pointers");
     const int64_t row = static_cast<int64_t>(pool->nh_kv) * 128;
     DKV_REQUIRE(k_stride >= row && v_stride >= row && k_stride % 8 == 0 && v_stride % 8 == 0, "k / v strides too small or unaligned");
+    Kv4RowsParams p = kv4_rows_params(ctx, pool, slots, slots_int64, n_tokens);
+    p.k = static_cast<const __nv_bfloat16*>(k), p.v = static_cast<const __nv_bfloat16*>(v);
+    p.k_stride = k_stride, p.v_stride = v_stride;
+    p.k_scale = 1.f / pool->k_scale, p.v_scale = 1.f / pool->v_scale;
+    p.wide = aligned(k, 32) && aligned(v, 32) && k_stride % 16 == 0 && v_stride % 16 == 0;
     DKV_ON_DEVICE(ctx);
-    Kv4StoreParams p{};
-    p.src[0] = static_cast<const __nv_bfloat16*>(k), p.src[1] = static_cast<const __nv_bfloat16*>(v);
-    p.src_stride[0] = k_stride, p.src_stride[1] = v_stride;
-    p.codes[0] = static_cast<uint8_t*>(pool->k_codes), p.codes[1] = static_cast<uint8_t*>(pool->v_codes);
-    p.scales[0] = static_cast<uint8_t*>(pool->k_scales), p.scales[1] = static_cast<uint8_t*>(pool->v_scales);
-    p.inv_scale[0] = 1.f / pool->k_scale, p.inv_scale[1] = 1.f / pool->v_scale;
-    p.slots = slots, p.slots64 = slots_int64;
-    p.n_rows = n_tokens * pool->nh_kv;
-    p.nh = pool->nh_kv;
-    p.n_slots = pool->n_slots;
-    p.status = ctx->status;
-    kv4_store_kernel<<<dim3(static_cast<unsigned>((p.n_rows + 31) / 32), 2), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    kv4_store_kernel<<<static_cast<unsigned>((n_tokens + p.per_block - 1) / p.per_block), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
     DKV_CUDA(cudaGetLastError());
     ctx->launches += 1;
     return DKV_OK;
@@ -176,18 +183,12 @@ int dkv_kv4_load(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, 
     int rc = kv4_rows(ctx, pool, slots, n_tokens);
     if (rc != DKV_OK || n_tokens == 0) return rc;
     DKV_REQUIRE(k != nullptr && v != nullptr && aligned(k, 16) && aligned(v, 16), "k / v must be 16-byte aligned device pointers");
+    Kv4RowsParams p = kv4_rows_params(ctx, pool, slots, slots_int64, n_tokens);
+    p.k_out = static_cast<__nv_bfloat16*>(k), p.v_out = static_cast<__nv_bfloat16*>(v);
+    p.k_scale = pool->k_scale, p.v_scale = pool->v_scale;
+    p.wide = aligned(k, 32) && aligned(v, 32);
     DKV_ON_DEVICE(ctx);
-    Kv4LoadParams p{};
-    p.codes[0] = static_cast<const uint8_t*>(pool->k_codes), p.codes[1] = static_cast<const uint8_t*>(pool->v_codes);
-    p.scales[0] = static_cast<const uint8_t*>(pool->k_scales), p.scales[1] = static_cast<const uint8_t*>(pool->v_scales);
-    p.scale[0] = pool->k_scale, p.scale[1] = pool->v_scale;
-    p.dst[0] = static_cast<__nv_bfloat16*>(k), p.dst[1] = static_cast<__nv_bfloat16*>(v);
-    p.slots = slots, p.slots64 = slots_int64;
-    p.n_rows = n_tokens * pool->nh_kv;
-    p.nh = pool->nh_kv;
-    p.n_slots = pool->n_slots;
-    p.status = ctx->status;
-    kv4_load_kernel<<<dim3(static_cast<unsigned>((p.n_rows + 31) / 32), 2), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    kv4_load_kernel<<<static_cast<unsigned>((n_tokens + p.per_block - 1) / p.per_block), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
     DKV_CUDA(cudaGetLastError());
     ctx->launches += 1;
     return DKV_OK;
@@ -273,10 +274,10 @@ int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* a, void* stream) 
     for (int i = 0; i < 2; ++i) {
         p.heads[i] = nh[i];
         if (nh[i] == 0) continue;
-        DKV_REQUIRE(x[i] != nullptr && y[i] != nullptr && aligned(x[i], 8) && aligned(y[i], 8), "q / k and their outputs must be 8-byte aligned device pointers");
-        DKV_REQUIRE(xs[i] >= static_cast<int64_t>(nh[i]) * 128 && xs[i] % 4 == 0 && ys[i] >= static_cast<int64_t>(nh[i]) * 128 && ys[i] % 4 == 0,
-                    "q / k token strides too small or not a multiple of 4");
-        DKV_REQUIRE(w[i] == nullptr || aligned(w[i], wf[i] ? 16 : 8), "norm weights must be 16-byte (fp32) or 8-byte (bf16) aligned");
+        DKV_REQUIRE(x[i] != nullptr && y[i] != nullptr && aligned(x[i], 16) && aligned(y[i], 16), "q / k and their outputs must be 16-byte aligned device pointers");
+        DKV_REQUIRE(xs[i] >= static_cast<int64_t>(nh[i]) * 128 && xs[i] % 8 == 0 && ys[i] >= static_cast<int64_t>(nh[i]) * 128 && ys[i] % 8 == 0,
+                    "q / k token strides too small or not a multiple of 8");
+        DKV_REQUIRE(w[i] == nullptr || aligned(w[i], 16), "norm weights must be 16-byte aligned");
         p.x[i] = static_cast<const __nv_bfloat16*>(x[i]);
         p.y[i] = static_cast<__nv_bfloat16*>(y[i]);
         p.x_stride[i] = xs[i], p.y_stride[i] = ys[i];
@@ -288,7 +289,13 @@ int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* a, void* stream) 
     p.n_tokens = a->n_tokens;
     p.status = ctx->status;
     DKV_ON_DEVICE(ctx);
-    qk_norm_rope_kernel<<<static_cast<unsigned>((rows + 15) / 16), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // Four heads per eight lanes once that still gives every SM 16 warps, else one.
+    const int q4 = (a->nh_q + 3) / 4, g4 = q4 + (a->nh_k + 3) / 4;
+    if (a->n_tokens * g4 >= static_cast<int64_t>(ctx->sm_count) * 64)
+        qk_norm_rope_kernel<4><<<static_cast<unsigned>((a->n_tokens * g4 + 31) / 32), 256, 0, st>>>(p, q4, g4);
+    else
+        qk_norm_rope_kernel<1><<<static_cast<unsigned>((rows + 31) / 32), 256, 0, st>>>(p, a->nh_q, a->nh_q + a->nh_k);
     DKV_CUDA(cudaGetLastError());
     ctx->launches += 1;
     return DKV_OK;
@@ -322,7 +329,8 @@ int dkv_assign_pages(dkv_context* ctx, const dkv_pages_args* a, int32_t* slots, 
     DKV_REQUIRE(cu_new != nullptr && (a->batch == 0 || seq_lens != nullptr), "seq_lens / cu_new must not be NULL");
     p.slots = slots, p.positions = positions, p.capacity = capacity, p.seq_lens = seq_lens, p.cu_new = cu_new;
     DKV_ON_DEVICE(ctx);
-    const int64_t want = (capacity + kPagesThreads - 1) / kPagesThreads;
+    p.vector = aligned(slots, 16) && aligned(positions, 16);
+    const int64_t want = (capacity + 4 * kPagesThreads - 1) / (4 * kPagesThreads);
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, ctx->sm_count * 2)));
     pages_kernel<false><<<grid, kPagesThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
     DKV_CUDA(cudaGetLastError());
@@ -336,7 +344,7 @@ int dkv_release_pages(dkv_context* ctx, const dkv_pages_args* a, void* stream) {
     if (rc != DKV_OK || a->batch == 0) return rc;
     DKV_ON_DEVICE(ctx);
     const int64_t most = std::min<int64_t>(static_cast<int64_t>(a->batch) * p.max_pages, p.free_cap);
-    const int64_t want = (most + 4 * kPagesThreads - 1) / (4 * kPagesThreads);
+    const int64_t want = (most + kPagesThreads - 1) / kPagesThreads;
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, ctx->sm_count)));
     pages_kernel<true><<<grid, kPagesThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
     DKV_CUDA(cudaGetLastError());

@@ -33,6 +33,7 @@ struct PagesParams {
     int* slots;                      // assign only, [capacity]
     int* positions;                  // [capacity] or nullptr
     long long capacity;
+    int vector;                      // slots and positions are 16-byte aligned
     int* seq_lens;                   // [batch]: lens + more
     int* cu_new;                     // [batch + 1]
     unsigned int* status;
@@ -121,27 +122,48 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(const PagesParams 
                 if (p.positions != nullptr) p.positions[v] = 0;
             }
         } else {
-            for (long long v = me; v < tok; v += stride) {
-                int lo = 0, hi = p.batch - 1;         // largest b with cu_tok[b] <= v (empty requests fall out)
+            // Four tokens per thread: one search, and one look at the table or the stack as long as the page is the same.
+            for (long long v0 = me * 4; v0 < tok; v0 += stride * 4) {
+                int lo = 0, hi = p.batch - 1;         // largest b with cu_tok[b] <= v0 (empty requests fall out)
                 while (lo < hi) {
                     const int mid = (lo + hi + 1) >> 1;
-                    if (cu_tok[mid] <= v) lo = mid;
+                    if (cu_tok[mid] <= v0) lo = mid;
                     else hi = mid - 1;
                 }
-                const int len = p.lens[lo];
-                const int pos = len + static_cast<int>(v - cu_tok[lo]);
-                const int have = static_cast<int>((static_cast<long long>(len) + P - 1) >> p.page_shift);
-                const int pg = pos >> p.page_shift;
-                int* entry = p.page_table + (p.rows != nullptr ? p.rows[lo] : lo) * p.pt_stride + pg;
-                int number;
-                if (pg >= have) {
-                    number = p.free_pages[top - 1 - (cu_page[lo] + pg - have)];
-                    if ((pos & (P - 1)) == 0) *entry = number;
-                } else {
-                    number = *entry;
+                const int n = static_cast<int>(min(tok - v0, 4ll));
+                int slot[4], where[4], len = 0, have = 0, page = -1, number = 0;
+                int* line = nullptr;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i >= n) break;
+                    const int v = static_cast<int>(v0) + i;
+                    while (v >= cu_tok[lo + 1]) ++lo, line = nullptr;
+                    if (line == nullptr) {
+                        len = p.lens[lo];
+                        have = static_cast<int>((static_cast<long long>(len) + P - 1) >> p.page_shift);
+                        line = p.page_table + (p.rows != nullptr ? p.rows[lo] : lo) * p.pt_stride;
+                        page = -1;
+                    }
+                    const int pos = len + (v - cu_tok[lo]), pg = pos >> p.page_shift;
+                    if (pg != page) {
+                        page = pg;
+                        number = pg >= have ? p.free_pages[top - 1 - (cu_page[lo] + pg - have)] : line[pg];
+                    }
+                    if (pg >= have && (pos & (P - 1)) == 0) line[pg] = number;
+                    slot[i] = number >= 0 && number <= (0x7fffffff >> p.page_shift) ? number * P + (pos & (P - 1)) : -1;
+                    where[i] = pos;
                 }
-                p.slots[v] = number >= 0 && number <= (0x7fffffff >> p.page_shift) ? number * P + (pos & (P - 1)) : -1;
-                if (p.positions != nullptr) p.positions[v] = pos;
+                if (n == 4 && p.vector) {
+                    *reinterpret_cast<int4*>(p.slots + v0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+                    if (p.positions != nullptr) *reinterpret_cast<int4*>(p.positions + v0) = make_int4(where[0], where[1], where[2], where[3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (i >= n) break;
+                        p.slots[v0 + i] = slot[i];
+                        if (p.positions != nullptr) p.positions[v0 + i] = where[i];
+                    }
+                }
             }
         }
     } else if (ok) {

@@ -401,8 +401,8 @@ int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_
 /*
  * RMS norm of every query and key head (x / sqrt(mean(x^2) + eps) * weight; weight NULL: no norm) and the Neox rotation at
  * the tokens' positions (cos_sin NULL: none) in one pass, computed in fp32.  q [n_tokens, nh_q, 128], k
- * [n_tokens, nh_k, 128] bf16 device with token strides in elements (multiples of 4); outputs likewise, in place when they are the
- * inputs.  Weights are [128], or [heads, 128] with *_per_head, bf16 or fp32.  A position outside the table leaves the
+ * [n_tokens, nh_k, 128] bf16 device 16-byte aligned with token strides in elements (multiples of 8); outputs likewise, in place when they are
+ * the inputs.  Weights are [128], or [heads, 128] with *_per_head, bf16 or fp32.  A position outside the table leaves the
  * token unrotated (DKV_STATUS_BAD_POSITION).  nh_q or nh_k may be 0.
  */
 typedef struct {
