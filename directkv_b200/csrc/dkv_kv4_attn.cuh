@@ -61,6 +61,7 @@ struct Kv4AttnParams {
     int n_pages;                     // pages that begin inside the pool
     int batch, n_q, nh_q, nh_kv, group;
     int cols;                        // n_q * group: columns of one KV head
+    int whole;                       // no segment is split: the list has one entry per segment, and nothing is left to merge
     int n_cc;                        // column chunks of 8 * NT
     int hg, ts, n_hg;                // heads and token lanes of a block (hg * ts <= kKv4Warps<NT>), head groups
     float scale_log2;                // softmax scale * k_scale * log2(e)
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
             const int code = kv4_length(p, b, &row);
             if (code < 0 && blockIdx.x == 0) atomicOr(p.status, kStatusBadPage);
             const int len = kv4_clean_length(p, code);
-            n = max(1, static_cast<int>((static_cast<long long>(len) + kKv4Tile * p.ts - 1) / (kKv4Tile * p.ts)));
+            n = p.whole ? 1 : max(1, static_cast<int>((static_cast<long long>(len) + kKv4Tile * p.ts - 1) / (kKv4Tile * p.ts)));
         }
         int inc = n;
 #pragma unroll
@@ -206,15 +207,16 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
             else hi = mid - 1;
         }
         const int b = lo;
-        const int tiles = cum[b + 1] - cum[b];
+        const int entries = cum[b + 1] - cum[b];
         const long long r = x - static_cast<long long>(cum[b]) * per_tile;
-        const int seg = static_cast<int>(r / tiles), tile0 = static_cast<int>(r - static_cast<long long>(seg) * tiles);
-        const int n_tiles = static_cast<int>(min(static_cast<long long>(tiles - tile0), x1 - x));
-        const int hgi = seg / p.n_cc, cc = seg - hgi * p.n_cc;
-        const bool whole = n_tiles == tiles;
-        const int kvh = hgi * p.hg + hl;
+        const int seg = static_cast<int>(r / entries), tile0 = static_cast<int>(r - static_cast<long long>(seg) * entries);
         long long row;
         const int len = kv4_clean_length(p, kv4_length(p, b, &row));
+        const int taken = static_cast<int>(min(static_cast<long long>(entries - tile0), x1 - x));
+        const int n_tiles = p.whole ? (len + kKv4Tile * p.ts - 1) / (kKv4Tile * p.ts) : taken;
+        const int hgi = seg / p.n_cc, cc = seg - hgi * p.n_cc;
+        const bool whole = taken == entries;
+        const int kvh = hgi * p.hg + hl;
         const int* table = p.page_table + row * p.pt_stride;
 
         if (active) {
@@ -551,7 +553,7 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
                     }
                 }
         }
-        x += n_tiles;
+        x += taken;
     }
 }
 

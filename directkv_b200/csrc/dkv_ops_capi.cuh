@@ -46,6 +46,7 @@ void kv4_block_shape(int nh_kv, int warps, int* hg, int* ts) {
     }
 }
 
+constexpr int kKv4WholeSteps = 9;      // (tables of up to 8 steps)
 constexpr size_t kKv4CumBytes = (kKv4LaunchBatch + 1) * sizeof(int) / 256 * 256 + 256;
 
 template <int NT>
@@ -69,15 +70,20 @@ int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
     kv4_block_shape(p.nh_kv, kKv4Warps<NT>, &p.hg, &p.ts);
     p.n_hg = p.nh_kv / p.hg;
     p.n_cc = (p.cols + 8 * NT - 1) / (8 * NT);
+    const int64_t most_parts = (static_cast<int64_t>(p.max_pages) << p.page_shift) / (kKv4Tile * p.ts) + 1;
+    // A table with room for a few steps only: splitting them costs more (a second launch and the records' way through
+    // memory) than doing them one behind the other.
+    p.whole = most_parts <= kKv4WholeSteps;
     const int grid = kv4_grid<NT>(ctx);
     const size_t smem = kv4_smem<NT>(p.batch);
     if (p.page_shift >= 4) kv4_attn_kernel<NT, true><<<grid, kKv4Warps<NT> * 32, smem, st>>>(p);
     else kv4_attn_kernel<NT, false><<<grid, kKv4Warps<NT> * 32, smem, st>>>(p);
     DKV_CUDA(cudaGetLastError());
+    ctx->launches += 1;
+    if (p.whole) return DKV_OK;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.n_q * p.nh_q);
     // Few rows: many blocks had a part of each.
-    const int64_t most_parts = (static_cast<int64_t>(p.max_pages) << p.page_shift) / (kKv4Tile * p.ts) + 1;
     const bool few = cfg.gridDim.x <= static_cast<unsigned>(2 * ctx->sm_count) && most_parts > 16;
     cfg.blockDim = dim3(few ? 512 : 128);
     cfg.dynamicSmemBytes = grid * sizeof(float2);
@@ -89,7 +95,7 @@ int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
     cfg.numAttrs = 1;
     if (few) DKV_CUDA(cudaLaunchKernelEx(&cfg, kv4_merge_kernel<NT, 16>, p, grid));
     else DKV_CUDA(cudaLaunchKernelEx(&cfg, kv4_merge_kernel<NT, 4>, p, grid));
-    ctx->launches += 2;
+    ctx->launches += 1;
     return DKV_OK;
 }
 
@@ -290,12 +296,12 @@ int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* a, void* stream) 
     p.status = ctx->status;
     DKV_ON_DEVICE(ctx);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // Four heads per eight lanes once that still gives every SM 16 warps, else one.
-    const int q4 = (a->nh_q + 3) / 4, g4 = q4 + (a->nh_k + 3) / 4;
-    if (a->n_tokens * g4 >= static_cast<int64_t>(ctx->sm_count) * 64)
-        qk_norm_rope_kernel<4><<<static_cast<unsigned>((a->n_tokens * g4 + 31) / 32), 256, 0, st>>>(p, q4, g4);
+    // Eight heads per half warp once that still gives every SM 32 warps, else one.
+    const int qn = (a->nh_q + 7) / 8, gn = qn + (a->nh_k + 7) / 8;
+    if (a->n_tokens * gn >= static_cast<int64_t>(ctx->sm_count) * 64)
+        qk_norm_rope_kernel<8, 16><<<static_cast<unsigned>((a->n_tokens * gn + 3) / 4), 64, 0, st>>>(p, qn, gn);
     else
-        qk_norm_rope_kernel<1><<<static_cast<unsigned>((rows + 31) / 32), 256, 0, st>>>(p, a->nh_q, a->nh_q + a->nh_k);
+        qk_norm_rope_kernel<1, 16><<<static_cast<unsigned>((rows + 3) / 4), 64, 0, st>>>(p, a->nh_q, a->nh_q + a->nh_k);
     DKV_CUDA(cudaGetLastError());
     ctx->launches += 1;
     return DKV_OK;

@@ -25,95 +25,120 @@ struct QkNormParams {
     unsigned int* status;
 };
 
-__device__ __forceinline__ void unpack8(const uint4& u, float (&o)[8]) {
-    o[0] = bf16lo(u.x), o[1] = bf16hi(u.x), o[2] = bf16lo(u.y), o[3] = bf16hi(u.y);
-    o[4] = bf16lo(u.z), o[5] = bf16hi(u.z), o[6] = bf16lo(u.w), o[7] = bf16hi(u.w);
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 
-__device__ __forceinline__ void load_f32x8(const float* p, float (&o)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
+// Four values as two pairs.
+__device__ __forceinline__ void unpack4(const uint2& u, uint64_t (&o)[2]) {
+    o[0] = f32x2(bf16lo(u.x), bf16hi(u.x)), o[1] = f32x2(bf16lo(u.y), bf16hi(u.y));
 }
 
-__device__ __forceinline__ void load_weight8(const void* w, int is_f32, int at, float (&o)[8]) {
-    if (is_f32) load_f32x8(static_cast<const float*>(w) + at, o);
-    else unpack8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w) + at), o);
+__device__ __forceinline__ void load_f32x4(const float* p, uint64_t (&o)[2]) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    o[0] = f32x2(a.x, a.y), o[1] = f32x2(a.z, a.w);
 }
 
-// Eight lanes per row: lane l holds dimensions 8 l .. 8 l + 7 and 64 + 8 l .. 64 + 8 l + 7, two 16-byte loads.  The eight
-// lanes take R heads of one token, so that the angles (512 bytes per token, as much as two rows) and the weights are
-// loaded once for all of them and R rows are on their way at a time.
-template <int R>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkNormParams p, int q_groups, int groups) {
-    const int l = threadIdx.x & 7;
-    const long long id = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 3;
-    const bool live = id < p.n_tokens * groups;
-    const long long tok = live ? (id < 0x7fffffff ? static_cast<unsigned>(id) / static_cast<unsigned>(groups) : id / groups) : 0;
-    const int grp = live ? static_cast<int>(id - tok * groups) : 0;
+__device__ __forceinline__ void load_weight4(const void* w, int is_f32, int at, uint64_t (&o)[2]) {
+    if (is_f32) load_f32x4(static_cast<const float*>(w) + at, o);
+    else unpack4(*reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(w) + at), o);
+}
+
+__device__ __forceinline__ uint2 pack4(const uint64_t (&v)[2]) {
+    float a, b, c, d;
+    f32x2_split(v[0], a, b);
+    f32x2_split(v[1], c, d);
+    return make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+}
+
+// Half a warp per row: lane l holds dimensions 4 l .. 4 l + 3 and 64 + 4 l .. 64 + 4 l + 3.  The sixteen lanes take R heads of
+// one token: the angles (512 bytes per token, as much as two rows) and the weights are loaded and
+// multiplied with one another once for all of them, y = inv (u A - v B), inv (v C + u D), and R rows are on their way at a time.
+template <int R, int BLOCKS>
+__global__ void __launch_bounds__(64, BLOCKS) qk_norm_rope_kernel(const QkNormParams p, int q_groups, int groups) {
+    const int l = threadIdx.x & 15;
+    const long long id = (static_cast<long long>(blockIdx.x) * 64 + threadIdx.x) >> 4;
+    if (id >= p.n_tokens * groups) return;                // by halves of a warp
+    const long long tok = id < 0x7fffffff ? static_cast<unsigned>(id) / static_cast<unsigned>(groups) : id / groups;
+    const int grp = static_cast<int>(id - tok * groups);
     const int which = grp >= q_groups ? 1 : 0;
-    const int h0 = (which ? grp - q_groups : grp) * R, n = live ? min(R, p.heads[which] - h0) : 0;
-    const __nv_bfloat16* x = (which ? p.x[1] + tok * p.x_stride[1] : p.x[0] + tok * p.x_stride[0]) + h0 * 128 + l * 8;
-    __nv_bfloat16* y = (which ? p.y[1] + tok * p.y_stride[1] : p.y[0] + tok * p.y_stride[0]) + h0 * 128 + l * 8;
+    const int h0 = (which ? grp - q_groups : grp) * R, n = min(R, p.heads[which] - h0);
+    const __nv_bfloat16* x = (which ? p.x[1] + tok * p.x_stride[1] : p.x[0] + tok * p.x_stride[0]) + h0 * 128 + l * 4;
+    uint2 a[R], b[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (i < n) {
+            a[i] = *reinterpret_cast<const uint2*>(x + i * 128);
+            b[i] = *reinterpret_cast<const uint2*>(x + i * 128 + 64);
+        }
+    }
     const void* weight = which ? p.weight[1] : p.weight[0];
     const int weight_f32 = which ? p.weight_f32[1] : p.weight_f32[0], weight_stride = which ? p.weight_stride[1] : p.weight_stride[0];
-    uint4 a[R], b[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-        if (i < n) {
-            a[i] = __ldcs(reinterpret_cast<const uint4*>(x + i * 128));
-            b[i] = __ldcs(reinterpret_cast<const uint4*>(x + i * 128 + 64));
-        }
-    float c[8], s[8], wl[8], wh[8];
+    uint64_t ca[2], cb[2], cc[2], cd[2];                  // A, -B, C, D
     bool turn = false;
-    if (p.cos_sin != nullptr && live) {
+    const uint64_t one = f32x2(1.f, 1.f);
+#pragma unroll
+    for (int d = 0; d < 2; ++d) ca[d] = cc[d] = one, cb[d] = cd[d] = 0;
+    if (p.cos_sin != nullptr) {
         const long long pos = p.pos64 ? static_cast<const long long*>(p.positions)[tok]
                                       : static_cast<long long>(static_cast<const int*>(p.positions)[tok]);
         turn = pos >= 0 && pos < p.max_pos;
         if (turn) {
-            load_f32x8(p.cos_sin + pos * 128 + l * 8, c);
-            load_f32x8(p.cos_sin + pos * 128 + 64 + l * 8, s);
+            load_f32x4(p.cos_sin + pos * 128 + l * 4, ca);
+            load_f32x4(p.cos_sin + pos * 128 + 64 + l * 4, cd);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) cc[d] = ca[d], cb[d] = cd[d] ^ 0x8000000080000000ull;
         } else if (l == 0) {
             atomicOr(p.status, kStatusBadPosition);
         }
     }
+    uint64_t wl[2], wh[2];
     if (weight != nullptr && weight_stride == 0) {
-        load_weight8(weight, weight_f32, l * 8, wl);
-        load_weight8(weight, weight_f32, l * 8 + 64, wh);
+        load_weight4(weight, weight_f32, l * 4, wl);
+        load_weight4(weight, weight_f32, l * 4 + 64, wh);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            ca[d] = mul_f32x2(ca[d], wl[d]), cb[d] = mul_f32x2(cb[d], wh[d]);
+            cc[d] = mul_f32x2(cc[d], wh[d]), cd[d] = mul_f32x2(cd[d], wl[d]);
+        }
     }
+    __nv_bfloat16* y = (which ? p.y[1] + tok * p.y_stride[1] : p.y[0] + tok * p.y_stride[0]) + h0 * 128 + l * 4;
+    const unsigned half = 0xffffu << (threadIdx.x & 16);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        if (i >= n) a[i] = b[i] = make_uint4(0u, 0u, 0u, 0u);
-        float lo[8], hi[8];
-        unpack8(a[i], lo), unpack8(b[i], hi);
+        if (i >= n) break;
+        uint64_t lo[2], hi[2];
+        unpack4(a[i], lo), unpack4(b[i], hi);
+        uint64_t inv = one;
         if (weight != nullptr) {
-            float ss = 0.f;
+            uint64_t sq = mul_f32x2(lo[0], lo[0]), sr = mul_f32x2(hi[0], hi[0]);
 #pragma unroll
-            for (int d = 0; d < 8; ++d) ss = fmaf(lo[d], lo[d], fmaf(hi[d], hi[d], ss));
-            const unsigned eight = 0xffu << (threadIdx.x & 24);
+            for (int d = 1; d < 2; ++d) sq = fma_f32x2(lo[d], lo[d], sq), sr = fma_f32x2(hi[d], hi[d], sr);
+            float ss, st;
+            f32x2_split(add_f32x2(sq, sr), ss, st);
+            ss += st;
 #pragma unroll
-            for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(eight, ss, o);
-            const float inv = 1.f / sqrtf(ss * (1.f / 128.f) + p.eps);
-            if (weight_stride != 0 && i < n) {
-                load_weight8(weight, weight_f32, (h0 + i) * weight_stride + l * 8, wl);
-                load_weight8(weight, weight_f32, (h0 + i) * weight_stride + l * 8 + 64, wh);
-            }
+            for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(half, ss, o);
+            const float r = rsqrtf(ss * (1.f / 128.f) + p.eps);
+            inv = f32x2(r, r);
+            if (weight_stride != 0) {
+                load_weight4(weight, weight_f32, (h0 + i) * weight_stride + l * 4, wl);
+                load_weight4(weight, weight_f32, (h0 + i) * weight_stride + l * 4 + 64, wh);
 #pragma unroll
-            for (int d = 0; d < 8; ++d) lo[d] *= inv * wl[d], hi[d] *= inv * wh[d];
-        }
-        if (turn) {
-#pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                const float u = lo[d], v = hi[d];
-                lo[d] = u * c[d] - v * s[d];
-                hi[d] = v * c[d] + u * s[d];
+                for (int d = 0; d < 2; ++d) lo[d] = mul_f32x2(lo[d], wl[d]), hi[d] = mul_f32x2(hi[d], wh[d]);
             }
         }
-        if (i < n) {
-            *reinterpret_cast<uint4*>(y + i * 128) =
-                make_uint4(pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(lo[4], lo[5]), pack_bf16x2(lo[6], lo[7]));
-            *reinterpret_cast<uint4*>(y + i * 128 + 64) =
-                make_uint4(pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3]), pack_bf16x2(hi[4], hi[5]), pack_bf16x2(hi[6], hi[7]));
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            const uint64_t u = mul_f32x2(lo[d], inv), v = mul_f32x2(hi[d], inv);
+            lo[d] = mul_f32x2(u, ca[d]);
+            hi[d] = mul_f32x2(v, cc[d]);
+            if (turn) lo[d] = fma_f32x2(v, cb[d], lo[d]), hi[d] = fma_f32x2(u, cd[d], hi[d]);
         }
+        __stcs(reinterpret_cast<uint2*>(y + i * 128), pack4(lo));
+        __stcs(reinterpret_cast<uint2*>(y + i * 128 + 64), pack4(hi));
     }
 }
 

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -376,7 +377,14 @@ def stream_copy(dst: torch.Tensor, src: torch.Tensor) -> None:
 # ---------------------------------------------------------------------------
 # A paged cache held in 4 bits, and what a decode step over it needs beside the attention
 # ---------------------------------------------------------------------------
+# These calls are short on the GPU, so the host side is kept short too: arguments are packed straight into the C structs' bytes, and a
+# contiguous tensor is recognised by one question.
 KV4_BLOCK = 16          # consecutive dimensions that share a scale
+_BF16, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
+_protos = {}            # device -> an empty bf16 tensor there, to allocate like
+_pack_decode_kv4 = struct.Struct("@iiiPqPqPPqiiPfP").pack     # _lib.DecodeKv4Args
+_pack_qk_norm = struct.Struct("@qiiPqPqPqPqPPiiiiPiPif").pack  # _lib.QkNormArgs
+_pack_pages = struct.Struct("@PqiiPPPiiPiP").pack              # _lib.PagesArgs
 
 
 def _call(dev: int):
@@ -385,29 +393,45 @@ def _call(dev: int):
     return ctx.handle, torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _on_device(dev: int, named) -> None:
-    for t, name in named:
-        if t is not None and (dev < 0 or t.get_device() != dev):
-            raise RuntimeError(f"{name} must be a CUDA tensor on the same device as the other tensors")
+def _contiguous_pair(like: torch.Tensor, shape_a, shape_b):
+    """Two contiguous tensors of like's type and device in one allocation (an allocation costs as much as the rest of a
+    short call's host side)."""
+    na, nb = math.prod(shape_a), math.prod(shape_b)
+    flat = like.new_empty(na + nb)
+    ra, rb = shape_a[-2] * HEAD_DIM, shape_b[-2] * HEAD_DIM
+    return flat.as_strided(shape_a, (ra, HEAD_DIM, 1)), flat.as_strided(shape_b, (rb, HEAD_DIM, 1), na)
+
+
+def _elsewhere(name: str) -> None:
+    raise RuntimeError(f"{name} must be a CUDA tensor on the same device as the other tensors")
 
 
 def _int32_1d(t: torch.Tensor, n: int, name: str) -> None:
-    if t.dtype is not torch.int32 or t.dim() != 1 or t.size(0) != n or not t.is_contiguous():
+    if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():
         raise RuntimeError(f"{name} must be a contiguous int32 tensor of {n} entries")
 
 
 def _heads_stride(t: torch.Tensor, name: str) -> int:
     """Elements from token to token of ``[..., NH, 128]`` whose heads lie next to each other (a slice of a fused
     projection's output is fine)."""
-    shape, st = t.shape, t.stride()
-    if t.dtype is not torch.bfloat16 or len(shape) < 3 or shape[-1] != HEAD_DIM or st[-1] != 1 or (st[-2] != HEAD_DIM and shape[-2] > 1):
-        raise RuntimeError(f"{name} must be bfloat16 [..., NH, {HEAD_DIM}] with the heads of a token next to each other")
-    row = shape[-2] * HEAD_DIM
-    if len(shape) == 3:
-        return st[0] if shape[0] > 1 else row
-    if len(shape) != 4 or (shape[0] > 1 and shape[1] > 1 and st[0] != shape[1] * st[1]):
-        raise RuntimeError(f"{name} must be 3D or 4D with evenly spaced tokens")
-    return st[1] if shape[1] > 1 else (st[0] if shape[0] > 1 else row)
+    shape = t.shape
+    if t.dtype is _BF16 and len(shape) in (3, 4) and shape[-1] == HEAD_DIM:
+        row = shape[-2] * HEAD_DIM
+        if t.is_contiguous():
+            return row
+        st = t.stride()
+        if st[-1] == 1 and (st[-2] == HEAD_DIM or shape[-2] == 1):
+            if len(shape) == 3:
+                return st[0] if shape[0] > 1 else row
+            if shape[0] == 1 or shape[1] == 1 or st[0] == shape[1] * st[1]:
+                return st[1] if shape[1] > 1 else (st[0] if shape[0] > 1 else row)
+            raise RuntimeError(f"{name} must have evenly spaced tokens")
+    raise RuntimeError(f"{name} must be bfloat16 [..., NH, {HEAD_DIM}], 3D or 4D, with the heads of a token next to each other")
+
+
+def _check_page_table(t: torch.Tensor) -> None:
+    if t.dtype is not _I32 or t.dim() != 2 or not (t.is_contiguous() or t.stride(1) == 1):
+        raise RuntimeError("page_table must be 2D int32 with unit inner stride")
 
 
 class KV4Pool:
@@ -439,6 +463,8 @@ class KV4Pool:
         self.page_size, self.k_scale, self.v_scale = int(page_size), float(k_scale), float(v_scale)
         self.n_slots, self.nh_kv = n_slots, nh
         self._descs = {}
+        if k_codes.is_cuda:
+            self._resolve(k_codes.get_device())
 
     @classmethod
     def empty(cls, n_slots: int, nh_kv: int, page_size: int = 1, device="cuda", k_scale: float = 1.0, v_scale: float = 1.0) -> "KV4Pool":
@@ -457,23 +483,22 @@ class KV4Pool:
     def nbytes(self) -> int:
         return 2 * self.n_slots * self.nh_kv * (HEAD_DIM // 2 + HEAD_DIM // KV4_BLOCK)
 
-    def _ref(self, dev: int, handle):
-        """The C struct for one device, checked and resolved by the library on first use."""
-        ref = self._descs.get(dev)
-        if ref is None:
-            if self.k_codes.is_cuda and self.k_codes.get_device() != dev:
-                raise RuntimeError("the pool must be on the device of the other tensors")
-            d = _lib.Kv4PoolDesc(_ptr(self.k_codes), _ptr(self.k_scales), _ptr(self.v_codes), _ptr(self.v_scales), self.n_slots,
-                                 self.nh_kv, self.page_size, self.k_scale, self.v_scale, 0)
-            _lib.check(_lib.load().dkv_kv4_pool_resolve(handle, C.byref(d)))
-            ref = self._descs[dev] = C.byref(d)
+    def _resolve(self, dev: int):
+        """The C struct for one device, checked and resolved by the library on first use (never under stream capture: it
+        makes room for the attention's workspace)."""
+        if self.k_codes.is_cuda and self.k_codes.get_device() != dev:
+            raise RuntimeError("the pool must be on the device of the other tensors")
+        d = _lib.Kv4PoolDesc(_ptr(self.k_codes), _ptr(self.k_scales), _ptr(self.v_codes), _ptr(self.v_scales), self.n_slots,
+                             self.nh_kv, self.page_size, self.k_scale, self.v_scale, 0)
+        _lib.check(_lib.load().dkv_kv4_pool_resolve((_lib._contexts.get(dev) or get_context(dev)).handle, C.byref(d)))
+        self._descs[dev] = ref = C.byref(d)
         return ref
 
 
 def _check_slots(slots: torch.Tensor) -> int:
-    if slots.dtype not in (torch.int32, torch.int64) or slots.dim() != 1 or not slots.is_contiguous():
+    if (slots.dtype is not _I32 and slots.dtype is not _I64) or slots.dim() != 1 or not slots.is_contiguous():
         raise RuntimeError("slots must be a contiguous 1D int32 or int64 tensor")
-    return slots.size(0)
+    return slots.numel()
 
 
 def store_kv4(pool: KV4Pool, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -483,15 +508,17 @@ def store_kv4(pool: KV4Pool, slots: torch.Tensor, k: torch.Tensor, v: torch.Tens
     value) and not-a-numbers (stored as zero).  Slots must be distinct, save for a padding slot that nobody attends.
     """
     n = _check_slots(slots)
-    if k.dim() != 3 or v.dim() != 3 or k.size(0) != n or v.size(0) != n or k.size(1) != pool.nh_kv or v.size(1) != pool.nh_kv:
+    want = (n, pool.nh_kv, HEAD_DIM)
+    if k.shape != want or v.shape != want:
         raise RuntimeError(f"k and v must be [{n}, {pool.nh_kv}, {HEAD_DIM}]")
     ks, vs = _heads_stride(k, "k"), _heads_stride(v, "v")
     dev = k.get_device()
-    _on_device(dev, ((k, "k"), (v, "v"), (slots, "slots")))
+    if dev < 0 or v.get_device() != dev or slots.get_device() != dev:
+        _elsewhere("k, v and slots each")
     if n == 0:
         return
     handle, stream = _call(dev)
-    rc = _lib.load().dkv_kv4_store(handle, pool._ref(dev, handle), slots.data_ptr(), slots.dtype is torch.int64, k.data_ptr(), ks,
+    rc = _lib.load().dkv_kv4_store(handle, pool._descs.get(dev) or pool._resolve(dev), slots.data_ptr(), slots.dtype is _I64, k.data_ptr(), ks,
                                    v.data_ptr(), vs, n, stream)
     if rc:
         _lib.check(rc)
@@ -502,20 +529,26 @@ def load_kv4(pool: KV4Pool, slots: torch.Tensor, k_out: Optional[torch.Tensor] =
     is reported in the status word."""
     n = _check_slots(slots)
     dev = slots.get_device()
-    _on_device(dev, ((slots, "slots"),))
+    if dev < 0:
+        _elsewhere("slots")
     shape = (n, pool.nh_kv, HEAD_DIM)
+    if k_out is None and v_out is None:
+        proto = _protos.get(dev)
+        if proto is None:
+            proto = _protos[dev] = torch.empty(0, dtype=_BF16, device=slots.device)
+        k_out, v_out = _contiguous_pair(proto, shape, shape)
     if k_out is None:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
+        k_out = torch.empty(shape, dtype=_BF16, device=slots.device)
+    elif k_out.dtype is not _BF16 or k_out.shape != shape or not k_out.is_contiguous() or k_out.get_device() != dev:
+        raise RuntimeError(f"k_out must be contiguous bfloat16 [{n}, {pool.nh_kv}, {HEAD_DIM}] on the device of slots")
     if v_out is None:
-        v_out = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
-    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
-        if t.dtype is not torch.bfloat16 or t.shape != shape or not t.is_contiguous():
-            raise RuntimeError(f"{name} must be contiguous bfloat16 [{n}, {pool.nh_kv}, {HEAD_DIM}]")
-    _on_device(dev, ((k_out, "k_out"), (v_out, "v_out")))
+        v_out = torch.empty_like(k_out)
+    elif v_out.dtype is not _BF16 or v_out.shape != shape or not v_out.is_contiguous() or v_out.get_device() != dev:
+        raise RuntimeError(f"v_out must be contiguous bfloat16 [{n}, {pool.nh_kv}, {HEAD_DIM}] on the device of slots")
     if n:
         handle, stream = _call(dev)
-        rc = _lib.load().dkv_kv4_load(handle, pool._ref(dev, handle), slots.data_ptr(), slots.dtype is torch.int64, k_out.data_ptr(),
-                                      v_out.data_ptr(), n, stream)
+        rc = _lib.load().dkv_kv4_load(handle, pool._descs.get(dev) or pool._resolve(dev), slots.data_ptr(), slots.dtype is _I64,
+                                      k_out.data_ptr(), v_out.data_ptr(), n, stream)
         if rc:
             _lib.check(rc)
     return k_out, v_out
@@ -536,44 +569,82 @@ def decode_kv4(
     With ``n_q`` query tokens per request, token ``j`` attends the first ``seq_lens - n_q + 1 + j`` stored tokens (drafted
     tokens under verification, a short chunk of a prompt).  A row that attends nothing is zero, its LSE -inf.
     """
-    flat = q.dim() == 2
-    if flat and (q.size(1) % HEAD_DIM or q.size(1) == 0):
-        raise RuntimeError(f"q must be [B, NH_q*{HEAD_DIM}]")
-    q3 = q.view(q.size(0), -1, HEAD_DIM) if flat else q
-    qs = _heads_stride(q3, "q")
-    b, nh_q = q3.size(0), q3.size(-2)
-    n_q = q3.size(1) if q3.dim() == 4 else 1
+    shape = q.shape
+    nd = len(shape)
+    if nd == 3:
+        b, nh_q, _ = shape
+        n_q = 1
+        qs = _heads_stride(q, "q")
+    elif nd == 2:
+        if shape[1] % HEAD_DIM or shape[1] == 0:
+            raise RuntimeError(f"q must be [B, NH_q*{HEAD_DIM}]")
+        b, nh_q, n_q = shape[0], shape[1] // HEAD_DIM, 1
+        qs = _heads_stride(q.view(b, nh_q, HEAD_DIM), "q")
+    else:
+        qs = _heads_stride(q, "q")
+        b, n_q, nh_q, _ = shape
     if nh_q == 0 or nh_q % pool.nh_kv:
         raise RuntimeError(f"q has {nh_q} heads, not a multiple of the pool's {pool.nh_kv}")
     if b > 4096 or not 1 <= n_q <= 1024:
         raise RuntimeError(f"{b} requests of {n_q} query tokens: at most 4096 of 1 to 1024")
     _int32_1d(seq_lens, b, "seq_lens")
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 and page_table.size(1) > 1:
-        raise RuntimeError("page_table must be 2D int32 with unit inner stride")
+    _check_page_table(page_table)
+    rows, max_pages = page_table.shape
+    dev = q.get_device()
+    row_ptr = lse_ptr = 0
     if row_map is not None:
         _int32_1d(row_map, b, "row_map")
-    elif page_table.size(0) < b:
-        raise RuntimeError(f"page_table has {page_table.size(0)} rows for {b} requests")
-    if lse_out is not None and (lse_out.dtype is not torch.float32 or lse_out.numel() != b * n_q * nh_q or not lse_out.is_contiguous()):
-        raise RuntimeError("lse_out must be contiguous fp32 with one entry per query row")
-    dev = q.get_device()
-    _on_device(dev, ((q, "q"), (seq_lens, "seq_lens"), (page_table, "page_table"), (row_map, "row_map"), (lse_out, "lse_out")))
+        if row_map.get_device() != dev:
+            _elsewhere("row_map")
+        row_ptr = row_map.data_ptr()
+    elif rows < b:
+        raise RuntimeError(f"page_table has {rows} rows for {b} requests")
+    if lse_out is not None:
+        if lse_out.dtype is not _F32 or lse_out.numel() != b * n_q * nh_q or not lse_out.is_contiguous() or lse_out.get_device() != dev:
+            raise RuntimeError("lse_out must be contiguous fp32 CUDA with one entry per query row")
+        lse_ptr = lse_out.data_ptr()
+    if dev < 0 or seq_lens.get_device() != dev or page_table.get_device() != dev:
+        _elsewhere("q, seq_lens and page_table each")
+    row = nh_q * HEAD_DIM
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-        os = nh_q * HEAD_DIM
+        out = torch.empty_like(q) if qs == row and q.is_contiguous() else torch.empty(shape, dtype=_BF16, device=q.device)
+        os = row
     else:
-        if out.shape != q.shape or out.get_device() != dev:
+        if out.shape != shape or out.get_device() != dev:
             raise RuntimeError("out must have q's shape and device")
-        os = _heads_stride(out.view(b, -1, HEAD_DIM) if flat else out, "out")
+        os = _heads_stride(out.view(b, nh_q, HEAD_DIM) if nd == 2 else out, "out")
     if b == 0:
         return out
     handle, stream = _call(dev)
-    a = _lib.DecodeKv4Args(b, n_q, nh_q, q.data_ptr(), qs, out.data_ptr(), os, seq_lens.data_ptr(), page_table.data_ptr(),
-                           page_table.stride(0), page_table.size(0), page_table.size(1), _ptr(row_map), softmax_scale, _ptr(lse_out))
-    rc = _lib.load().dkv_decode_kv4(handle, pool._ref(dev, handle), C.byref(a), stream)
+    a = _pack_decode_kv4(b, n_q, nh_q, q.data_ptr(), qs, out.data_ptr(), os, seq_lens.data_ptr(), page_table.data_ptr(),
+                         page_table.stride(0), rows, max_pages, row_ptr, softmax_scale, lse_ptr)
+    rc = _lib.load().dkv_decode_kv4(handle, pool._descs.get(dev) or pool._resolve(dev), a, stream)
     if rc:
         _lib.check(rc)
     return out
+
+
+def _norm_side(x, y, w, n: int, dev: int, name: str):
+    """Output and struct fields of the queries or the keys."""
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != n:
+        raise RuntimeError(f"{name} must be [{n}, NH, {HEAD_DIM}]")
+    xs, nh = _heads_stride(x, name), shape[1]
+    if y is None:
+        # (a slice of a fused projection gives a contiguous output)
+        y, ys = (torch.empty_like(x) if x.is_contiguous() else torch.empty(shape, dtype=_BF16, device=x.device)), nh * HEAD_DIM
+    else:
+        if y.shape != shape or y.get_device() != dev:
+            raise RuntimeError(f"{name}_out must have the shape of {name} and its device")
+        ys = xs if y is x else _heads_stride(y, f"{name}_out")
+    per_head = f32 = w_ptr = 0
+    if w is not None:
+        per_head, f32, w_ptr = w.dim() == 2, w.dtype is _F32, w.data_ptr()
+        if not (f32 or w.dtype is _BF16) or not w.is_contiguous() or w.shape != ((nh, HEAD_DIM) if per_head else (HEAD_DIM,)) or w.get_device() != dev:
+            raise RuntimeError(f"{name}_weight must be contiguous bfloat16 or float32 [{HEAD_DIM}] or [{nh}, {HEAD_DIM}], a CUDA tensor on the device of {name}")
+    if dev < 0 or x.get_device() != dev:
+        _elsewhere(name)
+    return y, nh, x.data_ptr(), xs, y.data_ptr(), ys, w_ptr, f32, per_head
 
 
 def qk_norm_rope(
@@ -595,74 +666,60 @@ def qk_norm_rope(
     lead = q if q is not None else k
     if lead is None:
         raise RuntimeError("q or k must be given")
-    n, dev = lead.size(0), lead.get_device()
-    args, keep = [], []
-    for x, y, w, name in ((q, q_out, q_weight, "q"), (k, k_out, k_weight, "k")):
-        if x is None:
-            keep.append(None)
-            args.append((0, None, 0, None, 0, None, 0, 0))
-            continue
-        if x.dim() != 3 or x.size(0) != n:
-            raise RuntimeError(f"{name} must be [{n}, NH, {HEAD_DIM}]")
-        xs, nh = _heads_stride(x, name), x.size(1)
-        if y is None:
-            y, ys = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device), nh * HEAD_DIM
-        else:
-            if y.shape != x.shape:
-                raise RuntimeError(f"{name}_out must have the shape of {name}")
-            ys = _heads_stride(y, f"{name}_out")
-        per_head = f32 = 0
-        if w is not None:
-            per_head, f32 = int(w.dim() == 2), int(w.dtype is torch.float32)
-            if (not f32 and w.dtype is not torch.bfloat16) or not w.is_contiguous() or w.size(-1) != HEAD_DIM or w.dim() > 2 or (per_head and w.size(0) != nh):
-                raise RuntimeError(f"{name}_weight must be contiguous bfloat16 or float32, [{HEAD_DIM}] or [{nh}, {HEAD_DIM}]")
-        _on_device(dev, ((x, name), (y, f"{name}_out"), (w, f"{name}_weight")))
-        keep.append(y)
-        args.append((nh, x.data_ptr(), xs, y.data_ptr(), ys, _ptr(w), f32, per_head))
-    max_pos = 0
+    n, dev = lead.shape[0], lead.get_device()
+    if q is not None and k is not None and q_out is None and k_out is None and q.dtype is _BF16 and q.dim() == 3 and k.dim() == 3:
+        q_out, k_out = _contiguous_pair(q, q.shape, k.shape)
+    qy, hq, qp, qs, qo, qos, qw, qf, qh = _norm_side(q, q_out, q_weight, n, dev, "q") if q is not None else (None, 0, 0, 0, 0, 0, 0, 0, 0)
+    ky, hk, kp, ks, ko, kos, kw, kf, kh = _norm_side(k, k_out, k_weight, n, dev, "k") if k is not None else (None, 0, 0, 0, 0, 0, 0, 0, 0)
+    max_pos = pos_ptr = pos64 = cs_ptr = 0
     if cos_sin is not None:
-        if cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or cos_sin.size(1) != HEAD_DIM or not cos_sin.is_contiguous() or cos_sin.size(0) == 0:
+        if cos_sin.dtype is not _F32 or cos_sin.dim() != 2 or cos_sin.shape[1] != HEAD_DIM or not cos_sin.is_contiguous() or cos_sin.shape[0] == 0:
             raise RuntimeError(f"cos_sin must be contiguous float32 [max_pos, {HEAD_DIM}]")
-        if positions is None or positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1 or positions.size(0) != n or not positions.is_contiguous():
+        pos64 = positions is not None and positions.dtype is _I64
+        if positions is None or not (pos64 or positions.dtype is _I32) or positions.shape != (n,) or not positions.is_contiguous():
             raise RuntimeError(f"positions must be a contiguous int32 or int64 tensor of {n} entries")
-        _on_device(dev, ((cos_sin, "cos_sin"), (positions, "positions")))
-        max_pos = cos_sin.size(0)
+        if cos_sin.get_device() != dev or positions.get_device() != dev:
+            _elsewhere("cos_sin and positions each")
+        max_pos, pos_ptr, cs_ptr = cos_sin.shape[0], positions.data_ptr(), cos_sin.data_ptr()
     if not eps >= 0.0:
         raise RuntimeError("eps must not be negative")
-    if n == 0:
-        return tuple(keep)
-    (hq, qp, qs, qo, qos, qw, qf, qh), (hk, kp, ks, ko, kos, kw, kf, kh) = args
-    handle, stream = _call(dev)
-    a = _lib.QkNormArgs(n, hq, hk, qp, qs, kp, ks, qo, qos, ko, kos, qw, kw, qf, kf, qh, kh, _ptr(positions) if max_pos else None,
-                        bool(max_pos) and positions.dtype is torch.int64, _ptr(cos_sin), max_pos, eps)
-    rc = _lib.load().dkv_qk_norm_rope(handle, C.byref(a), stream)
-    if rc:
-        _lib.check(rc)
-    return tuple(keep)
+    if n:
+        handle, stream = _call(dev)
+        a = _pack_qk_norm(n, hq, hk, qp, qs, kp, ks, qo, qos, ko, kos, qw, kw, qf, kf, qh, kh, pos_ptr, pos64, cs_ptr, max_pos, eps)
+        rc = _lib.load().dkv_qk_norm_rope(handle, a, stream)
+        if rc:
+            _lib.check(rc)
+    return qy, ky
 
 
 def _pages_args(page_table, lens, more, more_name, free_pages, n_free, page_size, rows):
     b = lens.numel()
     _int32_1d(lens, b, "lens")
     _int32_1d(more, b, more_name)
-    if rows is not None:
-        _int32_1d(rows, b, "rows")
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1 and page_table.size(1) > 1:
-        raise RuntimeError("page_table must be 2D int32 with unit inner stride")
-    if page_table.size(0) > 1 and page_table.stride(0) < page_table.size(1):
+    _check_page_table(page_table)
+    n_rows, max_pages = page_table.shape
+    stride = page_table.stride(0)
+    if n_rows > 1 and stride < max_pages:
         raise RuntimeError("the rows of page_table must not overlap")
-    if free_pages.dtype is not torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
+    if free_pages.dtype is not _I32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
         raise RuntimeError("free_pages must be a contiguous 1D int32 tensor")
     _int32_1d(n_free, 1, "n_free")
     if b > 4096:
         raise RuntimeError(f"{b} requests: at most 4096 per call")
     if page_size < 1 or page_size & (page_size - 1):
         raise RuntimeError(f"page_size ({page_size}) must be a power of two")
+    if rows is not None:
+        _int32_1d(rows, b, "rows")
     dev = page_table.get_device()
-    _on_device(dev, ((page_table, "page_table"), (lens, "lens"), (more, more_name), (free_pages, "free_pages"), (n_free, "n_free"), (rows, "rows")))
-    a = _lib.PagesArgs(page_table.data_ptr(), page_table.stride(0), page_table.size(0), page_table.size(1), _ptr(rows), lens.data_ptr(),
-                       more.data_ptr(), b, page_size, free_pages.data_ptr(), free_pages.size(0), n_free.data_ptr())
-    return dev, b, a
+    if dev < 0 or lens.get_device() != dev or more.get_device() != dev or free_pages.get_device() != dev or n_free.get_device() != dev:
+        _elsewhere(f"page_table, lens, {more_name}, free_pages and n_free each")
+    rows_ptr = 0
+    if rows is not None:
+        if rows.get_device() != dev:
+            _elsewhere("rows")
+        rows_ptr = rows.data_ptr()
+    return dev, b, _pack_pages(page_table.data_ptr(), stride, n_rows, max_pages, rows_ptr, lens.data_ptr(), more.data_ptr(), b, page_size,
+                               free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr())
 
 
 def assign_pages(
@@ -690,20 +747,25 @@ def assign_pages(
     dev, b, a = _pages_args(page_table, lens, new_lens, "new_lens", free_pages, n_free, page_size, rows)
     if not 0 <= n_tokens < 2 ** 31:
         raise RuntimeError(f"n_tokens ({n_tokens}) must be 0..2^31-1")
-    outs = []
-    for t, n, name in ((slots, n_tokens, "slots"), (positions, n_tokens, "positions"), (seq_lens, b, "seq_lens"), (cu_new, b + 1, "cu_new")):
-        if t is None:
-            t = torch.empty(n, dtype=torch.int32, device=page_table.device)
-        else:
-            _int32_1d(t, n, name)
-            _on_device(dev, ((t, name),))
-        outs.append(t)
+    if slots is None and positions is None and seq_lens is None and cu_new is None:
+        pad = -n_tokens & 3                                   # positions 16-byte aligned as well
+        slots, _, positions, seq_lens, cu_new = lens.new_empty(2 * n_tokens + pad + 2 * b + 1).split_with_sizes((n_tokens, pad, n_tokens, b, b + 1))
+    else:
+        outs = []
+        for t, n, name in ((slots, n_tokens, "slots"), (positions, n_tokens, "positions"), (seq_lens, b, "seq_lens"), (cu_new, b + 1, "cu_new")):
+            if t is None:
+                t = lens.new_empty(n)
+            else:
+                _int32_1d(t, n, name)
+            outs.append(t)
+        slots, positions, seq_lens, cu_new = outs
+    if slots.get_device() != dev or positions.get_device() != dev or seq_lens.get_device() != dev or cu_new.get_device() != dev:
+        _elsewhere("every output")
     handle, stream = _call(dev)
-    rc = _lib.load().dkv_assign_pages(handle, C.byref(a), outs[0].data_ptr(), outs[1].data_ptr(), n_tokens, outs[2].data_ptr(),
-                                      outs[3].data_ptr(), stream)
+    rc = _lib.load().dkv_assign_pages(handle, a, slots.data_ptr(), positions.data_ptr(), n_tokens, seq_lens.data_ptr(), cu_new.data_ptr(), stream)
     if rc:
         _lib.check(rc)
-    return tuple(outs)
+    return slots, positions, seq_lens, cu_new
 
 
 def release_pages(
@@ -724,7 +786,7 @@ def release_pages(
     if b == 0:
         return
     handle, stream = _call(dev)
-    rc = _lib.load().dkv_release_pages(handle, C.byref(a), stream)
+    rc = _lib.load().dkv_release_pages(handle, a, stream)
     if rc:
         _lib.check(rc)
 

@@ -131,3 +131,16 @@ def test_plain_pages_restore_the_stack():
     assert slots[:5] == [76, 77, 78, 79, 72] and pos[5:] == list(range(9)) and cu == [0, 5, 14] and p.n == 14
     p.release([0, 1], lens, [0, 0])
     assert p.stack == list(range(1, 20)) and p.n == 19
+
+
+def test_packed_arguments_are_the_c_structs():
+    """The wrappers pack the structs' bytes themselves: sizes and the place of every field agree with the declared ones."""
+    import ctypes
+    import struct
+
+    for cls, fmt in ((_lib.DecodeKv4Args, "@iiiPqPqPPqiiPfP"), (_lib.QkNormArgs, "@qiiPqPqPqPqPPiiiiPiPif"), (_lib.PagesArgs, "@PqiiPPPiiPiP")):
+        values = [float(i + 1) if f is ctypes.c_float else i + 1 for i, (_, f) in enumerate(cls._fields_)]
+        packed = struct.pack(fmt, *values)
+        assert len(packed) <= ctypes.sizeof(cls)
+        back = cls.from_buffer_copy(packed + bytes(ctypes.sizeof(cls) - len(packed)))
+        assert [getattr(back, n) for n, _ in cls._fields_] == values, cls
