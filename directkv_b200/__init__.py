@@ -2,7 +2,7 @@
 
 Public pieces: ``kernel`` (entry points over the C ABI), ``DirectKVBackend`` /
 ``DirectKVSmpV2Backend`` (attention backends), ``DirectKVTokenToKVPool`` / ``DirectKVRequestPool``
-(host-pinned KV stores), ``sharding`` (head-sharded and sequence-split multi-GPU helpers).
+(host-pinned KV stores), ``DirectKV4BitTokenToKVPool`` (a token pool held in 4 bits, in host memory or HBM), ``sharding`` (head-sharded and sequence-split multi-GPU helpers).
 The CUDA library is built in-tree with ``python -m directkv_b200.build``; nothing here computes on
 the CPU.
 """
@@ -10,7 +10,7 @@ the CPU.
 from .directkv_request_pool import DirectKVRequestPool  # noqa: F401
 from .directkv_pool import DirectKVTokenToKVPool  # noqa: F401
 
-__all__ = ["DirectKVRequestPool", "DirectKVTokenToKVPool", "DirectKVBackend", "DirectKVSmpV2Backend"]
+__all__ = ["DirectKVRequestPool", "DirectKVTokenToKVPool", "DirectKV4BitTokenToKVPool", "DirectKVBackend", "DirectKVSmpV2Backend"]
 
 
 def __getattr__(name):
@@ -21,4 +21,7 @@ def __getattr__(name):
     if name == "DirectKVSmpV2Backend":
         from .directkv_smpv2_backend import DirectKVSmpV2Backend
         return DirectKVSmpV2Backend
+    if name == "DirectKV4BitTokenToKVPool":
+        from .directkv_pool4 import DirectKV4BitTokenToKVPool
+        return DirectKV4BitTokenToKVPool
     raise AttributeError(name)

@@ -32,6 +32,7 @@ import torch
 
 from . import kernel
 from ._lib import get_context
+from .directkv_pool4 import DirectKV4BitTokenToKVPool
 from .directkv_request_pool import DirectKVRequestPool
 from .sglang_compat import AttentionBackend, get_attention_tp_size
 
@@ -109,6 +110,7 @@ class DirectKVBackend(AttentionBackend):
         self._cg_max_bs = 0
         self._cg_seq_lens: Optional[torch.Tensor] = None
         self._cg_rows: Optional[torch.Tensor] = None
+        self._cg_req: Optional[torch.Tensor] = None          # rows of req_to_token, for the token-pool path
 
     # ------------------------------------------------------------------ checks
     def _check_args(self, runner) -> None:
@@ -279,6 +281,7 @@ class DirectKVBackend(AttentionBackend):
         self._cg_max_bs = max_bs
         self._cg_seq_lens = torch.ones(max_bs, dtype=torch.int32, device=self.device)
         self._cg_rows = torch.zeros(max_bs, dtype=torch.int32, device=self.device)
+        self._cg_req = torch.zeros(max_bs, dtype=torch.int32, device=self.device)
         # Scratch for max_bs requests is sized now: nothing is allocated while a graph is captured.
         get_context(self._device_index()).reserve(max_bs, self.num_q_heads, self.num_kv_heads, self.hidden_size)
         logger.info(f"{self._TAG} CUDA graph state: max_bs={max_bs}, layers={len(self._wk)}.")
@@ -315,12 +318,13 @@ class DirectKVBackend(AttentionBackend):
             self._last_len[rid] = int(n)
         rows = [self._pool.row_of(r) for r in real] + [self._pool.pad_row] * (bs - n_real)
         self._cg_rows[:bs].copy_(torch.tensor(rows, dtype=torch.int32), non_blocking=False)
+        self._cg_req[:bs].copy_(req_pool_indices[:bs])
         if n_real < bs:
             self._cg_seq_lens[n_real:bs].fill_(1)
         self._fwd_meta = _FwdMeta(
             seq_lens_cpu=list(seq_lens_cpu[:n_real]) + [1] * (bs - n_real), req_pool_indices_cpu=rid_list,
             extend_seq_lens_cpu=None, extend_prefix_lens_cpu=None, seq_lens_dev=self._cg_seq_lens[:bs],
-            rows_dev=self._cg_rows[:bs], req_idx_dev=req_pool_indices[:bs].to(torch.int32), graph=True,
+            rows_dev=self._cg_rows[:bs], req_idx_dev=self._cg_req[:bs], graph=True,
         )
 
     def init_forward_metadata_capture_cuda_graph(self, bs, num_tokens, req_pool_indices, seq_lens, encoder_lens,
@@ -380,9 +384,13 @@ class DirectKVBackend(AttentionBackend):
         ``req_to_token[req, :seq_len]``."""
         meta = self._fwd_meta
         bs = forward_batch.batch_size
-        forward_batch.token_to_kv_pool.set_kv_buffer(layer, forward_batch.out_cache_loc, k, v)
-        eng = self._token_layer(layer, forward_batch)
+        pool = forward_batch.token_to_kv_pool
+        pool.set_kv_buffer(layer, forward_batch.out_cache_loc, k, v)
         table = forward_batch.req_to_token_pool.req_to_token
+        if isinstance(pool, DirectKV4BitTokenToKVPool):
+            return kernel.decode_kv4(q2, pool.layer_pool(layer.layer_id), meta.seq_lens_dev[:bs], float(layer.scaling), table,
+                                     row_map=meta.req_idx_dev[:bs])
+        eng = self._token_layer(layer, forward_batch)
         return kernel.decode(eng, q2, meta.seq_lens_dev[:bs], float(layer.scaling), page_table=table,
                              row_map=meta.req_idx_dev[:bs])
 
@@ -417,8 +425,10 @@ class DirectKVBackend(AttentionBackend):
         meta = self._fwd_meta
         bs = forward_batch.batch_size
         nh_q, d = self.num_q_heads, self.head_dim
-        forward_batch.token_to_kv_pool.set_kv_buffer(layer, forward_batch.out_cache_loc, k, v)
-        eng = self._token_layer(layer, forward_batch)
+        pool = forward_batch.token_to_kv_pool
+        pool.set_kv_buffer(layer, forward_batch.out_cache_loc, k, v)
+        four_bits = isinstance(pool, DirectKV4BitTokenToKVPool)
+        eng = _TOKEN_POOL_LAYER_BASE + layer.layer_id if four_bits else self._token_layer(layer, forward_batch)
         ext = meta.extend_seq_lens_cpu or [meta.seq_lens_cpu[i] for i in range(bs)]
         pre = meta.extend_prefix_lens_cpu or [0] * bs
         table = forward_batch.req_to_token_pool.req_to_token
@@ -443,9 +453,13 @@ class DirectKVBackend(AttentionBackend):
         if long_req:
             whole = len(long_req) == bs
             q_long = q if whole else torch.cat([q[o:o + n] for o, n in long_idx])
-            o_long = kernel.extend_ragged(eng, None, q_long.reshape(-1, nh_q, d).contiguous(), [r[0] for r in long_req],
-                                          [r[1] for r in long_req], [r[2] for r in long_req], float(layer.scaling), True,
-                                          page_table=table).view(-1, nh_q * d)
+            q_long = q_long.reshape(-1, nh_q, d).contiguous()
+            if four_bits:
+                o_long = self._extend_loaded_rows(eng, pool, layer, q_long, long_req, table).view(-1, nh_q * d)
+            else:
+                o_long = kernel.extend_ragged(eng, None, q_long, [r[0] for r in long_req],
+                                              [r[1] for r in long_req], [r[2] for r in long_req], float(layer.scaling), True,
+                                              page_table=table).view(-1, nh_q * d)
             if whole:
                 return o_long
             pos = 0
@@ -456,10 +470,33 @@ class DirectKVBackend(AttentionBackend):
             vlen_t = torch.tensor(vlen, dtype=torch.int32).to(self.device, non_blocking=True)
             vrow_t = torch.tensor(vrow, dtype=torch.int32).to(self.device, non_blocking=True)
             q2 = q.reshape(-1, nh_q * d)
+
+            def attend(rows):
+                if not four_bits:
+                    return kernel.decode(eng, rows, vlen_t, float(layer.scaling), page_table=table, row_map=vrow_t)
+                most = 4096                                   # requests of one call
+                parts = [kernel.decode_kv4(rows[i:i + most], pool.layer_pool(layer.layer_id), vlen_t[i:i + most], float(layer.scaling), table,
+                                           row_map=vrow_t[i:i + most]) for i in range(0, rows.shape[0], most)]
+                return parts[0] if len(parts) == 1 else torch.cat(parts)
+
             if len(vidx) != q2.shape[0]:
                 idx = torch.tensor(vidx, dtype=torch.long, device=q.device)
-                o_small = kernel.decode(eng, q2[idx].contiguous(), vlen_t, float(layer.scaling), page_table=table, row_map=vrow_t)
-                out[idx] = o_small
+                out[idx] = attend(q2[idx].contiguous())
             else:
-                out = kernel.decode(eng, q2.contiguous(), vlen_t, float(layer.scaling), page_table=table, row_map=vrow_t)
+                out = attend(q2.contiguous())
+        return out
+
+    def _extend_loaded_rows(self, eng: int, pool, layer, q_long: torch.Tensor, long_req, table: torch.Tensor) -> torch.Tensor:
+        """Long prompts over a 4-bit pool: the requests' rows come back to bf16 in HBM once, and the tensor-core extend
+        kernel attends them there."""
+        most = max(n_new + n_pre for n_new, n_pre, _ in long_req)
+        shape = (len(long_req), most, self.num_kv_heads, self.head_dim)
+        k_rows, v_rows = (torch.empty(shape, dtype=torch.bfloat16, device=q_long.device) for _ in range(2))
+        for i, (n_new, n_pre, rid) in enumerate(long_req):
+            n = n_new + n_pre
+            pool.load_rows(layer.layer_id, table[rid, :n], k_rows[i, :n], v_rows[i, :n])
+        kernel.register_layer(eng, k_rows, v_rows, page_size=1, row_stride=most, device=self._device_index())
+        out = kernel.extend_ragged(eng, None, q_long, [r[0] for r in long_req], [r[1] for r in long_req], list(range(len(long_req))),
+                                   float(layer.scaling), True)
+        kernel.unregister_layer(eng, device=self._device_index())
         return out

@@ -144,3 +144,23 @@ def test_packed_arguments_are_the_c_structs():
         assert len(packed) <= ctypes.sizeof(cls)
         back = cls.from_buffer_copy(packed + bytes(ctypes.sizeof(cls) - len(packed)))
         assert [getattr(back, n) for n, _ in cls._fields_] == values, cls
+
+
+def test_four_bit_token_pool_checks():
+    import directkv_b200
+
+    args = dict(size=30, page_size=1, dtype=BF, head_num=2, head_dim=128, layer_num=3)
+    pool = directkv_b200.DirectKV4BitTokenToKVPool(**args, start_layer=4, end_layer=6)
+    assert pool.n_slots == 31 and pool.get_kv_size_bytes() == (3 * 31 * 2 * 72,) * 2
+    assert pool.layer_pool(5).nh_kv == 2 and pool.layer_pool(5) is not pool.layer_pool(6)
+    for kw, why in ((dict(dtype=torch.float16), "bfloat16"), (dict(head_dim=64), "head_dim"), (dict(location="disk"), "location")):
+        with pytest.raises(ValueError, match=why):
+            directkv_b200.DirectKV4BitTokenToKVPool(**{**args, **kw})
+    rows = torch.zeros(2, 2, 128, dtype=BF)
+    with pytest.raises(RuntimeError, match="no CPU quantiser"):
+        pool.set_kv_buffer(None, torch.tensor([1, 2]), rows, rows, layer_id_override=4)
+    with pytest.raises(ValueError, match="v_scale"):
+        pool.set_kv_buffer(None, torch.tensor([1, 2]), rows, rows, v_scale=0.5, layer_id_override=4)
+    for f in (pool.get_key_buffer, pool.get_value_buffer):
+        with pytest.raises(NotImplementedError, match="4 bits"):
+            f(4)
