@@ -35,18 +35,38 @@ int check_kv4_pool(const dkv_context* ctx, const dkv_kv4_pool* pool) {
     return DKV_OK;
 }
 
-// Heads and token lanes of a block: as many of its warps as the number of heads allows, and of the shapes that use
-// them the one with the most heads side by side, whose rows of a token are one contiguous read.
-void kv4_block_shape(int nh_kv, int warps, int* hg, int* ts) {
+// How a launch cuts its work: heads (hg) and token lanes (ts) of a block of W warps, and whether segments are left whole.
+//  - By default as many warps as the number of heads allows, and of the shapes that use them the one with the most
+//    heads side by side, whose rows of a token are read together.
+//  - Where the page table has room for a few steps only (`room` tokens), nothing is split: a second launch and the
+//    records' way through memory cost more than a few steps one behind the other.  With blocks to spare, token lanes make it
+//    fewer steps (32 query heads on 8, one request of 77 tokens: 6.2 us as one step of four lanes, 8.4 us as three steps, 9.0 us
+//    split); with half a grid of segments up to 8 steps (64 requests of 256 tokens: 10.6 us, split 19.2 us).
+//  - Very few segments (one long request): two heads per block and the other warps as token lanes, joined in the block, leave
+//    a quarter of the records to merge (131071 tokens: 39 us, 42 us with eight heads).
+template <int NT>
+void kv4_shape(int batch, int nh_kv, int n_cc, int64_t room, int grid, int* hg, int* ts, int* whole) {
+    constexpr int W = kKv4Warps<NT>;
     int best = 0;
-    for (int h = 1; h <= warps; ++h) {
+    for (int h = 1; h <= W; ++h) {
         if (nh_kv % h != 0) continue;
-        const int t = warps / h;
+        const int t = W / h;
         if (h * t >= best) best = h * t, *hg = h, *ts = t;
     }
+    auto segments = [&](int h) { return static_cast<int64_t>(batch) * (nh_kv / h) * n_cc; };
+    auto steps = [&](int t) { return (room + static_cast<int64_t>(kKv4Tile) * t - 1) / (static_cast<int64_t>(kKv4Tile) * t); };
+    *whole = 0;
+    int h0 = *hg, t0 = *ts;
+    for (int t = t0; t <= W; ++t) {                       // the fewest lanes that give the fewest steps
+        const int h = W / t;
+        if (h * t != W || nh_kv % h != 0 || segments(h) > grid) continue;
+        if (steps(t) < steps(t0)) h0 = h, t0 = t;
+    }
+    if (steps(t0) <= 2) *hg = h0, *ts = t0, *whole = 1;
+    else if (2 * segments(*hg) >= grid) *whole = steps(*ts) <= 8;
+    else if (segments(*hg) <= 8 && *hg > 2 && nh_kv % 2 == 0) *hg = 2, *ts = W / 2;
 }
 
-constexpr int kKv4WholeSteps = 9;      // (tables of up to 8 steps)
 constexpr size_t kKv4CumBytes = (kKv4LaunchBatch + 1) * sizeof(int) / 256 * 256 + 256;
 
 template <int NT>
@@ -67,14 +87,12 @@ constexpr int kv4_smem(int batch) {
 
 template <int NT>
 int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
-    kv4_block_shape(p.nh_kv, kKv4Warps<NT>, &p.hg, &p.ts);
-    p.n_hg = p.nh_kv / p.hg;
     p.n_cc = (p.cols + 8 * NT - 1) / (8 * NT);
-    const int64_t most_parts = (static_cast<int64_t>(p.max_pages) << p.page_shift) / (kKv4Tile * p.ts) + 1;
-    // A table with room for a few steps only: splitting them costs more (a second launch and the records' way through
-    // memory) than doing them one behind the other.
-    p.whole = most_parts <= kKv4WholeSteps;
     const int grid = kv4_grid<NT>(ctx);
+    const int64_t room = static_cast<int64_t>(p.max_pages) << p.page_shift;
+    kv4_shape<NT>(p.batch, p.nh_kv, p.n_cc, room, grid, &p.hg, &p.ts, &p.whole);
+    p.n_hg = p.nh_kv / p.hg;
+    const int64_t most_parts = room / (kKv4Tile * p.ts) + 1;
     const size_t smem = kv4_smem<NT>(p.batch);
     if (p.page_shift >= 4) kv4_attn_kernel<NT, true><<<grid, kKv4Warps<NT> * 32, smem, st>>>(p);
     else kv4_attn_kernel<NT, false><<<grid, kKv4Warps<NT> * 32, smem, st>>>(p);
