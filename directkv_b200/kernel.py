@@ -393,15 +393,6 @@ def _call(dev: int):
     return ctx.handle, torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _contiguous_pair(like: torch.Tensor, shape_a, shape_b):
-    """Two contiguous tensors of like's type and device in one allocation (an allocation costs as much as the rest of a
-    short call's host side)."""
-    na, nb = math.prod(shape_a), math.prod(shape_b)
-    flat = like.new_empty(na + nb)
-    ra, rb = shape_a[-2] * HEAD_DIM, shape_b[-2] * HEAD_DIM
-    return flat.as_strided(shape_a, (ra, HEAD_DIM, 1)), flat.as_strided(shape_b, (rb, HEAD_DIM, 1), na)
-
-
 def _elsewhere(name: str) -> None:
     raise RuntimeError(f"{name} must be a CUDA tensor on the same device as the other tensors")
 
@@ -536,7 +527,8 @@ def load_kv4(pool: KV4Pool, slots: torch.Tensor, k_out: Optional[torch.Tensor] =
         proto = _protos.get(dev)
         if proto is None:
             proto = _protos[dev] = torch.empty(0, dtype=_BF16, device=slots.device)
-        k_out, v_out = _contiguous_pair(proto, shape, shape)
+        strides = (pool.nh_kv * HEAD_DIM, HEAD_DIM, 1)
+        k_out, v_out = proto.new_empty_strided(shape, strides), proto.new_empty_strided(shape, strides)
     if k_out is None:
         k_out = torch.empty(shape, dtype=_BF16, device=slots.device)
     elif k_out.dtype is not _BF16 or k_out.shape != shape or not k_out.is_contiguous() or k_out.get_device() != dev:
@@ -607,7 +599,7 @@ def decode_kv4(
         _elsewhere("q, seq_lens and page_table each")
     row = nh_q * HEAD_DIM
     if out is None:
-        out = torch.empty_like(q) if qs == row and q.is_contiguous() else torch.empty(shape, dtype=_BF16, device=q.device)
+        out = torch.empty_like(q)                             # (contiguous for a slice of a fused projection, too)
         os = row
     else:
         if out.shape != shape or out.get_device() != dev:
@@ -631,8 +623,7 @@ def _norm_side(x, y, w, n: int, dev: int, name: str):
         raise RuntimeError(f"{name} must be [{n}, NH, {HEAD_DIM}]")
     xs, nh = _heads_stride(x, name), shape[1]
     if y is None:
-        # (a slice of a fused projection gives a contiguous output)
-        y, ys = (torch.empty_like(x) if x.is_contiguous() else torch.empty(shape, dtype=_BF16, device=x.device)), nh * HEAD_DIM
+        y, ys = torch.empty_like(x), nh * HEAD_DIM            # (contiguous for a slice of a fused projection, too)
     else:
         if y.shape != shape or y.get_device() != dev:
             raise RuntimeError(f"{name}_out must have the shape of {name} and its device")
@@ -667,8 +658,6 @@ def qk_norm_rope(
     if lead is None:
         raise RuntimeError("q or k must be given")
     n, dev = lead.shape[0], lead.get_device()
-    if q is not None and k is not None and q_out is None and k_out is None and q.dtype is _BF16 and q.dim() == 3 and k.dim() == 3:
-        q_out, k_out = _contiguous_pair(q, q.shape, k.shape)
     qy, hq, qp, qs, qo, qos, qw, qf, qh = _norm_side(q, q_out, q_weight, n, dev, "q") if q is not None else (None, 0, 0, 0, 0, 0, 0, 0, 0)
     ky, hk, kp, ks, ko, kos, kw, kf, kh = _norm_side(k, k_out, k_weight, n, dev, "k") if k is not None else (None, 0, 0, 0, 0, 0, 0, 0, 0)
     max_pos = pos_ptr = pos64 = cs_ptr = 0

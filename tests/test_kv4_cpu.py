@@ -164,3 +164,12 @@ def test_four_bit_token_pool_checks():
     for f in (pool.get_key_buffer, pool.get_value_buffer):
         with pytest.raises(NotImplementedError, match="4 bits"):
             f(4)
+
+
+def test_outputs_like_a_slice_are_contiguous():
+    """The wrappers allocate with empty_like and take the result's tokens to lie one behind the other."""
+    rows = torch.zeros(6, 10, 128, dtype=BF)
+    for x in (rows[:, 2:5], rows[:, 2:3], rows[:1, 2:5], rows[::2, :4], rows.view(3, 2, 10, 128)[:, :, 1:3], rows.view(6, 1, 10, 128)[:, :, 1:3]):
+        assert kernel._heads_stride(x, "x") > 0 and torch.empty_like(x).is_contiguous()
+    flat = torch.zeros(6, 1280, dtype=BF)[:, 128:512]
+    assert torch.empty_like(flat).is_contiguous()
