@@ -495,6 +495,16 @@ cudaError_t attn_mma8_set_attr() {
     return e != cudaSuccess ? e : prefer_max_shared(attn_partial_mma8_kernel<NW, NST>);
 }
 
+template <int NT>
+constexpr int kv4_smem(int batch) {
+    return kKv4Warps<NT> * kKv4WarpBytes<NT> + (batch + 1) * static_cast<int>(sizeof(int));
+}
+
+template <int NT, bool WIDE>
+cudaError_t kv4_set_attr() {
+    return cudaFuncSetAttribute(kv4_attn_kernel<NT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kv4_smem<NT>(kKv4LaunchBatch));
+}
+
 template <int NW, int NST>
 cudaError_t attn_mma_set_attr() {
     return cudaFuncSetAttribute(attn_partial_mma_kernel<NW, NST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -905,6 +915,10 @@ int dkv_context_create(int device, dkv_context** out) {
     if (e == cudaSuccess) e = set_gemv_attributes<1>();
     if (e == cudaSuccess) e = set_gemv_attributes<2>();
     if (e == cudaSuccess) e = prefer_max_shared(attn_partial_kernel<1, 16, 1>);
+    if (e == cudaSuccess) e = kv4_set_attr<1, false>();
+    if (e == cudaSuccess) e = kv4_set_attr<1, true>();
+    if (e == cudaSuccess) e = kv4_set_attr<2, false>();
+    if (e == cudaSuccess) e = kv4_set_attr<2, true>();
     if (e != cudaSuccess) {
         delete ctx;
         return fail(DKV_ERR_CUDA, "context set-up failed: %s", cudaGetErrorString(e));

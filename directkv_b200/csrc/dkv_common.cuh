@@ -202,6 +202,12 @@ __device__ __forceinline__ uint64_t ex2_poly_f32x2(uint64_t x) {
                  __uint_as_float(__float_as_uint(q1) + (__float_as_uint(r1) << 23)));
 }
 
+// Launched with programmatic stream serialization, a kernel's blocks may be set up while the kernel before it ends.  The wait
+// comes before the first access to memory and returns when that kernel is complete and its stores are visible; the
+// trigger lets the kernel after it start its own set-up once every block has come this far.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ float round_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 
 // ---------------------------------------------------------------------------

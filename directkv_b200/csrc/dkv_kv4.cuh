@@ -161,6 +161,8 @@ __device__ __forceinline__ void kv4_read16(const __nv_bfloat16* src, int wide, u
 
 // A thread takes one block of 16 dimensions of K and the same one of V.
 __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4RowsParams p) {
+    grid_wait();
+    grid_trigger();
     const int units = p.nh * 8;                           // blocks of 16 per token
     for (int i = threadIdx.x; i < p.per_block * units; i += 256) {
         const int t = i / units, u = i - t * units;
@@ -206,6 +208,8 @@ __device__ __forceinline__ void kv4_write16(__nv_bfloat16* dst, uint2 codes, uin
 }
 
 __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4RowsParams p) {
+    grid_wait();
+    grid_trigger();
     const int units = p.nh * 8;
     for (int i = threadIdx.x; i < p.per_block * units; i += 256) {
         const int t = i / units, u = i - t * units;

@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int g = lane >> 2, c = lane & 3;
 
+    grid_wait();
     // Tiles (of 32 * ts tokens) before every request; a request without tokens has one, which writes its zeros.
     if (threadIdx.x == 0) cum[0] = 0;
     int before = 0;
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
     const int per_tile = p.n_hg * p.n_cc;
     const long long total = static_cast<long long>(before) * per_tile;
     const int blocks = kv4_blocks(total, static_cast<long long>(p.batch) * per_tile, gridDim.x);
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    grid_trigger();
     if (static_cast<int>(blockIdx.x) >= blocks) return;
     const long long x0 = kv4_share(total, blockIdx.x, blocks), x1 = kv4_share(total, blockIdx.x + 1, blocks);
 
@@ -571,7 +572,8 @@ __global__ void __launch_bounds__(NW * 32) kv4_merge_kernel(const Kv4AttnParams 
     extern __shared__ __align__(16) uint8_t smem[];
     float2* ml = reinterpret_cast<float2*>(smem);                         // [grid]
     __shared__ float part[NW][128];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    grid_wait();
+    grid_trigger();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int h = blockIdx.x % p.nh_q, j = (blockIdx.x / p.nh_q) % p.n_q, b = blockIdx.x / (p.nh_q * p.n_q);
     const int first = p.cum[b], tiles = p.cum[b + 1] - first, per_tile = p.n_hg * p.n_cc;

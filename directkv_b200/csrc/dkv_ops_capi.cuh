@@ -18,6 +18,22 @@ struct DeviceScope {
     }
 };
 
+// Launches a kernel that begins with grid_wait() so that its set-up overlaps the end of the kernel before it.
+template <typename... KernelArgs, typename... Args>
+cudaError_t launch_overlapped(void (*kernel)(KernelArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 #define DKV_ON_DEVICE(ctx)              \
     DeviceScope device_scope((ctx)->device); \
     DKV_CUDA(device_scope.err)
@@ -81,11 +97,6 @@ size_t kv4_workspace(const dkv_context* ctx) {
 }
 
 template <int NT>
-constexpr int kv4_smem(int batch) {
-    return kKv4Warps<NT> * kKv4WarpBytes<NT> + (batch + 1) * static_cast<int>(sizeof(int));
-}
-
-template <int NT>
 int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
     p.n_cc = (p.cols + 8 * NT - 1) / (8 * NT);
     const int grid = kv4_grid<NT>(ctx);
@@ -94,32 +105,21 @@ int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
     p.n_hg = p.nh_kv / p.hg;
     const int64_t most_parts = room / (kKv4Tile * p.ts) + 1;
     const size_t smem = kv4_smem<NT>(p.batch);
-    if (p.page_shift >= 4) kv4_attn_kernel<NT, true><<<grid, kKv4Warps<NT> * 32, smem, st>>>(p);
-    else kv4_attn_kernel<NT, false><<<grid, kKv4Warps<NT> * 32, smem, st>>>(p);
-    DKV_CUDA(cudaGetLastError());
+    const auto kernel = p.page_shift >= 4 ? kv4_attn_kernel<NT, true> : kv4_attn_kernel<NT, false>;
+    if (NT == 1) {
+        DKV_CUDA(launch_overlapped(kernel, grid, kKv4Warps<NT> * 32, smem, st, p));
+    } else {                            // takes all registers of an SM: set up beside a merge that still runs, it loses (16 drafts: 41 us, 37 us)
+        kernel<<<grid, kKv4Warps<NT> * 32, smem, st>>>(p);
+        DKV_CUDA(cudaGetLastError());
+    }
     ctx->launches += 1;
     if (p.whole) return DKV_OK;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(p.batch) * p.n_q * p.nh_q);
+    const unsigned rows = static_cast<unsigned>(p.batch) * p.n_q * p.nh_q;
     // Few rows: many blocks had a part of each.
-    const bool few = cfg.gridDim.x <= static_cast<unsigned>(2 * ctx->sm_count) && most_parts > 16;
-    cfg.blockDim = dim3(few ? 512 : 128);
-    cfg.dynamicSmemBytes = grid * sizeof(float2);
-    cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (few) DKV_CUDA(cudaLaunchKernelEx(&cfg, kv4_merge_kernel<NT, 16>, p, grid));
-    else DKV_CUDA(cudaLaunchKernelEx(&cfg, kv4_merge_kernel<NT, 4>, p, grid));
+    const bool few = rows <= static_cast<unsigned>(2 * ctx->sm_count) && most_parts > 16;
+    DKV_CUDA(launch_overlapped(few ? kv4_merge_kernel<NT, 16> : kv4_merge_kernel<NT, 4>, rows, few ? 512 : 128, grid * sizeof(float2), st, p, grid));
     ctx->launches += 1;
     return DKV_OK;
-}
-
-template <int NT, bool WIDE>
-cudaError_t kv4_set_attr() {
-    return cudaFuncSetAttribute(kv4_attn_kernel<NT, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kv4_smem<NT>(kKv4LaunchBatch));
 }
 
 }  // namespace
@@ -150,10 +150,6 @@ int dkv_kv4_pool_resolve(dkv_context* ctx, dkv_kv4_pool* pool) {
         int rc = device_pointer_of(*p, p, "a 4-bit pool");
         if (rc != DKV_OK) return rc;
     }
-    DKV_CUDA((kv4_set_attr<1, false>()));
-    DKV_CUDA((kv4_set_attr<1, true>()));
-    DKV_CUDA((kv4_set_attr<2, false>()));
-    DKV_CUDA((kv4_set_attr<2, true>()));
     int rc = ensure_buffer(ctx, &ctx->kv4, kv4_workspace(ctx), false, "workspace of the 4-bit attention");
     if (rc != DKV_OK) return rc;
     r.resolved = ctx->device + 1;
@@ -196,8 +192,7 @@ int dkv_kv4_store(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots,
     p.k_scale = 1.f / pool->k_scale, p.v_scale = 1.f / pool->v_scale;
     p.wide = aligned(k, 32) && aligned(v, 32) && k_stride % 16 == 0 && v_stride % 16 == 0;
     DKV_ON_DEVICE(ctx);
-    kv4_store_kernel<<<static_cast<unsigned>((n_tokens + p.per_block - 1) / p.per_block), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    DKV_CUDA(cudaGetLastError());
+    DKV_CUDA(launch_overlapped(kv4_store_kernel, static_cast<unsigned>((n_tokens + p.per_block - 1) / p.per_block), 256, 0, static_cast<cudaStream_t>(stream), p));
     ctx->launches += 1;
     return DKV_OK;
 }
@@ -212,8 +207,7 @@ int dkv_kv4_load(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, 
     p.k_scale = pool->k_scale, p.v_scale = pool->v_scale;
     p.wide = aligned(k, 32) && aligned(v, 32);
     DKV_ON_DEVICE(ctx);
-    kv4_load_kernel<<<static_cast<unsigned>((n_tokens + p.per_block - 1) / p.per_block), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    DKV_CUDA(cudaGetLastError());
+    DKV_CUDA(launch_overlapped(kv4_load_kernel, static_cast<unsigned>((n_tokens + p.per_block - 1) / p.per_block), 256, 0, static_cast<cudaStream_t>(stream), p));
     ctx->launches += 1;
     return DKV_OK;
 }
@@ -317,10 +311,9 @@ int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* a, void* stream) 
     // Eight heads per half warp once that still gives every SM 32 warps, else one.
     const int qn = (a->nh_q + 7) / 8, gn = qn + (a->nh_k + 7) / 8;
     if (a->n_tokens * gn >= static_cast<int64_t>(ctx->sm_count) * 64)
-        qk_norm_rope_kernel<8, 16><<<static_cast<unsigned>((a->n_tokens * gn + 3) / 4), 64, 0, st>>>(p, qn, gn);
+        DKV_CUDA(launch_overlapped(qk_norm_rope_kernel<8, 16>, static_cast<unsigned>((a->n_tokens * gn + 3) / 4), 64, 0, st, p, qn, gn));
     else
-        qk_norm_rope_kernel<1, 16><<<static_cast<unsigned>((rows + 3) / 4), 64, 0, st>>>(p, a->nh_q, a->nh_q + a->nh_k);
-    DKV_CUDA(cudaGetLastError());
+        DKV_CUDA(launch_overlapped(qk_norm_rope_kernel<1, 16>, static_cast<unsigned>((rows + 3) / 4), 64, 0, st, p, a->nh_q, a->nh_q + a->nh_k));
     ctx->launches += 1;
     return DKV_OK;
 }
@@ -356,8 +349,7 @@ int dkv_assign_pages(dkv_context* ctx, const dkv_pages_args* a, int32_t* slots, 
     p.vector = aligned(slots, 16) && aligned(positions, 16);
     const int64_t want = (capacity + 4 * kPagesThreads - 1) / (4 * kPagesThreads);
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, ctx->sm_count * 2)));
-    pages_kernel<false><<<grid, kPagesThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    DKV_CUDA(cudaGetLastError());
+    DKV_CUDA(launch_overlapped(pages_kernel<false>, grid, kPagesThreads, 0, static_cast<cudaStream_t>(stream), p));
     ctx->launches += 1;
     return DKV_OK;
 }
@@ -370,8 +362,7 @@ int dkv_release_pages(dkv_context* ctx, const dkv_pages_args* a, void* stream) {
     const int64_t most = std::min<int64_t>(static_cast<int64_t>(a->batch) * p.max_pages, p.free_cap);
     const int64_t want = (most + kPagesThreads - 1) / kPagesThreads;
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, ctx->sm_count)));
-    pages_kernel<true><<<grid, kPagesThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    DKV_CUDA(cudaGetLastError());
+    DKV_CUDA(launch_overlapped(pages_kernel<true>, grid, kPagesThreads, 0, static_cast<cudaStream_t>(stream), p));
     ctx->launches += 1;
     return DKV_OK;
 }

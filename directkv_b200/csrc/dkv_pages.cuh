@@ -68,6 +68,8 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(const PagesParams 
     __shared__ int cu_page[kPagesMaxBatch + 1];
     __shared__ long long sh[64];
     __shared__ int sh_last;
+    grid_wait();
+    grid_trigger();
     const int P = 1 << p.page_shift;
     const int top = *reinterpret_cast<const volatile int*>(p.n_free);
     bool bad = top < 0 || top > p.free_cap;

@@ -58,6 +58,8 @@ __device__ __forceinline__ uint2 pack4(const uint64_t (&v)[2]) {
 // multiplied with one another once for all of them, y = inv (u A - v B), inv (v C + u D), and R rows are on their way at a time.
 template <int R, int BLOCKS>
 __global__ void __launch_bounds__(64, BLOCKS) qk_norm_rope_kernel(const QkNormParams p, int q_groups, int groups) {
+    grid_wait();
+    grid_trigger();
     const int l = threadIdx.x & 15;
     const long long id = (static_cast<long long>(blockIdx.x) * 64 + threadIdx.x) >> 4;
     if (id >= p.n_tokens * groups) return;                // by halves of a warp
