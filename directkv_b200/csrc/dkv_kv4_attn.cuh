@@ -116,17 +116,22 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The share of the flattened tile list that block i of n takes, and the block that has tile x.
-__device__ __forceinline__ long long kv4_share(long long total, int i, int n) { return total * i / n; }
-__device__ __forceinline__ int kv4_owner(long long total, long long x, int n) {
-    return static_cast<int>(((x + 1) * n - 1) / total);
-}
+// The flattened tile list (its length fits 31 bits, the host sees to that) is dealt out evenly: block i of n begins at its
+// share, the first total % n blocks have one tile more.
+struct Kv4Deal {
+    int each, more;
+    __device__ __forceinline__ Kv4Deal(int total, int n) : each(static_cast<unsigned>(total) / static_cast<unsigned>(n)) { more = total - each * n; }
+    __device__ __forceinline__ int share(int i) const { return each * i + min(i, more); }
+    __device__ __forceinline__ int owner(int x) const {
+        const int edge = more * (each + 1);
+        return x < edge ? static_cast<unsigned>(x) / static_cast<unsigned>(each + 1) : more + static_cast<unsigned>(x - edge) / static_cast<unsigned>(each);
+    }
+};
 // Blocks that take part.  Segments of up to 4 tiles on average that are enough to occupy an eighth of the grid are not cut
 // finer than there are segments: what is gained in steps goes into merging (64 requests of 77 tokens, 32 heads on 8: 14 us
 // with a block per tile).
-__device__ __forceinline__ int kv4_blocks(long long total, long long segments, int grid) {
-    const long long n = total <= 4 * segments && 8 * segments >= grid ? segments : total;
-    return n < grid ? static_cast<int>(n) : grid;
+__device__ __forceinline__ int kv4_blocks(int total, int segments, int grid) {
+    return min(total <= 4ll * segments && 8ll * segments >= grid ? segments : total, grid);
 }
 
 // A request's length as far as the table reaches, and its row; a length or row outside is reported.
@@ -159,41 +164,45 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
     const int g = lane >> 2, c = lane & 3;
 
     grid_wait();
-    // Tiles (of 32 * ts tokens) before every request; a request without tokens has one, which writes its zeros.
-    if (threadIdx.x == 0) cum[0] = 0;
-    int before = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += W * 32) {
-        const int b = b0 + threadIdx.x;
-        int n = 0;
-        if (b < p.batch) {
-            long long row;
-            const int code = kv4_length(p, b, &row);
-            if (code < 0 && blockIdx.x == 0) atomicOr(p.status, kStatusBadPage);
-            const int len = kv4_clean_length(p, code);
-            n = p.whole ? 1 : max(1, static_cast<int>((static_cast<long long>(len) + kKv4Tile * p.ts - 1) / (kKv4Tile * p.ts)));
-        }
-        int inc = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += x;
-        }
-        if (lane == 31) sh_scan[w] = inc;
-        __syncthreads();
-        int base = before;
-        for (int i = 0; i < w; ++i) base += sh_scan[i];
-        if (b < p.batch) cum[b + 1] = base + inc;
-        for (int i = 0; i < W; ++i) before += sh_scan[i];
-        __syncthreads();
-    }
-    if (blockIdx.x == 0)
-        for (int b = threadIdx.x; b <= p.batch; b += blockDim.x) p.cum[b] = cum[b];
     const int per_tile = p.n_hg * p.n_cc;
-    const long long total = static_cast<long long>(before) * per_tile;
-    const int blocks = kv4_blocks(total, static_cast<long long>(p.batch) * per_tile, gridDim.x);
+    int total;
+    if (p.whole) {
+        total = p.batch * per_tile;                  // one entry per segment, whatever its length
+    } else {
+        // Tiles (of 32 * ts tokens) before every request; a request without tokens has one, which writes its zeros.
+        if (threadIdx.x == 0) cum[0] = 0;
+        int before = 0;
+        for (int b0 = 0; b0 < p.batch; b0 += W * 32) {
+            const int b = b0 + threadIdx.x;
+            int n = 0;
+            if (b < p.batch) {
+                long long row;
+                const int len = kv4_clean_length(p, kv4_length(p, b, &row));
+                n = max(1, static_cast<int>((static_cast<unsigned>(len) + kKv4Tile * p.ts - 1) / (kKv4Tile * p.ts)));
+            }
+            int inc = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += x;
+            }
+            if (lane == 31) sh_scan[w] = inc;
+            __syncthreads();
+            int base = before;
+            for (int i = 0; i < w; ++i) base += sh_scan[i];
+            if (b < p.batch) cum[b + 1] = base + inc;
+            for (int i = 0; i < W; ++i) before += sh_scan[i];
+            __syncthreads();
+        }
+        if (blockIdx.x == 0)
+            for (int b = threadIdx.x; b <= p.batch; b += blockDim.x) p.cum[b] = cum[b];
+        total = before * per_tile;
+    }
+    const int blocks = kv4_blocks(total, p.batch * per_tile, gridDim.x);
     grid_trigger();
     if (static_cast<int>(blockIdx.x) >= blocks) return;
-    const long long x0 = kv4_share(total, blockIdx.x, blocks), x1 = kv4_share(total, blockIdx.x + 1, blocks);
+    const Kv4Deal deal(total, blocks);
+    const int x0 = deal.share(blockIdx.x), x1 = deal.share(blockIdx.x + 1);
 
     const int hl = w % p.hg, tl = w / p.hg;
     const bool active = tl < p.ts;
@@ -204,23 +213,27 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
     const int page_mask = (1 << p.page_shift) - 1;
     Kv4State<NT> st;
 
-    for (long long x = x0; x < x1;) {
+    for (int x = x0; x < x1;) {
         // Segment: one request, head group and column chunk.
-        const int y = static_cast<int>(x / per_tile);
-        int lo = 0, hi = p.batch - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (cum[mid] <= y) lo = mid;
-            else hi = mid - 1;
+        const int y = x / per_tile;
+        int b = y, entries = 1, seg = x - y * per_tile, tile0 = 0;
+        if (!p.whole) {
+            int lo = 0, hi = p.batch - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (cum[mid] <= y) lo = mid;
+                else hi = mid - 1;
+            }
+            b = lo;
+            entries = cum[b + 1] - cum[b];
+            const int r = x - cum[b] * per_tile;
+            seg = r / entries, tile0 = r - seg * entries;
         }
-        const int b = lo;
-        const int entries = cum[b + 1] - cum[b];
-        const long long r = x - static_cast<long long>(cum[b]) * per_tile;
-        const int seg = static_cast<int>(r / entries), tile0 = static_cast<int>(r - static_cast<long long>(seg) * entries);
         long long row;
-        const int len = kv4_clean_length(p, kv4_length(p, b, &row));
-        const int taken = static_cast<int>(min(static_cast<long long>(entries - tile0), x1 - x));
-        const int n_tiles = p.whole ? (len + kKv4Tile * p.ts - 1) / (kKv4Tile * p.ts) : taken;
+        const int code = kv4_length(p, b, &row), len = kv4_clean_length(p, code);
+        if (code < 0 && threadIdx.x == 0) atomicOr(p.status, kStatusBadPage);
+        const int taken = min(entries - tile0, x1 - x);
+        const int n_tiles = p.whole ? static_cast<int>((static_cast<unsigned>(len) + kKv4Tile * p.ts - 1) / (kKv4Tile * p.ts)) : taken;
         const int hgi = seg / p.n_cc, cc = seg - hgi * p.n_cc;
         const bool whole = taken == entries;
         const int kvh = hgi * p.hg + hl;
@@ -577,12 +590,12 @@ __global__ void __launch_bounds__(NW * 32) kv4_merge_kernel(const Kv4AttnParams 
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int h = blockIdx.x % p.nh_q, j = (blockIdx.x / p.nh_q) % p.n_q, b = blockIdx.x / (p.nh_q * p.n_q);
     const int first = p.cum[b], tiles = p.cum[b + 1] - first, per_tile = p.n_hg * p.n_cc;
-    const long long total = static_cast<long long>(p.cum[p.batch]) * per_tile;
-    const int blocks = kv4_blocks(total, static_cast<long long>(p.batch) * per_tile, grid);
+    const int total = p.cum[p.batch] * per_tile;
+    const Kv4Deal deal(total, kv4_blocks(total, p.batch * per_tile, grid));
     const int kvh = h / p.group, col = j * p.group + (h - kvh * p.group);
     const int hgi = kvh / p.hg, hl = kvh - hgi * p.hg, cc = col / C, cl = col - cc * C;
-    const long long s0 = static_cast<long long>(first) * per_tile + static_cast<long long>(hgi * p.n_cc + cc) * tiles;
-    const int i0 = kv4_owner(total, s0, blocks), n = kv4_owner(total, s0 + tiles - 1, blocks) - i0 + 1;
+    const int s0 = first * per_tile + (hgi * p.n_cc + cc) * tiles;
+    const int i0 = deal.owner(s0), n = deal.owner(s0 + tiles - 1) - i0 + 1;
     if (n == 1) return;
     // The segment's first block has it as the one that goes on behind its share; for the others it began before theirs.
     const long long step = 2ll * p.hg * C * kKv4RecFloats;

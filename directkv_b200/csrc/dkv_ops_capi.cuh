@@ -99,11 +99,15 @@ size_t kv4_workspace(const dkv_context* ctx) {
 template <int NT>
 int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
     p.n_cc = (p.cols + 8 * NT - 1) / (8 * NT);
-    const int grid = kv4_grid<NT>(ctx);
+    const int full_grid = kv4_grid<NT>(ctx);
     const int64_t room = static_cast<int64_t>(p.max_pages) << p.page_shift;
-    kv4_shape<NT>(p.batch, p.nh_kv, p.n_cc, room, grid, &p.hg, &p.ts, &p.whole);
+    kv4_shape<NT>(p.batch, p.nh_kv, p.n_cc, room, full_grid, &p.hg, &p.ts, &p.whole);
     p.n_hg = p.nh_kv / p.hg;
     const int64_t most_parts = room / (kKv4Tile * p.ts) + 1;
+    const int64_t most_tiles = (p.whole ? 1 : most_parts) * p.batch * p.n_hg * p.n_cc;
+    if (most_tiles > INT32_MAX)
+        return fail(DKV_ERR_UNSUPPORTED, "%d requests of up to %lld tokens are too many for one call", p.batch, static_cast<long long>(room));
+    const int grid = static_cast<int>(std::min<int64_t>(full_grid, most_tiles));
     const size_t smem = kv4_smem<NT>(p.batch);
     const auto kernel = p.page_shift >= 4 ? kv4_attn_kernel<NT, true> : kv4_attn_kernel<NT, false>;
     if (NT == 1) {
@@ -252,8 +256,6 @@ int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_
     p.v_scale = pool->v_scale;
     p.status = ctx->status;
     DKV_REQUIRE(static_cast<int64_t>(a->batch) * a->n_q * a->nh_q <= INT32_MAX, "too many query rows");
-    DKV_REQUIRE((static_cast<int64_t>(p.max_pages) << p.page_shift) / 16 * a->batch < INT32_MAX, "%d requests of up to %lld tokens are too many for one call",
-                a->batch, static_cast<long long>(p.max_pages) << p.page_shift);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     rc = ensure_buffer(ctx, &ctx->kv4, kv4_workspace(ctx), stream_is_capturing(st), "workspace of the 4-bit attention");
     if (rc != DKV_OK) return rc;
