@@ -56,10 +56,10 @@ int check_kv4_pool(const dkv_context* ctx, const dkv_kv4_pool* pool) {
 //    heads side by side, whose rows of a token are read together.
 //  - Where the page table has room for a few steps only (`room` tokens), nothing is split: a second launch and the
 //    records' way through memory cost more than a few steps one behind the other.  With blocks to spare, token lanes make it
-//    fewer steps (32 query heads on 8, one request of 77 tokens: 6.2 us as one step of four lanes, 8.4 us as three steps, 9.0 us
+//    fewer steps (32 query heads on 8, one request of 77 tokens: 4.8 us as one step of four lanes, 7 us as three steps, 7.5 us
 //    split); with half a grid of segments up to 8 steps (64 requests of 256 tokens: 10.6 us, split 19.2 us).
 //  - Very few segments (one long request): two heads per block and the other warps as token lanes, joined in the block, leave
-//    a quarter of the records to merge (131071 tokens: 39 us, 42 us with eight heads).
+//    a quarter of the records to merge (131071 tokens: 40.5 us, 41.6 us with eight heads).
 template <int NT>
 void kv4_shape(int batch, int nh_kv, int n_cc, int64_t room, int grid, int* hg, int* ts, int* whole) {
     constexpr int W = kKv4Warps<NT>;
@@ -280,7 +280,7 @@ int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* a, void* stream) 
     DKV_REQUIRE(a->n_tokens >= 0 && a->nh_q >= 0 && a->nh_k >= 0 && a->nh_q <= 65535 && a->nh_k <= 65535, "bad sizes");
     if (a->n_tokens == 0 || a->nh_q + a->nh_k == 0) return DKV_OK;
     const int64_t rows = a->n_tokens * (a->nh_q + a->nh_k);
-    DKV_REQUIRE(rows <= (static_cast<int64_t>(INT32_MAX) - 1) * 16, "too many rows");
+    DKV_REQUIRE(rows <= static_cast<int64_t>(INT32_MAX) * 4, "too many rows");
     DKV_REQUIRE(a->cos_sin == nullptr || (a->positions != nullptr && a->max_pos > 0), "a rotation needs positions and a table");
     DKV_REQUIRE(a->cos_sin == nullptr || aligned(a->cos_sin, 16), "cos_sin must be 16-byte aligned");
     DKV_REQUIRE(a->eps >= 0.f, "eps must not be negative");

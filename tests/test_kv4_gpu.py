@@ -102,6 +102,18 @@ def test_empty_calls_do_nothing():
 
 
 # ------------------------------------------------------------------------------------------------ attention
+@pytest.fixture(params=[0, 3000], ids=["narrow", "wide"])
+def columns(request):
+    """Page tables with room for the lengths alone, where nothing is split, and with room for many more tokens, where segments
+    are cut and merged."""
+    return request.param
+
+
+def _widen(c, columns):
+    c["table"] = torch.cat([c["table"], torch.zeros(c["table"].shape[0], columns, dtype=torch.int32)], 1)
+    return c
+
+
 def _case(lens, nh_q, nh_kv, page, n_q, seed, host=False, k_scale=1.0, v_scale=1.0, spread=0.7, q_std=1.0):
     g = torch.Generator().manual_seed(seed)
     counts = [-(-n // page) for n in lens]
@@ -161,24 +173,24 @@ RAGGED = [1, 0, 2, 15, 16, 17, 31, 33, 64, 65, 127, 128, 129, 300, 513]
 
 
 @pytest.mark.parametrize("nh_q,nh_kv", [(4, 4), (8, 2), (8, 1), (6, 3), (7, 7), (12, 1), (16, 1), (40, 2), (34, 2), (9, 9), (20, 10), (32, 8), (33, 11), (17, 17)])
-def test_head_groupings(nh_q, nh_kv):
-    c = _case(RAGGED, nh_q, nh_kv, 16, 1, 100 + nh_q)
+def test_head_groupings(nh_q, nh_kv, columns):
+    c = _widen(_case(RAGGED, nh_q, nh_kv, 16, 1, 100 + nh_q), columns)
     _check(c, *_run(c))
     assert get_context(0).read_status() == 0
 
 
 @pytest.mark.parametrize("page", [1, 2, 4, 8, 32, 64, 256])
 @pytest.mark.parametrize("host", [False, True])
-def test_page_sizes_and_pool_places(page, host):
-    c = _case([1, 5, 40, 0, 257, 300], 8, 2, page, 1, 200 + page, host=host)
+def test_page_sizes_and_pool_places(page, host, columns):
+    c = _widen(_case([1, 5, 40, 0, 257, 300], 8, 2, page, 1, 200 + page, host=host), columns)
     _check(c, *_run(c))
 
 
 @pytest.mark.parametrize("n_q", [2, 3, 4, 5, 8, 17, 64])
 @pytest.mark.parametrize("nh_q,nh_kv", [(4, 4), (8, 2), (12, 1)])
-def test_several_query_tokens(n_q, nh_q, nh_kv):
+def test_several_query_tokens(n_q, nh_q, nh_kv, columns):
     """Every query token attends its own prefix; lengths shorter than n_q leave the first rows without any token."""
-    c = _case([n_q, 0, 1, n_q - 1, n_q + 1, 16 + n_q, 47, 100, 130], nh_q, nh_kv, 16, n_q, 300 + n_q)
+    c = _widen(_case([n_q, 0, 1, n_q - 1, n_q + 1, 16 + n_q, 47, 100, 130], nh_q, nh_kv, 16, n_q, 300 + n_q), columns)
     _check(c, *_run(c))
 
 
@@ -190,15 +202,15 @@ def test_pool_scales_and_softmax_scale():
 
 
 @pytest.mark.parametrize("q_std", [1e-30, 1e-3, 30.0])
-def test_small_and_large_queries(q_std):
+def test_small_and_large_queries(q_std, columns):
     """Large scores make the softmax a choice of one token; the running maximum moves on the way there."""
-    c = _case([1, 40, 333, 1025], 8, 2, 16, 1, 500, q_std=q_std)
+    c = _widen(_case([1, 40, 333, 1025], 8, 2, 16, 1, 500, q_std=q_std), columns)
     _check(c, *_run(c))
 
 
-def test_rising_scores_move_the_maximum_at_every_tile():
+def test_rising_scores_move_the_maximum_at_every_tile(columns):
     n = 700
-    c = _case([n, n], 4, 2, 16, 1, 510)
+    c = _widen(_case([n, n], 4, 2, 16, 1, 510), columns)
     k = torch.zeros((n // 16 + 1) * 16 * 2 + 16, 2, 128, dtype=torch.bfloat16)
     direction = torch.sign(torch.randn(128, generator=torch.Generator().manual_seed(1)))
     for b in range(2):
@@ -212,13 +224,18 @@ def test_rising_scores_move_the_maximum_at_every_tile():
     _check(c, *_run(c))
 
 
-def test_one_long_request_and_a_batch_of_short_ones():
-    c = _case([9001], 8, 2, 64, 1, 520)
+@pytest.mark.parametrize("nh_q,nh_kv,page,n_q", [(8, 2, 64, 1), (8, 8, 16, 1), (32, 8, 16, 2), (16, 4, 1, 3), (5, 5, 32, 1)])
+def test_one_long_request(nh_q, nh_kv, page, n_q):
+    c = _case([9001], nh_q, nh_kv, page, n_q, 520)
     _check(c, *_run(c))
-    c = _case([1 + i % 37 for i in range(300)], 4, 2, 4, 1, 521)
-    _check(c, *_run(c))
-    c = _case([i % 23 for i in range(2000)], 2, 2, 16, 1, 522)
-    _check(c, *_run(c))
+
+
+def test_many_short_requests(columns):
+    """More requests than blocks, and more than one launch takes."""
+    _check2 = lambda c: _check(c, *_run(c))  # noqa: E731
+    _check2(_widen(_case([1 + i % 37 for i in range(300)], 4, 2, 4, 1, 521), columns))
+    _check2(_widen(_case([i % 23 for i in range(2000)], 2, 2, 16, 1, 522), columns))
+    _check2(_widen(_case([40 + i % 90 for i in range(70)], 8, 8, 16, 1, 523), columns))
 
 
 def test_row_map_strides_and_2d_queries():
@@ -241,9 +258,9 @@ def test_row_map_strides_and_2d_queries():
     _check(c, flat, want=want)
 
 
-def test_tokens_behind_the_length_and_later_query_tokens_do_not_matter():
+def test_tokens_behind_the_length_do_not_matter(columns):
     """Slots behind a request's length hold not-a-number scales; they are never part of a result."""
-    c = _case([19, 40], 4, 2, 16, 2, 540)
+    c = _widen(_case([19, 40], 4, 2, 16, 2, 540), columns)
     for b, n in enumerate(c["lens"]):
         for t in range(n, -(-n // 16) * 16):
             slot = ref.slots_of(c["table"][b].tolist(), t + 1, 16)[t]
@@ -274,8 +291,8 @@ def test_bad_pages_rows_and_lengths_are_reported_and_bounded():
     assert torch.equal(out[[0, 3]], good[[0, 3]]) and not out[1:3].any()
 
 
-def test_not_a_number_in_a_query_stays_in_its_row():
-    c = _case([64, 64], 8, 2, 16, 2, 560)
+def test_not_a_number_in_a_query_stays_in_its_row(columns):
+    c = _widen(_case([64, 64], 8, 2, 16, 2, 560), columns)
     want = _want(c)
     c["q"][0, 1, 3, 5] = math.nan
     out, lse = _run(c)
@@ -286,8 +303,9 @@ def test_not_a_number_in_a_query_stays_in_its_row():
     assert ((got - want[0]).abs() <= want[2])[mask].all()
 
 
-def test_the_same_inputs_give_the_same_bits_on_another_stream_and_in_a_graph():
-    c = _case([1, 77, 900, 0, 2500, 33], 8, 2, 16, 1, 570)
+@pytest.mark.parametrize("n_q", [1, 3])
+def test_the_same_inputs_give_the_same_bits_on_another_stream_and_in_a_graph(n_q):
+    c = _case([1, 77, 900, 0, 2500, 33], 16, 4, 16, n_q, 570)
     first, lse = _run(c)
     q, table = c["q"].to(DEV), c["table"].to(DEV)
     lens = torch.tensor(c["lens"], dtype=torch.int32, device=DEV)
@@ -310,3 +328,85 @@ def test_the_same_inputs_give_the_same_bits_on_another_stream_and_in_a_graph():
     torch.cuda.synchronize()
     _check(c, out, want=_want(c, shorter))
     assert get_context(0).read_status() == 0
+
+
+def test_after_copies_fills_and_joined_streams_eager_and_captured():
+    """What comes before a call in its stream need not be a kernel: every call sees what was enqueued before it."""
+    c = _case([200, 77], 8, 2, 16, 1, 580)
+    want = _run(c)[0]
+    table, lens = c["table"].to(DEV), torch.tensor(c["lens"], dtype=torch.int32, device=DEV)
+    q_new, q = c["q"].to(DEV), torch.zeros(2, 1, 8, 128, dtype=torch.bfloat16, device=DEV)
+    rows = _rows(4, 2, 9).to(DEV)
+    k_in, slots = torch.zeros_like(rows), torch.arange(4, dtype=torch.int32, device=DEV)      # the padding page: nobody attends it
+    out = torch.zeros_like(q)
+    got = [torch.zeros_like(rows) for _ in range(2)]
+    side = torch.cuda.Stream()
+
+    def step():
+        q.copy_(q_new)                                   # a device-to-device copy just before the attention
+        kernel.decode_kv4(q, c["pool"], lens, c["scale"], table, out=out)
+        q.zero_()                                        # must not overtake it
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            k_in.copy_(rows)
+        here.wait_stream(side)
+        kernel.store_kv4(c["pool"], slots, k_in, k_in)   # after the join
+        k_in.zero_()
+        kernel.load_kv4(c["pool"], slots, *got)
+        kernel.decode_kv4(q_new, c["pool"], lens, c["scale"], table)
+
+    step()
+    torch.cuda.synchronize()
+    values = ref.values(*ref.quantise(rows.cpu()))
+    assert torch.equal(out, want) and torch.equal(got[0].cpu().double(), values)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(20):
+        for t in (out, *got, c["pool"].k_codes[:4], c["pool"].v_scales[:4]):
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(got[0].cpu().double(), values) and torch.equal(got[1].cpu().double(), values)
+
+
+def test_rows_behind_four_gigabytes():
+    n, nh = 8_500_000, 8                                  # 4.35 GB of codes
+    codes, scales = torch.empty(n, nh, 64, dtype=torch.uint8, device=DEV), torch.empty(n, nh, 8, dtype=torch.uint8, device=DEV)
+    for page in (16, 1):
+        pool = kernel.KV4Pool(codes, scales, codes, scales, page_size=page)      # K and V are the same rows
+        length = 40
+        first = (n // 16 - 3) * 16
+        slots = torch.arange(first, first + length, device=DEV)
+        k = _rows(length, nh, 31).to(DEV)
+        kernel.store_kv4(pool, slots, k, k)
+        back = kernel.load_kv4(pool, slots)
+        want = ref.values(*ref.quantise(k.cpu()))
+        assert torch.equal(back[0].cpu().double(), want) and torch.equal(back[1].cpu().double(), want)
+        table = (torch.arange(-(-length // page), dtype=torch.int32, device=DEV) + first // page)[None]
+        q = torch.randn(1, 16, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+        out = kernel.decode_kv4(q.to(DEV), pool, torch.tensor([length], dtype=torch.int32, device=DEV), 128 ** -0.5, table)
+        o, _, e = ref.attend(q, want, want, length, 128 ** -0.5)
+        assert ((out.cpu().double() - o).abs() <= e).all()
+    assert get_context(0).read_status() == 0
+
+
+def test_rows_that_are_aligned_to_16_bytes_only():
+    n, nh = 37, 3
+    flat = _rows(n, nh, 33).reshape(-1)
+    buf = torch.zeros(flat.numel() + 8, dtype=torch.bfloat16, device=DEV)
+    buf[8:] = flat.to(DEV)
+    k = buf[8:].view(n, nh, 128)
+    pool = kernel.KV4Pool.empty(n, nh, device=DEV)
+    slots = torch.arange(n, dtype=torch.int32, device=DEV)
+    kernel.store_kv4(pool, slots, k, k)
+    outs = [torch.zeros(flat.numel() + 8, dtype=torch.bfloat16, device=DEV)[8:].view(n, nh, 128) for _ in range(2)]
+    kernel.load_kv4(pool, slots, *outs)
+    want = ref.values(*ref.quantise(flat.view(n, nh, 128)))
+    assert torch.equal(outs[0].cpu().double(), want) and torch.equal(outs[1].cpu().double(), want)
+    odd = torch.zeros(flat.numel() + 4, dtype=torch.bfloat16, device=DEV)[4:].view(n, nh, 128)
+    with pytest.raises(RuntimeError, match="aligned"):
+        kernel.store_kv4(pool, slots, odd, k)
+    with pytest.raises(RuntimeError, match="aligned"):
+        kernel.load_kv4(pool, slots, odd, outs[0])

@@ -144,6 +144,18 @@ def test_release_takes_effect_as_a_whole_or_not_at_all():
         assert torch.equal(f.cpu(), free) and int(n_free) == 2
 
 
+def test_outputs_that_are_not_aligned():
+    lens, new, page = [0, 30], [5, 3000], 16
+    rows, table, order, spare = _setup(lens, page, 200, 200, 15)
+    state = ref.Pages(table, order, spare, page)
+    buf = torch.full((2, 3010), -9, dtype=torch.int32, device=DEV)
+    slots, positions = buf[0, 1:3006], buf[1, 2:3007]
+    kernel.assign_pages(table.to(DEV), _i32(lens), _i32(new), order.to(DEV), _i32([spare]), page, 3005, rows=_i32(rows), slots=slots, positions=positions)
+    want = state.assign(rows, lens, new)
+    assert slots.cpu().tolist() == want[0] and positions.cpu().tolist() == want[1]
+    assert (buf[0, :1] == -9).all() and (buf[0, 3006:] == -9).all() and (buf[1, :2] == -9).all() and (buf[1, 3007:] == -9).all()
+
+
 def test_no_requests():
     table, free, n_free = torch.zeros(2, 2, dtype=torch.int32, device=DEV), _i32([1, 2]), _i32([2])
     got = kernel.assign_pages(table, _i32([]), _i32([]), free, n_free, 16, 0)

@@ -32,14 +32,15 @@ def _close(got, want, bound):
 
 
 @pytest.mark.parametrize("fused", [False, True])
-@pytest.mark.parametrize("n,hq,hk", [(1, 1, 1), (1, 32, 8), (3, 5, 1), (7, 4, 4), (130, 28, 4), (1000, 3, 2), (2, 56, 56)])
+@pytest.mark.parametrize("n,hq,hk", [(1, 1, 1), (1, 32, 8), (3, 5, 1), (7, 4, 4), (130, 28, 4), (1000, 3, 2), (2, 56, 56), (5000, 32, 8), (6007, 9, 3), (12000, 5, 0)])
 def test_norm_and_rotation(n, hq, hk, fused):
     q, k, qd, kd, g = _inputs(n, hq, hk, n + hq, fused)
     cs = workloads.build_cos_sin(2000, 10000.0)
     pos = torch.randint(0, 2000, (n,), generator=g).to(torch.int32 if n % 2 else torch.int64)
     wq = (1 + 0.3 * torch.randn(128, generator=g)).to(torch.bfloat16)
     wk = torch.randn(hk, 128, generator=g)                                  # per head, fp32
-    for w_q, w_k, table in ((wq, wk, cs), (None, None, cs), (wq, None, None), (None, wk[0].contiguous(), cs)):
+    per_head = torch.randn(hq, 128, generator=g).to(torch.bfloat16)
+    for w_q, w_k, table in ((wq, wk, cs), (None, None, cs), (wq, None, None), (per_head, torch.randn(128, generator=g), cs)):
         dev = lambda t: None if t is None else t.to(DEV)  # noqa: E731
         got = kernel.qk_norm_rope(qd, kd, None if table is None else pos.to(DEV), dev(table), dev(w_q), dev(w_k), eps=1e-5)
         for y, x, w in zip(got, (q, k), (w_q, w_k)):
