@@ -83,6 +83,12 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
+// base + slot * row, in one instruction.
+__device__ __forceinline__ const uint8_t* row_of(const uint8_t* base, unsigned slot, unsigned row) {
+    const uint8_t* p;
+    asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(p) : "r"(slot), "r"(row), "l"(base));
+    return p;
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -253,7 +259,6 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
             const unsigned code_row = p.nh_kv * 64, scale_row = p.nh_kv * 8;                 // bytes per token
             const uint8_t* k_lane = p.k_codes + kvh * 64 + c * 16 + (WIDE ? tau * code_row : 0u);
             const uint8_t* v_lane = p.v_codes + kvh * 64 + c * 16 + (WIDE ? tau * code_row : 0u);
-            const unsigned long long row8 = 8ull * code_row;
             const int s_tau = tau + (c & 1) * 8;
             const uint8_t* s_lane = ((c & 2) ? p.v_scales : p.k_scales) + kvh * 8 + (WIDE ? s_tau * scale_row : 0);
             const uint32_t k_dst = ring + lane * 16;
@@ -285,29 +290,27 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
                 if constexpr (WIDE) {
                     // A page lies in the pool as a whole: rows behind the length may be addressed, but are not read.
                     const int s0 = __shfl_sync(0xffffffffu, now, (2 * i) & 31), s1 = __shfl_sync(0xffffffffu, now, (2 * i + 1) & 31);
-                    const bool plain = left >= kKv4Tile && (s0 | s1) >= 0;
+                    if (left >= kKv4Tile && (s0 | s1) >= 0) {
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {        // a half behind the length is filled with zeros
-                        const int slot = half ? s1 : s0;
-                        const unsigned first = plain ? slot : max(slot, 0);
-                        const unsigned long long codes = static_cast<unsigned long long>(first) * code_row;
-                        const uint8_t *k0 = k_lane + codes, *v0 = v_lane + codes, *k1 = k0 + row8, *v1 = v0 + row8;
-                        const uint8_t* sp = s_lane + static_cast<unsigned long long>(first) * scale_row;
-                        const uint32_t h = half * kKv4HalfBytes;
-                        if (plain) {
-                            cp_async16(kd + h, k0);
-                            cp_async16(kd + h + 512, k1);
-                            cp_async16(vd + h, v0);
-                            cp_async16(vd + h + 512, v1);
-                            cp_async8(sd + h, sp);
-                        } else {
-                            const int n = slot < 0 ? 0 : left - half * 16;
+                        for (int half = 0; half < 2; ++half) {
+                            const unsigned first = half ? s1 : s0, h = half * kKv4HalfBytes;
+                            cp_async16(kd + h, row_of(k_lane, first, code_row));
+                            cp_async16(kd + h + 512, row_of(k_lane, first + 8, code_row));
+                            cp_async16(vd + h, row_of(v_lane, first, code_row));
+                            cp_async16(vd + h + 512, row_of(v_lane, first + 8, code_row));
+                            cp_async8(sd + h, row_of(s_lane, first, scale_row));
+                        }
+                    } else {                              // the end of a request, or no page: what is not read is filled with zeros
+#pragma unroll 1
+                        for (int half = 0; half < 2; ++half) {
+                            const int slot = half ? s1 : s0, n = slot < 0 ? 0 : left - half * 16;
+                            const unsigned first = max(slot, 0), h = half * kKv4HalfBytes;
                             const uint32_t n0 = tau < n ? 16u : 0u, n1 = tau + 8 < n ? 16u : 0u;
-                            cp_async16(kd + h, k0, n0);
-                            cp_async16(kd + h + 512, k1, n1);
-                            cp_async16(vd + h, v0, n0);
-                            cp_async16(vd + h + 512, v1, n1);
-                            cp_async8(sd + h, sp, ((c & 1) ? n1 : n0) >> 1);
+                            cp_async16(kd + h, row_of(k_lane, first, code_row), n0);
+                            cp_async16(kd + h + 512, row_of(k_lane, first + 8, code_row), n1);
+                            cp_async16(vd + h, row_of(v_lane, first, code_row), n0);
+                            cp_async16(vd + h + 512, row_of(v_lane, first + 8, code_row), n1);
+                            cp_async8(sd + h, row_of(s_lane, first, scale_row), ((c & 1) ? n1 : n0) >> 1);
                         }
                     }
                 } else {
@@ -316,14 +319,12 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
                         const int a = __shfl_sync(0xffffffffu, now, half * 16 + tau), b8 = __shfl_sync(0xffffffffu, now, half * 16 + tau + 8);
                         const uint32_t n0 = a < 0 ? 0u : 16u, n1 = b8 < 0 ? 0u : 16u;
                         const unsigned ua = static_cast<unsigned>(max(a, 0)), ub = static_cast<unsigned>(max(b8, 0));
-                        const unsigned long long ra = static_cast<unsigned long long>(ua) * code_row, rb = static_cast<unsigned long long>(ub) * code_row;
-                        const uint8_t* sp = s_lane + static_cast<unsigned long long>((c & 1) ? ub : ua) * scale_row;
                         const uint32_t h = half * kKv4HalfBytes;
-                        cp_async16(kd + h, k_lane + ra, n0);
-                        cp_async16(kd + h + 512, k_lane + rb, n1);
-                        cp_async16(vd + h, v_lane + ra, n0);
-                        cp_async16(vd + h + 512, v_lane + rb, n1);
-                        cp_async8(sd + h, sp, ((c & 1) ? n1 : n0) >> 1);
+                        cp_async16(kd + h, row_of(k_lane, ua, code_row), n0);
+                        cp_async16(kd + h + 512, row_of(k_lane, ub, code_row), n1);
+                        cp_async16(vd + h, row_of(v_lane, ua, code_row), n0);
+                        cp_async16(vd + h + 512, row_of(v_lane, ub, code_row), n1);
+                        cp_async8(sd + h, row_of(s_lane, (c & 1) ? ub : ua, scale_row), ((c & 1) ? n1 : n0) >> 1);
                     }
                 }
             };

@@ -681,14 +681,13 @@ def qk_norm_rope(
     return qy, ky
 
 
-def _pages_args(page_table, lens, more, more_name, free_pages, n_free, page_size, rows):
+def _pages_refuse(page_table, lens, more, more_name, free_pages, n_free, page_size, rows) -> None:
+    """Says what is wrong with the arguments of assign_pages or release_pages."""
     b = lens.numel()
     _int32_1d(lens, b, "lens")
     _int32_1d(more, b, more_name)
     _check_page_table(page_table)
-    n_rows, max_pages = page_table.shape
-    stride = page_table.stride(0)
-    if n_rows > 1 and stride < max_pages:
+    if page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
         raise RuntimeError("the rows of page_table must not overlap")
     if free_pages.dtype is not _I32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
         raise RuntimeError("free_pages must be a contiguous 1D int32 tensor")
@@ -699,16 +698,23 @@ def _pages_args(page_table, lens, more, more_name, free_pages, n_free, page_size
         raise RuntimeError(f"page_size ({page_size}) must be a power of two")
     if rows is not None:
         _int32_1d(rows, b, "rows")
-    dev = page_table.get_device()
-    if dev < 0 or lens.get_device() != dev or more.get_device() != dev or free_pages.get_device() != dev or n_free.get_device() != dev:
-        _elsewhere(f"page_table, lens, {more_name}, free_pages and n_free each")
-    rows_ptr = 0
-    if rows is not None:
-        if rows.get_device() != dev:
-            _elsewhere("rows")
-        rows_ptr = rows.data_ptr()
-    return dev, b, _pack_pages(page_table.data_ptr(), stride, n_rows, max_pages, rows_ptr, lens.data_ptr(), more.data_ptr(), b, page_size,
-                               free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr())
+    _elsewhere(f"page_table, lens, {more_name}, free_pages, n_free and rows each")
+
+
+def _pages_args(page_table, lens, more, more_name, free_pages, n_free, page_size, rows):
+    n_rows, max_pages = page_table.shape if page_table.dim() == 2 else (0, 0)
+    b, stride, dev = lens.numel(), page_table.stride(0), page_table.get_device()
+    # One pass over what is right; what is wrong is told apart in _pages_refuse.
+    if not (page_table.dtype is _I32 and lens.dtype is _I32 and more.dtype is _I32 and free_pages.dtype is _I32 and n_free.dtype is _I32
+            and page_table.dim() == 2 and lens.dim() == 1 and free_pages.dim() == 1 and n_free.dim() == 1 and n_free.numel() == 1
+            and more.shape == lens.shape and b <= 4096 and (n_rows <= 1 or stride >= max_pages)
+            and (page_table.is_contiguous() or page_table.stride(1) == 1) and lens.is_contiguous() and more.is_contiguous() and free_pages.is_contiguous()
+            and page_size >= 1 and page_size & (page_size - 1) == 0
+            and lens.get_device() == dev >= 0 and more.get_device() == dev and free_pages.get_device() == dev and n_free.get_device() == dev
+            and (rows is None or (rows.dtype is _I32 and rows.shape == lens.shape and rows.is_contiguous() and rows.get_device() == dev))):
+        _pages_refuse(page_table, lens, more, more_name, free_pages, n_free, page_size, rows)
+    return dev, b, _pack_pages(page_table.data_ptr(), stride, n_rows, max_pages, 0 if rows is None else rows.data_ptr(), lens.data_ptr(),
+                               more.data_ptr(), b, page_size, free_pages.data_ptr(), free_pages.numel(), n_free.data_ptr())
 
 
 def assign_pages(
@@ -746,10 +752,10 @@ def assign_pages(
                 t = lens.new_empty(n)
             else:
                 _int32_1d(t, n, name)
+                if t.get_device() != dev:
+                    _elsewhere(name)
             outs.append(t)
         slots, positions, seq_lens, cu_new = outs
-    if slots.get_device() != dev or positions.get_device() != dev or seq_lens.get_device() != dev or cu_new.get_device() != dev:
-        _elsewhere("every output")
     handle, stream = _call(dev)
     rc = _lib.load().dkv_assign_pages(handle, a, slots.data_ptr(), positions.data_ptr(), n_tokens, seq_lens.data_ptr(), cu_new.data_ptr(), stream)
     if rc:
