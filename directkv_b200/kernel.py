@@ -454,8 +454,10 @@ class KV4Pool:
         self.page_size, self.k_scale, self.v_scale = int(page_size), float(k_scale), float(v_scale)
         self.n_slots, self.nh_kv = n_slots, nh
         self._descs = {}
-        if torch.cuda.is_available():
-            self._resolve(k_codes.get_device() if k_codes.is_cuda else torch.cuda.current_device())
+        if k_codes.is_cuda:
+            self._resolve(k_codes.get_device())
+        elif torch.cuda.is_available():
+            self._resolve(torch.cuda.current_device())
 
     @classmethod
     def empty(cls, n_slots: int, nh_kv: int, page_size: int = 1, device="cuda", k_scale: float = 1.0, v_scale: float = 1.0) -> "KV4Pool":
