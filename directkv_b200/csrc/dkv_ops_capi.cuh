@@ -177,7 +177,7 @@ static Kv4RowsParams kv4_rows_params(const dkv_context* ctx, const dkv_kv4_pool*
     p.slots = slots, p.slots64 = slots64;
     p.n = n;
     p.nh = pool->nh_kv;
-    p.per_block = std::max(1, 256 / (pool->nh_kv * 8));
+    p.per_block = std::max(1, kKv4RowThreads / (pool->nh_kv * 8));
     p.n_slots = pool->n_slots;
     p.status = ctx->status;
     return p;
@@ -196,7 +196,7 @@ int dkv_kv4_store(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots,
     p.k_scale = 1.f / pool->k_scale, p.v_scale = 1.f / pool->v_scale;
     p.wide = aligned(k, 32) && aligned(v, 32) && k_stride % 16 == 0 && v_stride % 16 == 0;
     DKV_ON_DEVICE(ctx);
-    DKV_CUDA(launch_overlapped(kv4_store_kernel, static_cast<unsigned>((n_tokens + p.per_block - 1) / p.per_block), 256, 0, static_cast<cudaStream_t>(stream), p));
+    DKV_CUDA(launch_overlapped(kv4_store_kernel, static_cast<unsigned>((n_tokens + p.per_block - 1) / p.per_block), kKv4RowThreads, 0, static_cast<cudaStream_t>(stream), p));
     ctx->launches += 1;
     return DKV_OK;
 }
@@ -211,7 +211,7 @@ int dkv_kv4_load(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, 
     p.k_scale = pool->k_scale, p.v_scale = pool->v_scale;
     p.wide = aligned(k, 32) && aligned(v, 32);
     DKV_ON_DEVICE(ctx);
-    DKV_CUDA(launch_overlapped(kv4_load_kernel, static_cast<unsigned>((n_tokens + p.per_block - 1) / p.per_block), 256, 0, static_cast<cudaStream_t>(stream), p));
+    DKV_CUDA(launch_overlapped(kv4_load_kernel, static_cast<unsigned>((n_tokens + p.per_block - 1) / p.per_block), kKv4RowThreads, 0, static_cast<cudaStream_t>(stream), p));
     ctx->launches += 1;
     return DKV_OK;
 }
@@ -280,7 +280,7 @@ int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* a, void* stream) 
     DKV_REQUIRE(a->n_tokens >= 0 && a->nh_q >= 0 && a->nh_k >= 0 && a->nh_q <= 65535 && a->nh_k <= 65535, "bad sizes");
     if (a->n_tokens == 0 || a->nh_q + a->nh_k == 0) return DKV_OK;
     const int64_t rows = a->n_tokens * (a->nh_q + a->nh_k);
-    DKV_REQUIRE(rows <= static_cast<int64_t>(INT32_MAX) * 4, "too many rows");
+    DKV_REQUIRE(rows <= static_cast<int64_t>(INT32_MAX) * 2, "too many rows");
     DKV_REQUIRE(a->cos_sin == nullptr || (a->positions != nullptr && a->max_pos > 0), "a rotation needs positions and a table");
     DKV_REQUIRE(a->cos_sin == nullptr || aligned(a->cos_sin, 16), "cos_sin must be 16-byte aligned");
     DKV_REQUIRE(a->eps >= 0.f, "eps must not be negative");
@@ -313,9 +313,9 @@ int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* a, void* stream) 
     // Eight heads per half warp once that still gives every SM 32 warps, else one.
     const int qn = (a->nh_q + 7) / 8, gn = qn + (a->nh_k + 7) / 8;
     if (a->n_tokens * gn >= static_cast<int64_t>(ctx->sm_count) * 64)
-        DKV_CUDA(launch_overlapped(qk_norm_rope_kernel<8, 16>, static_cast<unsigned>((a->n_tokens * gn + 3) / 4), 64, 0, st, p, qn, gn));
+        DKV_CUDA(launch_overlapped(qk_norm_rope_kernel<8, 24>, static_cast<unsigned>((a->n_tokens * gn + 1) / 2), 32, 0, st, p, qn, gn));
     else
-        DKV_CUDA(launch_overlapped(qk_norm_rope_kernel<1, 16>, static_cast<unsigned>((rows + 3) / 4), 64, 0, st, p, a->nh_q, a->nh_q + a->nh_k));
+        DKV_CUDA(launch_overlapped(qk_norm_rope_kernel<1, 32>, static_cast<unsigned>((rows + 1) / 2), 32, 0, st, p, a->nh_q, a->nh_q + a->nh_k));
     ctx->launches += 1;
     return DKV_OK;
 }

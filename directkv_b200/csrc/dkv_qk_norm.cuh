@@ -56,15 +56,16 @@ __device__ __forceinline__ uint2 pack4(const uint64_t (&v)[2]) {
 // Half a warp per row: lane l holds dimensions 4 l .. 4 l + 3 and 64 + 4 l .. 64 + 4 l + 3.  The sixteen lanes take R heads of
 // one token: the angles (512 bytes per token, as much as two rows) and the weights are loaded and
 // multiplied with one another once for all of them, y = inv (u A - v B), inv (v C + u D), and R rows are on their way at a time.
-// Bound by HBM once there are many tokens: 16384 tokens of 32 + 8 heads out of a fused projection take 65 us for 344 MB (5.3
-// TB/s, 0.81 of the copy rate; 69 us under the power limit).  One head per half warp takes 109 us (angles and weights
-// read for every row), four 75 us; blocks of two warps, which end and begin at all times, 3 us less than blocks of eight.
+// Bound by HBM once there are many tokens: 16384 tokens of 32 + 8 heads out of a fused projection take 61 us for 344 MB (5.7
+// TB/s, 0.87 of the copy rate).  One head per half warp takes 109 us (angles and weights read for every row), four 75 us.
+// Blocks of one warp end and begin at all times, so that loads, arithmetic and stores of different blocks overlap: 65 us with
+// two warps, 70 us with eight.
 template <int R, int BLOCKS>
-__global__ void __launch_bounds__(64, BLOCKS) qk_norm_rope_kernel(const QkNormParams p, int q_groups, int groups) {
+__global__ void __launch_bounds__(32, BLOCKS) qk_norm_rope_kernel(const QkNormParams p, int q_groups, int groups) {
     grid_wait();
     grid_trigger();
     const int l = threadIdx.x & 15;
-    const long long id = (static_cast<long long>(blockIdx.x) * 64 + threadIdx.x) >> 4;
+    const long long id = (static_cast<long long>(blockIdx.x) * 32 + threadIdx.x) >> 4;
     if (id >= p.n_tokens * groups) return;                // by halves of a warp
     const long long tok = id < 0x7fffffff ? static_cast<unsigned>(id) / static_cast<unsigned>(groups) : id / groups;
     const int grp = static_cast<int>(id - tok * groups);

@@ -620,24 +620,29 @@ def decode_kv4(
 
 def _norm_side(x, y, w, n: int, dev: int, name: str):
     """Output and struct fields of the queries or the keys."""
-    shape = x.shape
+    shape, st = x.shape, x.stride()
     if len(shape) != 3 or shape[0] != n:
         raise RuntimeError(f"{name} must be [{n}, NH, {HEAD_DIM}]")
-    xs, nh = _heads_stride(x, name), shape[1]
+    nh = shape[1]
+    row = nh * HEAD_DIM
+    if x.dtype is not _BF16 or shape[2] != HEAD_DIM or st[2] != 1 or (st[1] != HEAD_DIM and nh > 1):
+        _heads_stride(x, name)                                # raises
     if y is None:
-        y, ys = torch.empty_like(x), nh * HEAD_DIM            # (contiguous for a slice of a fused projection, too)
+        y, ys = torch.empty_like(x), row                      # (contiguous for a slice of a fused projection, too)
     else:
         if y.shape != shape or y.get_device() != dev:
             raise RuntimeError(f"{name}_out must have the shape of {name} and its device")
-        ys = xs if y is x else _heads_stride(y, f"{name}_out")
+        ys = _heads_stride(y, f"{name}_out")
     per_head = f32 = w_ptr = 0
     if w is not None:
-        per_head, f32, w_ptr = w.dim() == 2, w.dtype is _F32, w.data_ptr()
-        if not (f32 or w.dtype is _BF16) or not w.is_contiguous() or w.shape != ((nh, HEAD_DIM) if per_head else (HEAD_DIM,)) or w.get_device() != dev:
+        f32, w_shape = w.dtype is _F32, w.shape
+        per_head = len(w_shape) == 2
+        if not (f32 or w.dtype is _BF16) or w_shape != ((nh, HEAD_DIM) if per_head else (HEAD_DIM,)) or not w.is_contiguous() or w.get_device() != dev:
             raise RuntimeError(f"{name}_weight must be contiguous bfloat16 or float32 [{HEAD_DIM}] or [{nh}, {HEAD_DIM}], a CUDA tensor on the device of {name}")
+        w_ptr = w.data_ptr()
     if dev < 0 or x.get_device() != dev:
         _elsewhere(name)
-    return y, nh, x.data_ptr(), xs, y.data_ptr(), ys, w_ptr, f32, per_head
+    return y, nh, x.data_ptr(), st[0] if n > 1 else row, y.data_ptr(), ys, w_ptr, f32, per_head
 
 
 def qk_norm_rope(
