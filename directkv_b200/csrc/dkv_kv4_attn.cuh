@@ -11,9 +11,9 @@
 // fp32 scores).  P is rounded to fp16 (2^-11, against bf16's 2^-8); scores, maximum, sum and O are fp32.
 //
 // What bounds it is bytes, 144 per token and KV head, and close behind them the instructions that turn codes into fp16: 64
-// requests of 12000 to 20000 tokens, 32 query heads on 8, take 223 us (5.35 TB/s, 0.82 of the measured copy rate), copies
+// requests of 12000 to 20000 tokens, 32 query heads on 8, take 221 us (5.41 TB/s, 0.83 of the measured copy rate), copies
 // alone 192 us; the arithmetic needs 115 cycles per 16 tokens and SM, HBM 100.  Under sustained load the power limit
-// lowers the clock and with it this kernel (257 us at 1.68 GHz).  So the loop is written for few instructions: 32 tokens
+// lowers the clock and with it this kernel (248 us).  So the loop is written for few instructions: 32 tokens
 // per step with one vote on the running maximum, table entries looked up for 16 steps at a time, one multiply-add per
 // copy address.
 //
