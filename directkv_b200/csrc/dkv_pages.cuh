@@ -7,7 +7,9 @@
 // a release of exactly what the last call took restores the stack.
 //
 // A call takes effect as a whole or not at all: too few pages, a row or length outside the table, or more tokens
-// than the caller has room for leave stack, table and lengths as they were, give slots of -1, and set a status bit.
+// than the caller has room for leave stack, table and lengths as they were, give slots of -1, and set a status bit.  So do two
+// requests that change one row (they would share its new pages, or free its old ones twice); requests that change nothing, the padding
+// of a batch, may repeat a row.
 #pragma once
 
 #include "dkv_common.cuh"
@@ -62,12 +64,13 @@ __device__ __forceinline__ void block_scan2(long long& a, long long& b, long lon
     *ta = sa, *tb = sb;
 }
 
-// Bound by latency: one scan, one search and one look-up per thread.  64 requests with one more token each take 4 us, 256 prompts
-// of 1.0 M tokens 8 us (8 MB of slots and positions).
+// Bound by latency: one scan, one search and one look-up per thread.  64 requests with one more token each and their release take
+// 8.3 us in two launches, 256 prompts of 1.0 M tokens 17 us (8 MB of slots and positions); the look for repeated rows is 0.2 and 1.5
+// us of a launch.
 template <bool RELEASE>
 __global__ void __launch_bounds__(kPagesThreads) pages_kernel(const PagesParams p) {
-    __shared__ int cu_tok[kPagesMaxBatch + 1];       // release: unused
-    __shared__ int cu_page[kPagesMaxBatch + 1];
+    __shared__ int cu_tok[2 * (kPagesMaxBatch + 1)]; // (release: first half unused)
+    int* const cu_page = cu_tok + kPagesMaxBatch + 1;
     __shared__ long long sh[64];
     __shared__ int sh_last;
     grid_wait();
@@ -75,6 +78,23 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(const PagesParams 
     const int P = 1 << p.page_shift;
     const int top = *reinterpret_cast<const volatile int*>(p.n_free);
     bool bad = top < 0 || top > p.free_cap;
+    if (p.rows != nullptr && p.batch > 1) {
+        // The rows that change go into a hash table of at least twice as many places, in the room of the prefix sums.
+        const int bits = 33 - __clz(p.batch - 1), mask = (1 << bits) - 1;
+        for (int i = threadIdx.x; i <= mask; i += kPagesThreads) cu_tok[i] = -1;
+        __syncthreads();
+        for (int b = threadIdx.x; b < p.batch; b += kPagesThreads) {
+            const int row = p.rows[b], x = p.more[b];
+            const bool changes = RELEASE ? (p.lens[b] + P - 1ll) >> p.page_shift > (x + P - 1ll) >> p.page_shift : x > 0;
+            if (!changes || row < 0) continue;
+            for (unsigned at = (static_cast<unsigned>(row) * 0x9E3779B1u) >> (32 - bits);; at = (at + 1) & mask) {
+                const int other = atomicCAS(&cu_tok[at], -1, row);
+                bad |= other == row;
+                if (other == row || other == -1) break;
+            }
+        }
+        __syncthreads();
+    }
     long long tok = 0, pages = 0;
     // Every block scans the whole batch (a few thousand integers at most): no launch and no hand-over between
     // the scan and the fill.

@@ -742,9 +742,9 @@ def assign_pages(
 
     Returns ``(slots [n_tokens], positions [n_tokens], seq_lens [B], cu_new [B + 1])``: slot and position of each new token
     packed in request order, the lengths with the new tokens, and the packed offsets.  Entries behind the last token are
-    left as they were.  Rows must be distinct.  The call takes effect as a whole or not at all: when the pages run out, or a
-    length does not fit the table or ``n_tokens``, everything is left as it was, the slots are -1 and the status
-    word says why.
+    left as they were.  The call takes effect as a whole or not at all: when the pages run out, a length does not fit the
+    table or ``n_tokens``, or two requests with new tokens have one row, everything is left as it was, the slots are -1 and
+    the status word says why.
     """
     dev, b, a = _pages_args(page_table, lens, new_lens, "new_lens", free_pages, n_free, page_size, rows)
     if not 0 <= n_tokens < 2 ** 31:
@@ -782,7 +782,8 @@ def release_pages(
     """Puts the pages behind the tokens that stay back on the stack of free pages, on the GPU.
 
     A release of exactly what the last ``assign_pages`` gave restores the stack.  The table's entries are left; nothing reads
-    them once the lengths are shorter.  As a whole or not at all, like ``assign_pages``.
+    them once the lengths are shorter.  As a whole or not at all, like ``assign_pages``; two requests that give pages of one
+    row back are refused.
     """
     dev, b, a = _pages_args(page_table, lens, keep_lens, "keep_lens", free_pages, n_free, page_size, rows)
     if b == 0:

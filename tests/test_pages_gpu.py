@@ -144,6 +144,30 @@ def test_release_takes_effect_as_a_whole_or_not_at_all():
         assert torch.equal(f.cpu(), free) and int(n_free) == 2
 
 
+@pytest.mark.parametrize("batch", [2, 5, 513, 4096])
+def test_one_row_twice(batch):
+    """Two requests that change one row are refused as a whole; requests that change nothing may repeat it."""
+    page, at = 16, [0, batch - 1]
+    lens, rows = [page] * batch, list(range(batch))
+    rows[at[1]] = rows[at[0]]
+    table = torch.arange(batch, dtype=torch.int32)[:, None].repeat(1, 3).to(DEV)
+    free, n_free = torch.arange(batch, 4 * batch, dtype=torch.int32, device=DEV), _i32([2 * batch])
+    before = table.clone(), free.clone()
+    got = kernel.assign_pages(table, _i32(lens), _i32([1] * batch), free, n_free, page, batch, rows=_i32(rows))
+    assert (got[0] == -1).all() and got[2].tolist() == lens and got[3].tolist() == [0] * (batch + 1)
+    kernel.release_pages(table, _i32(lens), _i32([0] * batch), free, n_free, page, rows=_i32(rows))
+    assert torch.equal(table, before[0]) and torch.equal(free, before[1]) and int(n_free) == 2 * batch
+    assert get_context(0).read_status(clear=True) == BAD_PAGE
+    new = [1] * batch
+    new[at[1]] = 0
+    got = kernel.assign_pages(table, _i32(lens), _i32(new), free, n_free, page, batch, rows=_i32(rows))
+    taken = torch.arange(3 * batch - 1, 2 * batch, -1)
+    assert torch.equal(got[0][:batch - 1].cpu(), (taken * page).to(torch.int32)) and int(n_free) == batch + 1
+    kernel.release_pages(table, got[2], _i32(lens), free, n_free, page, rows=_i32(rows))
+    assert torch.equal(free, before[1]) and int(n_free) == 2 * batch
+    assert get_context(0).read_status() == 0
+
+
 def test_outputs_that_are_not_aligned():
     lens, new, page = [0, 30], [5, 3000], 16
     rows, table, order, spare = _setup(lens, page, 200, 200, 15)
