@@ -121,7 +121,7 @@ int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
     const unsigned rows = static_cast<unsigned>(p.batch) * p.n_q * p.nh_q;
     // Few rows: many blocks had a part of each.
     const bool few = rows <= static_cast<unsigned>(2 * ctx->sm_count) && most_parts > 16;
-    DKV_CUDA(launch_overlapped(few ? kv4_merge_kernel<NT, 16> : kv4_merge_kernel<NT, 4>, rows, few ? 512 : 128, grid * sizeof(float2), st, p, grid));
+    DKV_CUDA(launch_overlapped(few ? kv4_merge_kernel<NT, 16> : kv4_merge_kernel<NT, 4>, rows, few ? 512 : 128, 0, st, p, grid));
     ctx->launches += 1;
     return DKV_OK;
 }
