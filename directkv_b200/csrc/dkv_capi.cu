@@ -497,7 +497,7 @@ cudaError_t attn_mma8_set_attr() {
 
 template <int NT>
 constexpr int kv4_smem(int batch) {
-    return kKv4Warps<NT> * kKv4WarpBytes<NT> + (batch + 1) * static_cast<int>(sizeof(int));
+    return kKv4Warps<NT> * kKv4WarpBytes<NT> + std::max(batch + 1, kKv4Warps<NT> * 33) * static_cast<int>(sizeof(int));
 }
 
 template <int NT, bool WIDE>

@@ -45,6 +45,24 @@ constexpr int kKv4RecFloats = 132;                       // O[128], m (log2 doma
 constexpr float kKv4Low = -3e38f;                        // the running maximum before the first token
 constexpr float kKv4Lag = 8.f;                           // the maximum follows once a score is 2^8 above it: P <= 2^8 in fp16
 
+// Division of 0 .. 2^31 - 1 by a number that the host knows: with 2^(l-1) < d <= 2^l and m = ceil(2^(31+l) / d) < 2^32, the product
+// n m / 2^(31+l) is less than 1 / d above n / d.  A division by a variable is some 150 cycles of latency, and the way from a launch to
+// its first copy has several.
+struct Kv4Div {
+    unsigned m;
+    int shift;
+    Kv4Div() = default;
+    explicit Kv4Div(unsigned d) {
+        int l = 0;
+        while ((1ull << l) < d) ++l;
+        shift = 31 + l;
+        m = static_cast<unsigned>(((1ull << shift) + d - 1) / d);
+    }
+    __device__ __forceinline__ int operator()(int n) const {
+        return static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(n)) * m) >> shift);
+    }
+};
+
 struct Kv4AttnParams {
     const __nv_bfloat16* q;          // row (b, j) at q + (b * n_q + j) * q_stride, [nh_q, 128]
     long long q_stride;
@@ -55,7 +73,7 @@ struct Kv4AttnParams {
     const int* page_table;
     long long pt_stride;
     int pt_rows;                     // 0: unknown
-    int max_pages;                   // entries of a row that may be read
+    int room;                        // tokens that the entries of a row reach
     const int* row_map;              // [batch] or nullptr: row b + row0
     int row0;
     const uint8_t* k_codes;          // [n_slots, nh_kv, 64]
@@ -70,6 +88,8 @@ struct Kv4AttnParams {
     int whole;                       // no segment is split: the list has one entry per segment, and nothing is left to merge
     int n_cc;                        // column chunks of 8 * NT
     int hg, ts, n_hg;                // heads and token lanes of a block (hg * ts <= kKv4Warps<NT>), head groups
+    int tile_shift;                  // log2 of kKv4Tile * ts (ts is a power of two): tokens of a tile
+    Kv4Div by_seg, by_cc, by_hg, by_group, by_nh_q, by_n_q, by_grid;      // n_hg * n_cc, n_cc, ...
     float scale_log2;                // softmax scale * k_scale * log2(e)
     float v_scale;
     float* rec;                      // [blocks, 2, hg, 8 * NT, kKv4RecFloats]
@@ -132,7 +152,10 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 // share, the first total % n blocks have one tile more.
 struct Kv4Deal {
     int each, more;
-    __device__ __forceinline__ Kv4Deal(int total, int n) : each(static_cast<unsigned>(total) / static_cast<unsigned>(n)) { more = total - each * n; }
+    __device__ __forceinline__ Kv4Deal(int total, int n, int grid, Kv4Div by_grid) {
+        each = n == grid ? by_grid(total) : static_cast<unsigned>(total) / static_cast<unsigned>(n);
+        more = total - each * n;
+    }
     __device__ __forceinline__ int share(int i) const { return each * i + min(i, more); }
     __device__ __forceinline__ int owner(int x) const {
         const int edge = more * (each + 1);
@@ -151,12 +174,11 @@ __device__ __forceinline__ int kv4_length(const Kv4AttnParams& p, int b, long lo
     const long long row = p.row_map != nullptr ? p.row_map[b] : b + p.row0;
     *row_out = row;
     const int len = p.seq_lens[b];
-    const long long room = static_cast<long long>(p.max_pages) << p.page_shift;
     if (row < 0 || (p.pt_rows > 0 && row >= p.pt_rows) || len < 0) return -1;
-    return len > room ? -2 : len;
+    return len > p.room ? -2 : len;
 }
 __device__ __forceinline__ int kv4_clean_length(const Kv4AttnParams& p, int code) {
-    return code >= 0 ? code : (code == -2 ? static_cast<int>(static_cast<long long>(p.max_pages) << p.page_shift) : 0);
+    return code >= 0 ? code : (code == -2 ? p.room : 0);
 }
 
 template <int NT>
@@ -174,14 +196,38 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
     int* cum = reinterpret_cast<int*>(smem + W * kKv4WarpBytes<NT>);
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int g = lane >> 2, c = lane & 3;
+    const int tl = p.by_hg(w), hl = w - tl * p.hg;
+    const bool active = tl < p.ts;
+    auto tiles_of = [&](int len) { return static_cast<int>((static_cast<unsigned>(len) + (1u << p.tile_shift) - 1u) >> p.tile_shift); };
 
     grid_wait();
     const int per_tile = p.n_hg * p.n_cc;
     int total;
     if (p.whole) {
         total = p.batch * per_tile;                  // one entry per segment, whatever its length
+    } else if (p.batch <= 32) {
+        // Tiles (of 32 * ts tokens) before every request; a request without tokens has one, which writes its zeros.  Every warp
+        // for itself: without the block's barriers the first copies leave 0.4 us earlier.
+        cum += w * 33;
+        int n = 0;
+        if (lane < p.batch) {
+            long long row;
+            n = max(1, tiles_of(kv4_clean_length(p, kv4_length(p, lane, &row))));
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, n, o);
+            if (lane >= o) n += x;
+        }
+        cum[lane + 1] = n;
+        if (lane == 0) cum[0] = 0;
+        if (blockIdx.x == 0 && w == 0) {
+            p.cum[lane + 1] = n;
+            if (lane == 0) p.cum[0] = 0;
+        }
+        __syncwarp();
+        total = __shfl_sync(0xffffffffu, n, 31) * per_tile;
     } else {
-        // Tiles (of 32 * ts tokens) before every request; a request without tokens has one, which writes its zeros.
         if (threadIdx.x == 0) cum[0] = 0;
         int before = 0;
         for (int b0 = 0; b0 < p.batch; b0 += W * 32) {
@@ -190,7 +236,7 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
             if (b < p.batch) {
                 long long row;
                 const int len = kv4_clean_length(p, kv4_length(p, b, &row));
-                n = max(1, static_cast<int>((static_cast<unsigned>(len) + kKv4Tile * p.ts - 1) / (kKv4Tile * p.ts)));
+                n = max(1, tiles_of(len));
             }
             int inc = n;
 #pragma unroll
@@ -213,11 +259,9 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
     const int blocks = kv4_blocks(total, p.batch * per_tile, gridDim.x);
     grid_trigger();
     if (static_cast<int>(blockIdx.x) >= blocks) return;
-    const Kv4Deal deal(total, blocks);
+    const Kv4Deal deal(total, blocks, gridDim.x, p.by_grid);
     const int x0 = deal.share(blockIdx.x), x1 = deal.share(blockIdx.x + 1);
 
-    const int hl = w % p.hg, tl = w / p.hg;
-    const bool active = tl < p.ts;
     uint8_t* const ring_ptr = smem + w * kKv4WarpBytes<NT>;
     uint4* const q_smem = reinterpret_cast<uint4*>(ring_ptr + kKv4Stages * kKv4StageBytes) + lane;
     const uint32_t ring = smem_u32(ring_ptr);
@@ -227,8 +271,8 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
 
     for (int x = x0; x < x1;) {
         // Segment: one request, head group and column chunk.
-        const int y = x / per_tile;
-        int b = y, entries = 1, seg = x - y * per_tile, tile0 = 0;
+        const int y = p.by_seg(x);                   // (n_hg * n_cc once more below: a register less through the loop)
+        int b = y, entries = 1, seg = x - y * (p.n_hg * p.n_cc), tile0 = 0;
         if (!p.whole) {
             int lo = 0, hi = p.batch - 1;
             while (lo < hi) {
@@ -238,15 +282,16 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
             }
             b = lo;
             entries = cum[b + 1] - cum[b];
-            const int r = x - cum[b] * per_tile;
-            seg = r / entries, tile0 = r - seg * entries;
+            const int r = x - cum[b] * (p.n_hg * p.n_cc);
+            seg = p.n_hg * p.n_cc == 1 ? 0 : static_cast<unsigned>(r) / static_cast<unsigned>(entries);
+            tile0 = r - seg * entries;
         }
         long long row;
         const int code = kv4_length(p, b, &row), len = kv4_clean_length(p, code);
         if (code < 0 && threadIdx.x == 0) atomicOr(p.status, kStatusBadPage);
         const int taken = min(entries - tile0, x1 - x);
-        const int n_tiles = p.whole ? static_cast<int>((static_cast<unsigned>(len) + kKv4Tile * p.ts - 1) / (kKv4Tile * p.ts)) : taken;
-        const int hgi = seg / p.n_cc, cc = seg - hgi * p.n_cc;
+        const int n_tiles = p.whole ? tiles_of(len) : taken;
+        const int hgi = p.by_cc(seg), cc = seg - hgi * p.n_cc;
         const bool whole = taken == entries;
         const int kvh = hgi * p.hg + hl;
         const int* table = p.page_table + row * p.pt_stride;
@@ -347,7 +392,7 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
                 uint4 v[4];
                 uint32_t top = 0;
                 if (col < p.cols) {
-                    const int j = col / p.group, h = kvh * p.group + (col - j * p.group);
+                    const int j = p.by_group(col), h = kvh * p.group + (col - j * p.group);
                     const uint4* src = reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(b) * p.n_q + j) * p.q_stride + h * 128 + c * 32);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[i] = __ldg(src + i);
@@ -561,7 +606,7 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
                     for (int d = 0; d < 16; ++d) v[d] = st.o[(d >> 3) * 4 + (d & 1) * 2 + ((d >> 2) & 1)][n][k + (d & 2)];
                     const float l = st.l[n][k], m = st.m[n][k];
                     if (whole) {
-                        const int j = col / p.group, h = kvh * p.group + (col - j * p.group);
+                        const int j = p.by_group(col), h = kvh * p.group + (col - j * p.group);
                         const long long at = static_cast<long long>(b) * p.n_q + j;
                         const float inv = l == 0.f ? 0.f : p.v_scale / l;          // a not-a-number goes through
                         uint4* dst = reinterpret_cast<uint4*>(p.out + at * p.out_stride + h * 128 + g * 16);
@@ -595,12 +640,12 @@ __global__ void __launch_bounds__(NW * 32) kv4_merge_kernel(const Kv4AttnParams 
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     grid_wait();
     grid_trigger();
-    const int h = blockIdx.x % p.nh_q, j = (blockIdx.x / p.nh_q) % p.n_q, b = blockIdx.x / (p.nh_q * p.n_q);
-    const int kvh = h / p.group, col = j * p.group + (h - kvh * p.group);
-    const int hgi = kvh / p.hg, hl = kvh - hgi * p.hg, cc = col / C, cl = col - cc * C;
+    const int token = p.by_nh_q(blockIdx.x), h = blockIdx.x - token * p.nh_q, b = p.by_n_q(token), j = token - b * p.n_q;
+    const int kvh = p.by_group(h), col = j * p.group + (h - kvh * p.group);
+    const int hgi = p.by_hg(kvh), hl = kvh - hgi * p.hg, cc = col / C, cl = col - cc * C;
     const int first = p.cum[b], tiles = p.cum[b + 1] - first, per_tile = p.n_hg * p.n_cc;
     const int total = p.cum[p.batch] * per_tile;
-    const Kv4Deal deal(total, kv4_blocks(total, p.batch * per_tile, grid));
+    const Kv4Deal deal(total, kv4_blocks(total, p.batch * per_tile, grid), grid, p.by_grid);
     const int s0 = first * per_tile + (hgi * p.n_cc + cc) * tiles;
     const int i0 = deal.owner(s0), n = deal.owner(s0 + tiles - 1) - i0 + 1;
     if (n == 1) return;

@@ -100,14 +100,15 @@ template <int NT>
 int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
     p.n_cc = (p.cols + 8 * NT - 1) / (8 * NT);
     const int full_grid = kv4_grid<NT>(ctx);
-    const int64_t room = static_cast<int64_t>(p.max_pages) << p.page_shift;
-    kv4_shape<NT>(p.batch, p.nh_kv, p.n_cc, room, full_grid, &p.hg, &p.ts, &p.whole);
+    kv4_shape<NT>(p.batch, p.nh_kv, p.n_cc, p.room, full_grid, &p.hg, &p.ts, &p.whole);
     p.n_hg = p.nh_kv / p.hg;
-    const int64_t most_parts = room / (kKv4Tile * p.ts) + 1;
+    p.tile_shift = log2_of(kKv4Tile * p.ts);
+    const int64_t most_parts = p.room / (kKv4Tile * p.ts) + 1;
     const int64_t most_tiles = (p.whole ? 1 : most_parts) * p.batch * p.n_hg * p.n_cc;
     if (most_tiles > INT32_MAX)
-        return fail(DKV_ERR_UNSUPPORTED, "%d requests of up to %lld tokens are too many for one call", p.batch, static_cast<long long>(room));
+        return fail(DKV_ERR_UNSUPPORTED, "%d requests of up to %lld tokens are too many for one call", p.batch, static_cast<long long>(p.room));
     const int grid = static_cast<int>(std::min<int64_t>(full_grid, most_tiles));
+    p.by_seg = Kv4Div(p.n_hg * p.n_cc), p.by_cc = Kv4Div(p.n_cc), p.by_hg = Kv4Div(p.hg), p.by_grid = Kv4Div(grid);
     const size_t smem = kv4_smem<NT>(p.batch);
     const auto kernel = p.page_shift >= 4 ? kv4_attn_kernel<NT, true> : kv4_attn_kernel<NT, false>;
     if (NT == 1) {
@@ -243,7 +244,7 @@ int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_
     p.pt_stride = a->pt_stride;
     p.pt_rows = a->pt_rows;
     p.page_shift = log2_of(pool->page_size);
-    p.max_pages = std::min(a->max_pages, INT32_MAX >> p.page_shift);
+    p.room = std::min(a->max_pages, INT32_MAX >> p.page_shift) << p.page_shift;
     p.row_map = a->row_map;
     p.k_codes = static_cast<const uint8_t*>(pool->k_codes), p.v_codes = static_cast<const uint8_t*>(pool->v_codes);
     p.k_scales = static_cast<const uint8_t*>(pool->k_scales), p.v_scales = static_cast<const uint8_t*>(pool->v_scales);
@@ -252,6 +253,7 @@ int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_
     p.batch = a->batch, p.n_q = a->n_q, p.nh_q = a->nh_q, p.nh_kv = pool->nh_kv;
     p.group = a->nh_q / pool->nh_kv;
     p.cols = a->n_q * p.group;
+    p.by_group = Kv4Div(p.group), p.by_nh_q = Kv4Div(a->nh_q), p.by_n_q = Kv4Div(a->n_q);
     p.scale_log2 = a->softmax_scale * pool->k_scale * 1.4426950408889634f;
     p.v_scale = pool->v_scale;
     p.status = ctx->status;
