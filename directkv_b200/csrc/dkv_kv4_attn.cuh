@@ -11,7 +11,7 @@
 // fp32 scores).  P is rounded to fp16 (2^-11, against bf16's 2^-8); scores, maximum, sum and O are fp32.
 //
 // What bounds it is bytes, 144 per token and KV head, and close behind them the instructions that turn codes into fp16: 64
-// requests of 12000 to 20000 tokens, 32 query heads on 8, take 221 us (5.41 TB/s, 0.83 of the measured copy rate), copies
+// requests of 12000 to 20000 tokens, 32 query heads on 8, take 217 us (5.51 TB/s, 0.84 of the measured copy rate), copies
 // alone 192 us; the arithmetic needs 115 cycles per 16 tokens and SM, HBM 100.  Under sustained load the power limit
 // lowers the clock and with it this kernel (248 us).  So the loop is written for few instructions: 32 tokens
 // per step with one vote on the running maximum, table entries looked up for 16 steps at a time, one multiply-add per
@@ -32,7 +32,7 @@ constexpr int kKv4Stages = 2;
 constexpr int kKv4HalfBytes = 2 * 1024 + 2 * 128;        // 16 tokens: K codes, V codes, K scales, V scales
 constexpr int kKv4StageBytes = 2 * kKv4HalfBytes;
 // Warps of a block and blocks per SM: 16 warps per SM with 8 columns (query fragments in registers), 12 with 16 (in shared
-// memory; 16 drafts of up to 4096 tokens: 36 us, against 48 us as 16 warps that spill).
+// memory; 16 drafts of up to 4096 tokens: 32 us; as 16 warps that spill, at the time, 48 us against 37).
 template <int NT>
 constexpr int kKv4Warps = NT == 1 ? 8 : 4;
 template <int NT>
@@ -163,8 +163,8 @@ struct Kv4Deal {
     }
 };
 // Blocks that take part.  Segments of up to 4 tiles on average that are enough to occupy an eighth of the grid are not cut
-// finer than there are segments: what is gained in steps goes into merging (64 requests of 77 tokens, 32 heads on 8: 14 us
-// with a block per tile).
+// finer than there are segments: what is gained in steps goes into merging (64 requests of 77 tokens in a wide table, 32 heads on
+// 8: 10.5 us, 11.8 us with a block per tile).
 __device__ __forceinline__ int kv4_blocks(int total, int segments, int grid) {
     return min(total <= 4ll * segments && 8ll * segments >= grid ? segments : total, grid);
 }

@@ -56,10 +56,12 @@ int check_kv4_pool(const dkv_context* ctx, const dkv_kv4_pool* pool) {
 //    heads side by side, whose rows of a token are read together.
 //  - Where the page table has room for a few steps only (`room` tokens), nothing is split: a second launch and the
 //    records' way through memory cost more than a few steps one behind the other.  With blocks to spare, token lanes make it
-//    fewer steps (32 query heads on 8, one request of 77 tokens: 4.8 us as one step of four lanes, 7 us as three steps, 7.5 us
-//    split); with half a grid of segments up to 8 steps (64 requests of 256 tokens: 10.6 us, split 19.2 us).
+//    fewer steps (32 query heads on 8, one request of 77 tokens: 4.7 us as one step of four lanes, 6.3 us split).  Two steps are
+//    always left whole, four where the segments occupy a fifth of the grid (64 requests of 512 tokens: 12.6 us, split 18.6; of
+//    1 to 512 tokens: 12.0, split 17.1; 8 of 1024 tokens: 9.2, split 10.9; but one request of 1024 tokens: 8.7, split 7.5), eight
+//    of the plain shape with half a grid of segments (64 requests of 256 tokens, 32 heads: 20.9 us, split 26.6).
 //  - Very few segments (one long request): two heads per block and the other warps as token lanes, joined in the block, leave
-//    a quarter of the records to merge (131071 tokens: 40.5 us, 41.6 us with eight heads).
+//    a quarter of the records to merge (131071 tokens: 38.0 us, 39.7 us with eight heads).
 template <int NT>
 void kv4_shape(int batch, int nh_kv, int n_cc, int64_t room, int grid, int* hg, int* ts, int* whole) {
     constexpr int W = kKv4Warps<NT>;
@@ -78,7 +80,7 @@ void kv4_shape(int batch, int nh_kv, int n_cc, int64_t room, int grid, int* hg, 
         if (h * t != W || nh_kv % h != 0 || segments(h) > grid) continue;
         if (steps(t) < steps(t0)) h0 = h, t0 = t;
     }
-    if (steps(t0) <= 2) *hg = h0, *ts = t0, *whole = 1;
+    if (steps(t0) <= 2 || (steps(t0) <= 4 && 5 * segments(h0) >= grid)) *hg = h0, *ts = t0, *whole = 1;
     else if (2 * segments(*hg) >= grid) *whole = steps(*ts) <= 8;
     else if (segments(*hg) <= 8 && *hg > 2 && nh_kv % 2 == 0) *hg = 2, *ts = W / 2;
 }
@@ -113,7 +115,7 @@ int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
     const auto kernel = p.page_shift >= 4 ? kv4_attn_kernel<NT, true> : kv4_attn_kernel<NT, false>;
     if (NT == 1) {
         DKV_CUDA(launch_overlapped(kernel, grid, kKv4Warps<NT> * 32, smem, st, p));
-    } else {                            // takes all registers of an SM: set up beside a merge that still runs, it loses (16 drafts: 41 us, 37 us)
+    } else {                            // takes all registers of an SM: set up beside a merge that still runs, it loses (16 drafts: 32.5 us, 32.0 us)
         kernel<<<grid, kKv4Warps<NT> * 32, smem, st>>>(p);
         DKV_CUDA(cudaGetLastError());
     }

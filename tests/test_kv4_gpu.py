@@ -238,6 +238,19 @@ def test_many_short_requests(columns):
     _check2(_widen(_case([40 + i % 90 for i in range(70)], 8, 8, 16, 1, 523), columns))
 
 
+@pytest.mark.parametrize("batch,longest,nh_q,nh_kv", [(64, 480, 8, 8), (8, 992, 16, 8), (20, 1000, 8, 8)])
+def test_several_steps_and_token_lanes_of_whole_segments(batch, longest, nh_q, nh_kv, columns):
+    c = _widen(_case([longest] + [(i * 131) % (longest + 1) for i in range(batch - 1)], nh_q, nh_kv, 16, 1, 524), columns)
+    _check(c, *_run(c))
+
+
+@pytest.mark.parametrize("batch", [31, 32, 33, 257])
+def test_batches_that_a_warp_or_a_block_scans(batch, columns):
+    c = _widen(_case([(i * 77) % 400 for i in range(batch)], 4, 4, 16, 1, 525 + batch), columns)
+    _check(c, *_run(c))
+    assert get_context(0).read_status() == 0
+
+
 def test_row_map_strides_and_2d_queries():
     c = _case([50, 0, 300, 17], 8, 2, 16, 1, 530)
     rows = [2, 0, 3]
