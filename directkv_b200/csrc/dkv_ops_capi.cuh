@@ -113,12 +113,7 @@ int launch_kv4_attn(dkv_context* ctx, Kv4AttnParams& p, cudaStream_t st) {
     p.by_seg = Kv4Div(p.n_hg * p.n_cc), p.by_cc = Kv4Div(p.n_cc), p.by_hg = Kv4Div(p.hg), p.by_grid = Kv4Div(grid);
     const size_t smem = kv4_smem<NT>(p.batch);
     const auto kernel = p.page_shift >= 4 ? kv4_attn_kernel<NT, true> : kv4_attn_kernel<NT, false>;
-    if (NT == 1) {
-        DKV_CUDA(launch_overlapped(kernel, grid, kKv4Warps<NT> * 32, smem, st, p));
-    } else {                            // takes all registers of an SM: set up beside a merge that still runs, it loses (16 drafts: 32.5 us, 32.0 us)
-        kernel<<<grid, kKv4Warps<NT> * 32, smem, st>>>(p);
-        DKV_CUDA(cudaGetLastError());
-    }
+    DKV_CUDA(launch_overlapped(kernel, grid, kKv4Warps<NT> * 32, smem, st, p));
     ctx->launches += 1;
     if (p.whole) return DKV_OK;
     const unsigned rows = static_cast<unsigned>(p.batch) * p.n_q * p.nh_q;
