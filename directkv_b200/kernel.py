@@ -751,7 +751,11 @@ def assign_pages(
         raise RuntimeError(f"n_tokens ({n_tokens}) must be 0..2^31-1")
     if slots is None and positions is None and seq_lens is None and cu_new is None:
         pad = -n_tokens & 3                                   # positions 16-byte aligned as well
-        slots, _, positions, seq_lens, cu_new = lens.new_empty(2 * n_tokens + pad + 2 * b + 1).split_with_sizes((n_tokens, pad, n_tokens, b, b + 1))
+        room = lens.new_empty_strided((2 * n_tokens + pad + 2 * b + 1,), (1,))
+        if pad:
+            slots, _, positions, seq_lens, cu_new = room.split_with_sizes((n_tokens, pad, n_tokens, b, b + 1))
+        else:
+            slots, positions, seq_lens, cu_new = room.split_with_sizes((n_tokens, n_tokens, b, b + 1))
     else:
         outs = []
         for t, n, name in ((slots, n_tokens, "slots"), (positions, n_tokens, "positions"), (seq_lens, b, "seq_lens"), (cu_new, b + 1, "cu_new")):
