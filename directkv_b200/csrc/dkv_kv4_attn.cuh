@@ -80,7 +80,6 @@ struct Kv4AttnParams {
     const uint8_t* k_scales;         // [n_slots, nh_kv, 8]
     const uint8_t* v_codes;
     const uint8_t* v_scales;
-    long long n_slots;
     int page_shift;
     int n_pages;                     // pages that begin inside the pool
     int batch, n_q, nh_q, nh_kv, group;
@@ -655,12 +654,12 @@ __global__ void __launch_bounds__(NW * 32) kv4_merge_kernel(const Kv4AttnParams 
     const long long goes_on = static_cast<long long>(p.hg) * C * kKv4RecFloats;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float own = kKv4Low, own_sum = 0.f;
-    for (int i0 = w; i0 < n; i0 += 4 * NW) {
+    for (int first_of_4 = w; first_of_4 < n; first_of_4 += 4 * NW) {
         float2 m[4];
         float4 v[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * NW;
+            const int i = first_of_4 + u * NW;
             m[u] = make_float2(kKv4Low, 0.f), v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (i >= n) continue;
             const float* r = rec0 + i * step + (i == 0 ? goes_on : 0);

@@ -245,7 +245,6 @@ int dkv_decode_kv4(dkv_context* ctx, const dkv_kv4_pool* pool, const dkv_decode_
     p.row_map = a->row_map;
     p.k_codes = static_cast<const uint8_t*>(pool->k_codes), p.v_codes = static_cast<const uint8_t*>(pool->v_codes);
     p.k_scales = static_cast<const uint8_t*>(pool->k_scales), p.v_scales = static_cast<const uint8_t*>(pool->v_scales);
-    p.n_slots = pool->n_slots;
     p.n_pages = static_cast<int>(pool->n_slots / pool->page_size);
     p.batch = a->batch, p.n_q = a->n_q, p.nh_q = a->nh_q, p.nh_kv = pool->nh_kv;
     p.group = a->nh_q / pool->nh_kv;
