@@ -348,7 +348,7 @@ int dkv_assign_pages(dkv_context* ctx, const dkv_pages_args* a, int32_t* slots, 
     DKV_ON_DEVICE(ctx);
     p.vector = aligned(slots, 16) && aligned(positions, 16);
     const int64_t want = (capacity + 4 * kPagesThreads - 1) / (4 * kPagesThreads);
-    const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, ctx->sm_count * 2)));
+    const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, ctx->sm_count)));
     DKV_CUDA(launch_overlapped(pages_kernel<false>, grid, kPagesThreads, 0, static_cast<cudaStream_t>(stream), p));
     ctx->launches += 1;
     return DKV_OK;
