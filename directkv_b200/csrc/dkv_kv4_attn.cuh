@@ -6,9 +6,12 @@
 // One pass over the rows with a running maximum and sum.  The (query token, head) pairs that share a KV head are the
 // columns of two warp-level products (m16n8k16, fp16 in, fp32 out) per 16 tokens:
 //     S [16 tokens x 8 columns] = K Q^T            O^T [128 dims x 8 columns] += V^T P^T
-// so a row is decoded once for all of them.  Nothing is lost on the way in: code * block scale is exact in fp16, and a
-// query row is scaled by a power of two that brings its largest value to 2^14 before it becomes fp16 (undone in the
-// fp32 scores).  P is rounded to fp16 (2^-11, against bf16's 2^-8); scores, maximum, sum and O are fp32.
+// so a row is decoded once for all of them.  code * block scale is exact in fp16.  A query row is scaled by a power of two
+// that brings its largest value to 2^14 before it becomes fp16 (undone in the fp32 scores): exact for values down to 2^-31 of the
+// largest, off by at most 2^-39 of it below.  P is rounded to fp16, scaled so that the largest one lies between 2^12 and 2^15: off by
+// 2^-11 of itself, or where it is less than 2^-26 of the largest by 2^-37 of that.  Without the scaling weights below 2^-25 of
+// the largest vanish from O, but not from the sum: with one strong token whose value row is zero the output loses whatever is
+// that far below.  Scores, maximum, sum and O are fp32.
 //
 // What bounds it is bytes, 144 per token and KV head, and close behind them the instructions that turn codes into fp16: 64
 // requests of 12000 to 20000 tokens, 32 query heads on 8, take 217 us (5.51 TB/s, 0.84 of the measured copy rate), copies
@@ -43,7 +46,9 @@ constexpr int kKv4MaxBatch = 4096;                       // of a call
 constexpr int kKv4LaunchBatch = 1024;                    // of a launch: what leaves room for the blocks that share an SM
 constexpr int kKv4RecFloats = 132;                       // O[128], m (log2 domain), l, 2 pad
 constexpr float kKv4Low = -3e38f;                        // the running maximum before the first token
-constexpr float kKv4Lag = 8.f;                           // the maximum follows once a score is 2^8 above it: P <= 2^8 in fp16
+// What P is relative to lies 2^12 below the running maximum, and follows once a score is 2^15 above it: P <= 2^15 in fp16, the
+// largest one 2^12 at least.
+constexpr float kKv4Lift = 12.f, kKv4Lag = 15.f;
 
 // Division of 0 .. 2^31 - 1 by a number that the host knows: with 2^(l-1) < d <= 2^l and m = ceil(2^(31+l) / d) < 2^32, the product
 // n m / 2^(31+l) is less than 1 / d above n / d.  A division by a variable is some 150 cycles of latency, and the way from a launch to
@@ -490,7 +495,7 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                            const float m2 = fmaxf(st.m[n][k], top);
+                            const float m2 = fmaxf(st.m[n][k], top - kKv4Lift);
                             const float f = m2 == st.m[n][k] ? 1.f : ex2_approx(st.m[n][k] - m2);
                             st.m[n][k] = m2;
                             st.l[n][k] *= f;
