@@ -590,6 +590,8 @@ def decode_kv4(
         _int32_1d(row_map, b, "row_map")
         if row_map.get_device() != dev:
             _elsewhere("row_map")
+        if rows == 0 < b:                                     # (to the library 0 rows mean an unknown number)
+            raise RuntimeError(f"page_table has no rows for {b} requests")
         row_ptr = row_map.data_ptr()
     elif rows < b:
         raise RuntimeError(f"page_table has {rows} rows for {b} requests")

@@ -173,3 +173,12 @@ def test_outputs_like_a_slice_are_contiguous():
         assert kernel._heads_stride(x, "x") > 0 and torch.empty_like(x).is_contiguous()
     flat = torch.zeros(6, 1280, dtype=BF)[:, 128:512]
     assert torch.empty_like(flat).is_contiguous()
+
+
+def test_decode_refuses_a_row_map_into_a_table_without_rows():
+    """The library takes 0 rows for an unknown number and would follow the row map out of the table."""
+    q, lens = torch.zeros(2, 4, 128, dtype=BF), _i32(2)
+    with pytest.raises(RuntimeError, match="no rows"):
+        kernel.decode_kv4(q, _pool(), lens, 1.0, _i32(0, 3), row_map=_i32(2))
+    with pytest.raises(RuntimeError, match="CUDA tensor"):                    # no request, nothing to look up: only the device is wrong
+        kernel.decode_kv4(q[:0], _pool(), lens[:0], 1.0, _i32(0, 3), row_map=_i32(0))
