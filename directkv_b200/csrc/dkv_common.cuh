@@ -204,7 +204,8 @@ __device__ __forceinline__ uint64_t ex2_poly_f32x2(uint64_t x) {
 
 // Launched with programmatic stream serialization, a kernel's blocks may be set up while the kernel before it ends.  The wait
 // comes before the first access to memory and returns when that kernel is complete and its stores are visible; the
-// trigger lets the kernel after it start its own set-up once every block has come this far.
+// trigger lets the kernel after it start its own set-up once every block has come this far.  What the kernel before
+// may write is read with plain loads: those of the read-only path (__ldg) are for data that nobody writes while the kernel runs.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
                 const int t = token0(step) + (WIDE ? (lane & 1) * 16 : lane);
                 int slot = -1;
                 if (step < n_tiles && t < len) {
-                    const int e = __ldg(table + (t >> p.page_shift));
+                    const int e = table[t >> p.page_shift];
                     if (static_cast<unsigned>(e) < static_cast<unsigned>(p.n_pages)) slot = (e << p.page_shift) + (t & page_mask);
                     else atomicOr(p.status, kStatusBadPage);
                 }
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kKv4Warps<NT> * 32, kKv4BlocksPerSm<NT>) kv4_a
                     const int j = p.by_group(col), h = kvh * p.group + (col - j * p.group);
                     const uint4* src = reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(b) * p.n_q + j) * p.q_stride + h * 128 + c * 32);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = __ldg(src + i);
+                    for (int i = 0; i < 4; ++i) v[i] = src[i];
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);

@@ -182,3 +182,15 @@ def test_decode_refuses_a_row_map_into_a_table_without_rows():
         kernel.decode_kv4(q, _pool(), lens, 1.0, _i32(0, 3), row_map=_i32(2))
     with pytest.raises(RuntimeError, match="CUDA tensor"):                    # no request, nothing to look up: only the device is wrong
         kernel.decode_kv4(q[:0], _pool(), lens[:0], 1.0, _i32(0, 3), row_map=_i32(0))
+
+
+def test_kernels_that_overlap_the_one_before_use_plain_loads():
+    """A kernel that begins with grid_wait() runs while the one before it still writes: read-only loads are not for such data."""
+    csrc = os.path.join(ROOT, "directkv_b200", "csrc")
+    seen = 0
+    for name in sorted(os.listdir(csrc)):
+        text = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, name)).read())
+        if "grid_wait();" in text:
+            seen += 1
+            assert "__ldg" not in text and ".nc" not in text and "__restrict__" not in text, name
+    assert seen >= 4

@@ -248,3 +248,41 @@ def test_decode_steps_over_a_four_bit_cache():
     assert get_context(0).read_status() == 0
     kernel.release_pages(table, lens, torch.zeros_like(lens), free, n_free, page)
     assert int(n_free) == 49 and sorted(free.cpu().tolist()) == list(range(1, 50))
+
+
+@pytest.mark.parametrize("n_q", [1, 3])
+def test_tables_and_queries_written_by_the_kernel_just_before(n_q):
+    """assign_pages and qk_norm_rope directly before the attention: it reads the table and the queries that they have just written."""
+    batch, nh_q, nh_kv, page, n = 40, 8, 2, 4, 60
+    g = torch.Generator().manual_seed(31)
+    pool = kernel.KV4Pool.empty(batch * 20 * page, nh_kv, page, DEV)
+    parts = []
+    for codes, scales in ((pool.k_codes, pool.k_scales), (pool.v_codes, pool.v_scales)):
+        c, s = ref.quantise(torch.randn(*codes.shape[:2], 128, generator=g).to(torch.bfloat16))
+        codes.copy_(c), scales.copy_(s)
+        parts.append((c, s))
+    cs = workloads.build_cos_sin(64, 10000.0).to(DEV)
+    new, zero = _i32([n] * batch), _i32([0] * batch)
+    pos = _i32([n - 1] * (batch * n_q))
+    out = torch.zeros(batch, n_q, nh_q, 128, dtype=torch.bfloat16, device=DEV)
+    for step in range(6):
+        order = torch.randperm(batch * 20, generator=g).to(torch.int32)
+        free, n_free, table = order.to(DEV), _i32([order.numel()]), torch.zeros(batch, 20, dtype=torch.int32, device=DEV)
+        x = torch.randn(batch * n_q, nh_q, 128, generator=g).to(torch.bfloat16).to(DEV)
+        q = torch.zeros_like(x)
+        torch.cuda.synchronize()
+        if step % 2:
+            kernel.qk_norm_rope(x, None, pos, cs, q_out=q)
+            _, _, lens, _ = kernel.assign_pages(table, zero, new, free, n_free, page, n * batch)
+        else:
+            _, _, lens, _ = kernel.assign_pages(table, zero, new, free, n_free, page, n * batch)
+            kernel.qk_norm_rope(x, None, pos, cs, q_out=q)
+        kernel.decode_kv4(q.view(batch, n_q, nh_q, 128), pool, lens, 128 ** -0.5, table, out=out)
+        torch.cuda.synchronize()
+        state = ref.Pages(torch.zeros(batch, 20, dtype=torch.int32), order, order.numel(), page)
+        slots = torch.tensor(state.assign(range(batch), [0] * batch, [n] * batch)[0]).view(batch, n)
+        for b in range(0, batch, 7):
+            k, v = (ref.values(c[slots[b]], s[slots[b]]) for c, s in parts)
+            o, _, e = ref.attend(q.view(batch, n_q, nh_q, 128)[b].cpu(), k, v, n, 128 ** -0.5)
+            assert ((out[b].cpu().double() - o).abs() <= e).all(), (step, b)
+    assert get_context(0).read_status() == 0
