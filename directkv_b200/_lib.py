@@ -237,6 +237,7 @@ SIGNATURES = {
     "dkv_decode_kv4": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "dkv_qk_norm_rope": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "dkv_assign_pages": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "dkv_assign_pages_fresh": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
     "dkv_release_pages": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "dkv_stream_copy": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
 }

@@ -175,8 +175,8 @@ __global__ void __launch_bounds__(kKv4RowThreads) kv4_store_kernel(const Kv4Rows
         uint32_t kw[8], vw[8];
         kv4_read16(p.k + tok * p.k_stride + u * 16, p.wide, kw);
         kv4_read16(p.v + tok * p.v_stride + u * 16, p.wide, vw);
-        if (slot < 0 || slot >= p.n_slots) {
-            if (u == 0) atomicOr(p.status, kStatusBadSlot);
+        if (slot < 0 || slot >= p.n_slots) {                // (-1: no token)
+            if (u == 0 && slot != -1) atomicOr(p.status, kStatusBadSlot);
             continue;
         }
         uint2 kc, vc;
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kKv4RowThreads) kv4_load_kernel(const Kv4RowsP
             kc = reinterpret_cast<const uint2*>(p.k_codes)[at];
             vc = reinterpret_cast<const uint2*>(p.v_codes)[at];
             ks = p.k_scales[at], vs = p.v_scales[at];
-        } else if (u == 0) {
+        } else if (u == 0 && slot != -1) {
             atomicOr(p.status, kStatusBadSlot);
         }
         const long long at = (tok * units + u) * 16;

@@ -339,12 +339,17 @@ static int pages_common(dkv_context* ctx, const dkv_pages_args* a, PagesParams* 
 
 int dkv_assign_pages(dkv_context* ctx, const dkv_pages_args* a, int32_t* slots, int32_t* positions, int64_t capacity, int32_t* seq_lens,
                      int32_t* cu_new, void* stream) {
+    return dkv_assign_pages_fresh(ctx, a, slots, positions, capacity, seq_lens, cu_new, 0, stream);
+}
+
+int dkv_assign_pages_fresh(dkv_context* ctx, const dkv_pages_args* a, int32_t* slots, int32_t* positions, int64_t capacity, int32_t* seq_lens,
+                           int32_t* cu_new, int fresh, void* stream) {
     PagesParams p{};
     int rc = pages_common(ctx, a, &p);
     if (rc != DKV_OK) return rc;
     DKV_REQUIRE(capacity >= 0 && capacity <= INT32_MAX && (capacity == 0 || slots != nullptr), "slots must hold 0..2^31-1 tokens");
     DKV_REQUIRE(cu_new != nullptr && (a->batch == 0 || seq_lens != nullptr), "seq_lens / cu_new must not be NULL");
-    p.slots = slots, p.positions = positions, p.capacity = capacity, p.seq_lens = seq_lens, p.cu_new = cu_new;
+    p.slots = slots, p.positions = positions, p.capacity = capacity, p.fresh = fresh, p.seq_lens = seq_lens, p.cu_new = cu_new;
     DKV_ON_DEVICE(ctx);
     p.vector = aligned(slots, 16) && aligned(positions, 16);
     const int64_t want = (capacity + 4 * kPagesThreads - 1) / (4 * kPagesThreads);

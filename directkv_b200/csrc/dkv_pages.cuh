@@ -3,7 +3,9 @@
 // The free pages are a stack in device memory: free_pages[0 .. n_free).  Request b (row r of the page table) has
 // a_b tokens on ceil(a_b / P) pages and gets n_b more.  Pages are taken in request order, then in page order, from the
 // top of the stack: the i-th page taken is free_pages[n_free - 1 - i].  The packed new tokens get their positions
-// a_b + j and their slots page * P + position % P.  Release puts the pages of the tokens [keep_b, len_b) back so that
+// a_b + j and their slots page * P + position % P.  Places behind the last new token (a captured call has room for the most
+// that it may get) hold no token: a slot there becomes -1, which store and load pass over, and a position 0; what is negative already
+// is left.  Without that a later step would store its padding rows into the slots of an earlier one.  Release puts the pages of the tokens [keep_b, len_b) back so that
 // a release of exactly what the last call took restores the stack.
 //
 // A call takes effect as a whole or not at all: too few pages, a row or length outside the table, or more tokens
@@ -35,6 +37,7 @@ struct PagesParams {
     int* slots;                      // assign only, [capacity]
     int* positions;                  // [capacity] or nullptr
     long long capacity;
+    int fresh;                       // bit 0: slots, bit 1: positions hold nothing yet
     int vector;                      // slots and positions are 16-byte aligned
     int* seq_lens;                   // [batch]: lens + more
     int* cu_new;                     // [batch + 1]
@@ -188,6 +191,10 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(const PagesParams 
                         if (p.positions != nullptr) p.positions[v0 + i] = where[i];
                     }
                 }
+            }
+            for (long long v = tok + me; v < p.capacity; v += stride) {
+                if ((p.fresh & 1) || p.slots[v] >= 0) p.slots[v] = -1;
+                if (p.positions != nullptr && ((p.fresh & 2) || p.positions[v] >= 0)) p.positions[v] = 0;
             }
         }
     } else if (ok) {

@@ -497,8 +497,9 @@ def _check_slots(slots: torch.Tensor) -> int:
 def store_kv4(pool: KV4Pool, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
     """Quantises row ``i`` of ``k`` / ``v`` ``[n, NH_kv, 128]`` (bf16, tokens may be strided) into slot ``slots[i]``.
 
-    Slots outside the pool are not written and reported in the status word, and so are infinities (stored as the largest
-    value) and not-a-numbers (stored as zero).  Slots must be distinct, save for a padding slot that nobody attends.
+    A slot of -1 stands for no token (``assign_pages`` gives it to the padding of a batch): its row is passed over.  Other slots
+    outside the pool are not written and reported in the status word, and so are infinities (stored as the largest value)
+    and not-a-numbers (stored as zero).  Slots must be distinct, save for a padding slot that nobody attends.
     """
     n = _check_slots(slots)
     want = (n, pool.nh_kv, HEAD_DIM)
@@ -519,7 +520,7 @@ def store_kv4(pool: KV4Pool, slots: torch.Tensor, k: torch.Tensor, v: torch.Tens
 
 def load_kv4(pool: KV4Pool, slots: torch.Tensor, k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None):
     """The values of ``slots`` as bf16 ``(k, v)``, each ``[n, NH_kv, 128]``; exact.  A slot outside the pool gives zeros and
-    is reported in the status word."""
+    is reported in the status word, but for -1 (no token)."""
     n = _check_slots(slots)
     dev = slots.get_device()
     if dev < 0:
@@ -743,14 +744,16 @@ def assign_pages(
     """Gives every request pages for its new tokens, on the GPU: no host copy of the lengths, capturable in a CUDA graph.
 
     Returns ``(slots [n_tokens], positions [n_tokens], seq_lens [B], cu_new [B + 1])``: slot and position of each new token
-    packed in request order, the lengths with the new tokens, and the packed offsets.  Entries behind the last token are
-    left as they were.  The call takes effect as a whole or not at all: when the pages run out, a length does not fit the
+    packed in request order, the lengths with the new tokens, and the packed offsets.  Behind the last token a slot becomes -1,
+    which ``store_kv4`` and ``load_kv4`` pass over, and a position 0 (given tensors: entries that are negative there are
+    left as they were).  The call takes effect as a whole or not at all: when the pages run out, a length does not fit the
     table or ``n_tokens``, or two requests with new tokens have one row, everything is left as it was, the slots are -1 and
     the status word says why.
     """
     dev, b, a = _pages_args(page_table, lens, new_lens, "new_lens", free_pages, n_free, page_size, rows)
     if not 0 <= n_tokens < 2 ** 31:
         raise RuntimeError(f"n_tokens ({n_tokens}) must be 0..2^31-1")
+    fresh = (slots is None) + 2 * (positions is None)
     if slots is None and positions is None and seq_lens is None and cu_new is None:
         pad = -n_tokens & 3                                   # positions 16-byte aligned as well
         room = lens.new_empty_strided((2 * n_tokens + pad + 2 * b + 1,), (1,))
@@ -770,7 +773,7 @@ def assign_pages(
             outs.append(t)
         slots, positions, seq_lens, cu_new = outs
     handle, stream = _call(dev)
-    rc = _lib.load().dkv_assign_pages(handle, a, slots.data_ptr(), positions.data_ptr(), n_tokens, seq_lens.data_ptr(), cu_new.data_ptr(), stream)
+    rc = _lib.load().dkv_assign_pages_fresh(handle, a, slots.data_ptr(), positions.data_ptr(), n_tokens, seq_lens.data_ptr(), cu_new.data_ptr(), fresh, stream)
     if rc:
         _lib.check(rc)
     return slots, positions, seq_lens, cu_new

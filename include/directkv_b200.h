@@ -360,13 +360,13 @@ typedef struct {
 int dkv_kv4_pool_resolve(dkv_context* ctx, dkv_kv4_pool* pool);
 
 /* The 4-bit counterpart of dkv_scatter_kv: row i of k / v ([n_tokens, nh_kv, 128] bf16 device, k_stride / v_stride
- * elements from token to token) is quantised into slot slots[i] (int32 or int64, device).  A slot outside the
- * pool is not written (DKV_STATUS_BAD_SLOT).  Two rows for one slot leave either of them or a mixture. */
+ * elements from token to token) is quantised into slot slots[i] (int32 or int64, device).  A slot of -1 stands for no token:
+ * the row is passed over.  Another slot outside the pool is not written either (DKV_STATUS_BAD_SLOT).  Two rows for one slot leave either of them or a mixture. */
 int dkv_kv4_store(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, int slots_int64, const void* k, int64_t k_stride,
                   const void* v, int64_t v_stride, int64_t n_tokens, void* stream);
 
 /* Reads slots back: k / v [n_tokens, nh_kv, 128] bf16 device, contiguous; exact (see the format).  A slot outside the
- * pool gives zeros (DKV_STATUS_BAD_SLOT). */
+ * pool gives zeros (DKV_STATUS_BAD_SLOT, but for -1: no token). */
 int dkv_kv4_load(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, int slots_int64, void* k, void* v, int64_t n_tokens,
                  void* stream);
 
@@ -436,8 +436,8 @@ int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* args, void* strea
  * Page tables and slot maps on the GPU.  The free pages are a stack, free_pages[0 .. *n_free) of room for free_cap.
  * dkv_assign_pages gives request b (row rows[b] of the table, or b) room for more[b] tokens behind its lens[b]: pages
  * come off the top of the stack in request order, then page order, and are entered in the table; slots and positions
- * [capacity] receive slot and position of every new token, packed in request order (entries behind the last one are
- * left as they were); seq_lens[b] = lens[b] + more[b] (may be lens itself); cu_new [batch + 1] is the packed offset
+ * [capacity] receive slot and position of every new token, packed in request order (behind the last one a slot becomes
+ * -1, no token, and a position 0; entries that are negative there are left as they were); seq_lens[b] = lens[b] + more[b] (may be lens itself); cu_new [batch + 1] is the packed offset
  * of every request.  dkv_release_pages puts the pages of the tokens [more[b], lens[b]) back on the stack - in the
  * opposite order, so that a release of exactly the last assignment restores it - and leaves the table's entries.
  * Requests that change nothing may repeat a row.  A call takes effect as a whole or not at all: a row, length or page beyond the
@@ -461,6 +461,10 @@ typedef struct {
 
 int dkv_assign_pages(dkv_context* ctx, const dkv_pages_args* args, int32_t* slots, int32_t* positions, int64_t capacity,
                      int32_t* seq_lens, int32_t* cu_new, void* stream);
+/* dkv_assign_pages into memory that holds nothing yet: with bit 0 of `fresh` every slot behind the last token becomes -1, with bit
+ * 1 every position 0. */
+int dkv_assign_pages_fresh(dkv_context* ctx, const dkv_pages_args* args, int32_t* slots, int32_t* positions, int64_t capacity,
+                           int32_t* seq_lens, int32_t* cu_new, int fresh, void* stream);
 int dkv_release_pages(dkv_context* ctx, const dkv_pages_args* args, void* stream);
 
 /* Measurement aid, not part of the drop-in surface (no counterpart in the reference): a device-side copy

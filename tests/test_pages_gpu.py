@@ -286,3 +286,62 @@ def test_tables_and_queries_written_by_the_kernel_just_before(n_q):
             o, _, e = ref.attend(q.view(batch, n_q, nh_q, 128)[b].cpu(), k, v, n, 128 ** -0.5)
             assert ((out[b].cpu().double() - o).abs() <= e).all(), (step, b)
     assert get_context(0).read_status() == 0
+
+
+@pytest.mark.parametrize("room", [3, 64, 5000])
+def test_places_behind_the_last_token_hold_no_slot(room):
+    """n_tokens may be more than the tokens there are.  What the call allocates, and what an earlier call left in the caller's
+    tensors, becomes no token: slot -1, position 0."""
+    rows, table, order, spare = _setup([5, 0], 16, 400, 400, 16)
+    t, free, n_free, lens = table.to(DEV), order.to(DEV), _i32([spare]), _i32([5, 0])
+    for junk in (7, -123456):                            # what the allocator hands out again
+        for n in (room, 2 * room + 5 + (-room & 3)):
+            torch.full((n,), junk, dtype=torch.int32, device=DEV)
+        got = kernel.assign_pages(t, lens, _i32([2, 1]), free, n_free, 16, room, rows=_i32(rows))
+        assert (got[0][:3] >= 0).all() and got[1][:3].tolist() == [5, 6, 0] and (got[0][3:] == -1).all() and (got[1][3:] == 0).all()
+        kernel.release_pages(t, got[2], lens, free, n_free, 16, rows=_i32(rows))
+    slots, positions = _i32([9] * room), _i32([4] * room)
+    kernel.assign_pages(t, lens, _i32([1, 0]), free, n_free, 16, room, rows=_i32(rows), slots=slots)
+    got = kernel.assign_pages(t, _i32([6, 0]), _i32([0, 1]), free, n_free, 16, room, rows=_i32(rows), slots=slots, positions=positions)
+    assert got[0] is slots and slots[0] >= 0 and (slots[1:] == -1).all() and (positions == 0).all()
+    assert get_context(0).read_status() == 0
+
+
+def test_a_replay_with_fewer_tokens_than_the_graph_has_room_for_changes_no_other_row():
+    """A captured step of up to 8 tokens: bookkeeping, rotation, store, load.  Replayed with fewer it stores those alone."""
+    nh, page, room = 2, 4, 8
+    g = torch.Generator().manual_seed(33)
+    cs = workloads.build_cos_sin(64, 10000.0).to(DEV)
+    pool = kernel.KV4Pool.empty(80, nh, page, DEV)
+    table, free, n_free = torch.zeros(3, 6, dtype=torch.int32, device=DEV), torch.arange(1, 19, dtype=torch.int32, device=DEV), _i32([18])
+    state = ref.Pages(table.cpu(), free.cpu(), 18, page)
+    lens, new, cu = _i32([0] * 3), _i32([0] * 3), _i32([0] * 4)
+    slots, pos = _i32([-1] * room), _i32([0] * room)
+    k, v = (torch.zeros(room, nh, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    back = [torch.zeros_like(k) for _ in range(2)]
+
+    def step():
+        kernel.assign_pages(table, lens, new, free, n_free, page, room, slots=slots, positions=pos, seq_lens=lens, cu_new=cu)
+        kernel.qk_norm_rope(None, k, pos, cs, k_out=k)
+        kernel.store_kv4(pool, slots, k, v)
+        kernel.load_kv4(pool, slots, *back)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    want = torch.zeros(80, nh, 128, dtype=torch.float64)
+    host = [0] * 3
+    for more in ([4, 3, 1], [1, 0, 1], [0, 0, 0], [0, 5, 0], [1, 1, 1]):
+        rows = [torch.randn(room, nh, 128, generator=g).to(torch.bfloat16) for _ in range(2)]
+        k.copy_(rows[0]), v.copy_(rows[1]), new.copy_(torch.tensor(more, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        at, where, host, _ = state.assign(range(3), host, more)
+        n = sum(more)
+        assert slots.tolist() == at + [-1] * (room - n) and pos.tolist() == where + [0] * (room - n)
+        want[at] = ref.values(*ref.quantise(v.cpu()[:n]))
+        got = kernel.load_kv4(pool, torch.arange(80, dtype=torch.int32, device=DEV))[1]
+        assert torch.equal(got.cpu().double(), want)
+        assert torch.equal(back[1].cpu().double()[:n], want[at]) and not back[1][n:].any()
+    assert get_context(0).read_status() == 0
