@@ -153,6 +153,7 @@ class DirectKVTokenToKVPool(KVCache):
         return self.head_num * self.head_dim
 
     # ---- host-side block moves (directkv/directkv_pool.py:230-257) ---------------------
+    # Rows of both pools may still be written by kernels (set_kv_buffer of device tensors): the moves wait for them.
     def move_kv_cache(self, tgt_loc: torch.Tensor, src_loc: torch.Tensor):
         self.synchronize()
         tgt, src = tgt_loc.cpu().long(), src_loc.cpu().long()
@@ -164,6 +165,8 @@ class DirectKVTokenToKVPool(KVCache):
         return (x if isinstance(x, torch.Tensor) else torch.as_tensor(x)).cpu().long()
 
     def load_from_host_per_layer(self, host_pool, host_indices, device_indices, layer_id, io_backend):
+        self.synchronize()
+        host_pool.synchronize()
         src, dst = self._as_index(host_indices), self._as_index(device_indices)
         li, h_li = self._li(layer_id), layer_id - host_pool.start_layer
         self.k_buffer[li][dst] = host_pool.k_buffer[h_li][src]
@@ -171,6 +174,7 @@ class DirectKVTokenToKVPool(KVCache):
 
     def backup_to_host_all_layer(self, host_pool, host_indices, device_indices, io_backend):
         self.synchronize()
+        host_pool.synchronize()
         h_idx, d_idx = self._as_index(host_indices), self._as_index(device_indices)
         for li in range(len(self.k_buffer)):
             h_li = self.start_layer + li - host_pool.start_layer

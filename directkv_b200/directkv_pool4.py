@@ -108,10 +108,12 @@ class DirectKV4BitTokenToKVPool(DirectKVTokenToKVPool):
 
     def load_from_host_per_layer(self, host_pool, host_indices, device_indices, layer_id, io_backend):
         self.synchronize()
+        host_pool.synchronize()
         self._move(self.layer_pool(layer_id), self._as_index(device_indices), host_pool.layer_pool(layer_id), self._as_index(host_indices))
 
     def backup_to_host_all_layer(self, host_pool, host_indices, device_indices, io_backend):
         self.synchronize()
+        host_pool.synchronize()
         h_idx, d_idx = self._as_index(host_indices), self._as_index(device_indices)
         for li in range(len(self._layers)):
             lid = self.start_layer + li

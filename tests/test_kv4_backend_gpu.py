@@ -145,3 +145,24 @@ def test_pool_moves_keep_the_bytes():
         dev.set_kv_buffer(None, loc, k, v, k_scale=2.0, layer_id_override=0)
     with pytest.raises(NotImplementedError, match="4 bits"):
         dev.get_key_buffer(0)
+
+
+@pytest.mark.parametrize("name", ["DirectKV4BitTokenToKVPool", "DirectKVTokenToKVPool"])
+def test_a_fresh_pool_loads_rows_that_the_gpu_has_just_stored(name):
+    make = lambda: getattr(directkv_b200, name)(size=127, page_size=1, dtype=torch.bfloat16, head_num=4, head_dim=128, layer_num=1,  # noqa: E731
+                                                start_layer=0, end_layer=0)
+    host, fresh = make(), make()
+    g = torch.Generator().manual_seed(6)
+    k, v = (torch.randn(64, 4, 128, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    loc, busy = torch.arange(64, device=DEV), torch.randn(4096, 4096, device=DEV)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        busy = busy @ busy * 1e-3                         # the store is still to come when the copy is asked for
+    host.set_kv_buffer(None, loc, k, v, layer_id_override=0)
+    fresh.load_from_host_per_layer(host, list(range(64)), list(range(30, 94)), 0, None)
+    if name == "DirectKV4BitTokenToKVPool":
+        got = fresh.load_rows(0, loc + 30)
+        want = [ref.values(*ref.quantise(x.cpu())) for x in (k, v)]
+        assert all(torch.equal(a.cpu().double(), b) for a, b in zip(got, want))
+    else:
+        assert torch.equal(fresh.k_buffer[0][30:94], k.cpu()) and torch.equal(fresh.v_buffer[0][30:94], v.cpu())

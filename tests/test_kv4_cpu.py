@@ -194,3 +194,24 @@ def test_kernels_that_overlap_the_one_before_use_plain_loads():
             seen += 1
             assert "__ldg" not in text and ".nc" not in text and "__restrict__" not in text, name
     assert seen >= 4
+
+
+@pytest.mark.parametrize("name", ["DirectKV4BitTokenToKVPool", "DirectKVTokenToKVPool"])
+def test_moves_between_pools_wait_for_the_stores_of_both(name, monkeypatch):
+    """set_kv_buffer of device tensors returns before the rows are written: the host copies afterwards, from either pool's side."""
+    import directkv_b200
+
+    waited = []
+    monkeypatch.setattr(torch.cuda, "synchronize", waited.append)
+    make = lambda: getattr(directkv_b200, name)(size=7, page_size=1, dtype=BF, head_num=1, head_dim=128, layer_num=1, start_layer=0, end_layer=0)  # noqa: E731
+    for stored in ("one", "other", "both"):
+        here, there = make(), make()
+        if stored != "other":
+            here._compute_device = torch.device("cuda", 1)
+        if stored != "one":
+            there._compute_device = torch.device("cuda", 2)
+        want = {"one": [1], "other": [2], "both": [1, 2]}[stored]
+        for move in (lambda: here.load_from_host_per_layer(there, [1, 2], [3, 4], 0, None), lambda: here.backup_to_host_all_layer(there, [1, 2], [3, 4], None)):
+            waited.clear()
+            move()
+            assert sorted(d.index for d in waited) == want, (stored, waited)
