@@ -40,6 +40,7 @@ logger = logging.getLogger(__name__)
 
 _TILE = 64                       # directkv/directkv_backend.py:42
 _TOKEN_POOL_LAYER_BASE = 1 << 20  # engine layer ids of the token-pool registrations
+_LOADED_ROWS_LAYER_BASE = 1 << 21  # and of rows that were brought back to bf16 for one call
 
 
 def _pad64(n: int) -> int:
@@ -428,7 +429,7 @@ class DirectKVBackend(AttentionBackend):
         pool = forward_batch.token_to_kv_pool
         pool.set_kv_buffer(layer, forward_batch.out_cache_loc, k, v)
         four_bits = isinstance(pool, DirectKV4BitTokenToKVPool)
-        eng = _TOKEN_POOL_LAYER_BASE + layer.layer_id if four_bits else self._token_layer(layer, forward_batch)
+        eng = None if four_bits else self._token_layer(layer, forward_batch)
         ext = meta.extend_seq_lens_cpu or [meta.seq_lens_cpu[i] for i in range(bs)]
         pre = meta.extend_prefix_lens_cpu or [0] * bs
         table = forward_batch.req_to_token_pool.req_to_token
@@ -455,7 +456,7 @@ class DirectKVBackend(AttentionBackend):
             q_long = q if whole else torch.cat([q[o:o + n] for o, n in long_idx])
             q_long = q_long.reshape(-1, nh_q, d).contiguous()
             if four_bits:
-                o_long = self._extend_loaded_rows(eng, pool, layer, q_long, long_req, table).view(-1, nh_q * d)
+                o_long = self._extend_loaded_rows(pool, layer, q_long, long_req, table).view(-1, nh_q * d)
             else:
                 o_long = kernel.extend_ragged(eng, None, q_long, [r[0] for r in long_req],
                                               [r[1] for r in long_req], [r[2] for r in long_req], float(layer.scaling), True,
@@ -486,7 +487,7 @@ class DirectKVBackend(AttentionBackend):
                 out = attend(q2.contiguous())
         return out
 
-    def _extend_loaded_rows(self, eng: int, pool, layer, q_long: torch.Tensor, long_req, table: torch.Tensor) -> torch.Tensor:
+    def _extend_loaded_rows(self, pool, layer, q_long: torch.Tensor, long_req, table: torch.Tensor) -> torch.Tensor:
         """Long prompts over a 4-bit pool: the requests' rows come back to bf16 in HBM once, and the tensor-core extend
         kernel attends them there."""
         most = max(n_new + n_pre for n_new, n_pre, _ in long_req)
@@ -495,6 +496,7 @@ class DirectKVBackend(AttentionBackend):
         for i, (n_new, n_pre, rid) in enumerate(long_req):
             n = n_new + n_pre
             pool.load_rows(layer.layer_id, table[rid, :n], k_rows[i, :n], v_rows[i, :n])
+        eng = _LOADED_ROWS_LAYER_BASE + layer.layer_id
         kernel.register_layer(eng, k_rows, v_rows, page_size=1, row_stride=most, device=self._device_index())
         out = kernel.extend_ragged(eng, None, q_long, [r[0] for r in long_req], [r[1] for r in long_req], list(range(len(long_req))),
                                    float(layer.scaling), True)
