@@ -498,7 +498,8 @@ class DirectKVBackend(AttentionBackend):
             pool.load_rows(layer.layer_id, table[rid, :n], k_rows[i, :n], v_rows[i, :n])
         eng = _LOADED_ROWS_LAYER_BASE + layer.layer_id
         kernel.register_layer(eng, k_rows, v_rows, page_size=1, row_stride=most, device=self._device_index())
-        out = kernel.extend_ragged(eng, None, q_long, [r[0] for r in long_req], [r[1] for r in long_req], list(range(len(long_req))),
-                                   float(layer.scaling), True)
-        kernel.unregister_layer(eng, device=self._device_index())
-        return out
+        try:
+            return kernel.extend_ragged(eng, None, q_long, [r[0] for r in long_req], [r[1] for r in long_req], list(range(len(long_req))),
+                                        float(layer.scaling), True)
+        finally:
+            kernel.unregister_layer(eng, device=self._device_index())

@@ -101,3 +101,11 @@ def test_a_long_prompt_leaves_another_pools_registration_alone(monkeypatch):
     assert engine.layers == before                          # the rows of one call are gone, the bf16 pool is as it was
     _extend(be, r2t, layer, wide, [(1, 40, 0)])             # fails where its layer was taken away
     assert [c[1] for c in engine.calls if c[0] == "extend"][0::2] == [next(iter(before))] * 2
+
+
+def test_a_long_prompt_that_fails_leaves_nothing_registered(monkeypatch):
+    engine, be, r2t, layer = _setup(monkeypatch)
+    engine.fail = True
+    with pytest.raises(RuntimeError, match="no room"):
+        _extend(be, r2t, layer, _pool(FourBits), [(1, 40, 0)])
+    assert not engine.layers
