@@ -47,6 +47,22 @@ def _pad64(n: int) -> int:
     return -(-int(n) // _TILE) * _TILE
 
 
+def _groups_of_like_length(lengths: List[int]) -> List[List[int]]:
+    """Indexes of requests whose rows are held side by side, padded to the longest of a group: all of them while padding takes no more
+    room than the rows, else groups whose longest is at most twice the shortest.  The rows held at a time are at most twice those there
+    are (one request of 131072 tokens beside 31 of 500, 8 KV heads: 0.5 GB, 17 GB in one group)."""
+    if max(lengths) * len(lengths) <= 2 * sum(lengths):
+        return [list(range(len(lengths)))]
+    groups: List[List[int]] = []
+    longest = 0
+    for i in sorted(range(len(lengths)), key=lambda i: -lengths[i]):
+        if not groups or 2 * lengths[i] < longest:
+            groups.append([])
+            longest = lengths[i]
+        groups[-1].append(i)
+    return [sorted(g) for g in groups]
+
+
 @dataclass
 class _FwdMeta:
     """Host copies made once per step (directkv/directkv_backend.py:52-57) plus their device twins."""
@@ -490,16 +506,33 @@ class DirectKVBackend(AttentionBackend):
     def _extend_loaded_rows(self, pool, layer, q_long: torch.Tensor, long_req, table: torch.Tensor) -> torch.Tensor:
         """Long prompts over a 4-bit pool: the requests' rows come back to bf16 in HBM once, and the tensor-core extend
         kernel attends them there."""
-        most = max(n_new + n_pre for n_new, n_pre, _ in long_req)
-        shape = (len(long_req), most, self.num_kv_heads, self.head_dim)
-        k_rows, v_rows = (torch.empty(shape, dtype=torch.bfloat16, device=q_long.device) for _ in range(2))
-        for i, (n_new, n_pre, rid) in enumerate(long_req):
+        groups = _groups_of_like_length([n_new + n_pre for n_new, n_pre, _ in long_req])
+        if len(groups) == 1:
+            return self._extend_loaded_group(pool, layer, q_long, long_req, table)
+        first = [0]
+        for n_new, _, _ in long_req:
+            first.append(first[-1] + n_new)
+        out = torch.empty_like(q_long)
+        for group in groups:
+            part = self._extend_loaded_group(pool, layer, torch.cat([q_long[first[i]:first[i + 1]] for i in group]), [long_req[i] for i in group], table)
+            pos = 0
+            for i in group:
+                n_new = long_req[i][0]
+                out[first[i]:first[i + 1]] = part[pos:pos + n_new]
+                pos += n_new
+        return out
+
+    def _extend_loaded_group(self, pool, layer, q: torch.Tensor, requests, table: torch.Tensor) -> torch.Tensor:
+        most = max(n_new + n_pre for n_new, n_pre, _ in requests)
+        shape = (len(requests), most, self.num_kv_heads, self.head_dim)
+        k_rows, v_rows = (torch.empty(shape, dtype=torch.bfloat16, device=q.device) for _ in range(2))
+        for i, (n_new, n_pre, rid) in enumerate(requests):
             n = n_new + n_pre
             pool.load_rows(layer.layer_id, table[rid, :n], k_rows[i, :n], v_rows[i, :n])
         eng = _LOADED_ROWS_LAYER_BASE + layer.layer_id
         kernel.register_layer(eng, k_rows, v_rows, page_size=1, row_stride=most, device=self._device_index())
         try:
-            return kernel.extend_ragged(eng, None, q_long, [r[0] for r in long_req], [r[1] for r in long_req], list(range(len(long_req))),
+            return kernel.extend_ragged(eng, None, q, [r[0] for r in requests], [r[1] for r in requests], list(range(len(requests))),
                                         float(layer.scaling), True)
         finally:
             kernel.unregister_layer(eng, device=self._device_index())

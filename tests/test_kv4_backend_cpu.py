@@ -109,3 +109,28 @@ def test_a_long_prompt_that_fails_leaves_nothing_registered(monkeypatch):
     with pytest.raises(RuntimeError, match="no room"):
         _extend(be, r2t, layer, _pool(FourBits), [(1, 40, 0)])
     assert not engine.layers
+
+
+def test_long_prompts_hold_at_most_twice_their_rows_in_bf16(monkeypatch):
+    """One long request beside short ones: nobody is padded to its length, and every request gets its own answer."""
+    engine, be, r2t, layer = _setup(monkeypatch)
+    plan = [(1, 40, 20), (2, 50, 3000), (3, 32, 0), (4, 33, 0), (5, 64, 100), (6, 40, 0)]
+    for rid, e, p in plan:
+        r2t.req_to_token[rid, :p + e] = 100 * rid
+    n = sum(e for _, e, _ in plan)
+    q = torch.randn(n, NH_Q * D, generator=torch.Generator().manual_seed(1)).to(BF)
+    out = _extend(be, r2t, layer, _pool(FourBits), plan, q=q)
+    total = sum(e + p for _, e, p in plan)
+    assert all(c[4] <= 2 * 2 * total * NH_KV * D for c in engine.calls), [c[4] for c in engine.calls]
+    assert sorted(x for c in engine.calls for x in c[2]) == sorted(e for _, e, _ in plan)
+    at = 0
+    for rid, e, p in plan:
+        of = torch.full((p + e, NH_KV, D), 100 * rid / 2 ** 20).to(BF).float().sum()
+        want = (q[at:at + e].float() + of).to(BF)
+        assert torch.equal(out[at:at + e], want), rid
+        at += e
+    assert not engine.layers
+    # like lengths stay one call
+    engine.calls.clear()
+    _extend(be, r2t, layer, _pool(FourBits), [(1, 40, 20), (2, 50, 60), (3, 32, 0)])
+    assert len(engine.calls) == 1

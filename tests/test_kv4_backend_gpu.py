@@ -166,3 +166,50 @@ def test_a_fresh_pool_loads_rows_that_the_gpu_has_just_stored(name):
         assert all(torch.equal(a.cpu().double(), b) for a, b in zip(got, want))
     else:
         assert torch.equal(fresh.k_buffer[0][30:94], k.cpu()) and torch.equal(fresh.v_buffer[0][30:94], v.cpu())
+
+
+def test_long_prompts_of_unlike_lengths_are_not_padded_to_the_longest():
+    """One prompt of 3000 tokens beside 12 short ones: what a call holds on the device stays near the rows themselves, and every request
+    gets its own answer."""
+    torch.manual_seed(0)
+    ctx_len, n_req = 3000, 13
+    model = FakeModel(LAYERS, H, NH_Q, NH_KV, None, ctx_len).to(DEV)
+    runner = make_runner(model, H, NH_Q, NH_KV, LAYERS, DEV, max_reqs=n_req, context_len=ctx_len)
+    be = directkv_b200.DirectKVBackend(runner)
+    pool = directkv_b200.DirectKV4BitTokenToKVPool(size=5000, page_size=1, dtype=torch.bfloat16, head_num=NH_KV, head_dim=D, layer_num=LAYERS,
+                                                   start_layer=0, end_layer=LAYERS - 1, location="device")
+    lens = [40 + 5 * i for i in range(n_req)]
+    lens[4] = ctx_len
+    perm, at = (torch.randperm(5000, generator=torch.Generator().manual_seed(3)) + 1).int(), 0
+    r2t = runner.req_to_token_pool
+    for rid, n in enumerate(lens):
+        r2t.req_to_token[rid, :n] = perm[at:at + n].to(DEV)
+        at += n
+    g = torch.Generator().manual_seed(12)
+    n = sum(lens)
+    q, k, v = _rows(g, n, NH_Q), _rows(g, n, NH_KV), _rows(g, n, NH_KV)
+    loc = torch.cat([r2t.req_to_token[rid, :m] for rid, m in enumerate(lens)])
+    fb = make_batch(EXTEND, lens, list(range(n_req)), DEV, extend_lens=lens, prefix_lens=[0] * n_req, token_pool=pool, req_to_token_pool=r2t, out_cache_loc=loc)
+    be.init_forward_metadata(fb)
+    qd, kd, vd = (x.to(DEV) for x in (q, k, v))
+    for _ in range(2):                                    # (the first call sizes the library's own scratch)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = be.forward_extend(qd, kd, vd, model.layers[1].attn, fb)
+        torch.cuda.synchronize()
+    row = NH_KV * D * 2
+    queries = 4 * n * NH_Q * D * 2                        # out, its parts and gathered queries
+    assert torch.cuda.max_memory_allocated() - before <= 2 * (2 * n * row) + queries + (1 << 20)
+    ref_kv, at = Mirror(), 0
+    for rid, m in enumerate(lens):
+        if m < 200:
+            ref_kv.add(rid, k[at:at + m], v[at:at + m])
+            ref_kv.check(rid, q[at:at + m], out[at:at + m], extend=True)
+        else:                                             # the last rows of the long one
+            kk, vv = (ref.values(*ref.quantise(x[at:at + m].view(-1, NH_KV, D))) for x in (k, v))
+            o, _, bound = ref.attend(q[at + m - 9:at + m].view(-1, NH_Q, D), kk, vv, m, D ** -0.5)
+            bound = bound + 2 * 2.0 ** -8 * vv.abs().amax(0).repeat_interleave(NH_Q // NH_KV, 0)
+            assert ((out[at + m - 9:at + m].cpu().double().view(o.shape) - o).abs() <= bound).all()
+        at += m
+    assert get_context(0).read_status() == 0
