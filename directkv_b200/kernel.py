@@ -381,7 +381,6 @@ def stream_copy(dst: torch.Tensor, src: torch.Tensor) -> None:
 # contiguous tensor is recognised by one question.
 KV4_BLOCK = 16          # consecutive dimensions that share a scale
 _BF16, _I32, _I64, _F32 = torch.bfloat16, torch.int32, torch.int64, torch.float32
-_protos = {}            # device -> an empty bf16 tensor there, to allocate like
 _pack_decode_kv4 = struct.Struct("@iiiPqPqPPqiiPfP").pack     # _lib.DecodeKv4Args
 _pack_qk_norm = struct.Struct("@qiiPqPqPqPqPPiiiiPiPif").pack  # _lib.QkNormArgs
 _pack_pages = struct.Struct("@PqiiPPPiiPiP").pack              # _lib.PagesArgs
@@ -527,11 +526,8 @@ def load_kv4(pool: KV4Pool, slots: torch.Tensor, k_out: Optional[torch.Tensor] =
         _elsewhere("slots")
     shape = (n, pool.nh_kv, HEAD_DIM)
     if k_out is None and v_out is None:
-        proto = _protos.get(dev)
-        if proto is None:
-            proto = _protos[dev] = torch.empty(0, dtype=_BF16, device=slots.device)
-        strides = (pool.nh_kv * HEAD_DIM, HEAD_DIM, 1)
-        k_out, v_out = proto.new_empty_strided(shape, strides), proto.new_empty_strided(shape, strides)
+        k_out = slots.new_empty_strided(shape, (pool.nh_kv * HEAD_DIM, HEAD_DIM, 1), dtype=_BF16)
+        v_out = torch.empty_like(k_out)
     if k_out is None:
         k_out = torch.empty(shape, dtype=_BF16, device=slots.device)
     elif k_out.dtype is not _BF16 or k_out.shape != shape or not k_out.is_contiguous() or k_out.get_device() != dev:

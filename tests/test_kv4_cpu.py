@@ -215,3 +215,14 @@ def test_moves_between_pools_wait_for_the_stores_of_both(name, monkeypatch):
             waited.clear()
             move()
             assert sorted(d.index for d in waited) == want, (stored, waited)
+
+
+def test_calls_keep_no_tensor_between_them():
+    """A call under FakeTensorMode fails, and nothing of it may be left for the calls that follow."""
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+
+    pool = _pool()
+    with FakeTensorMode(), pytest.raises(RuntimeError):
+        kernel.load_kv4(pool, torch.empty(3, dtype=torch.int32, device="cuda"))
+    kept = [x for value in vars(kernel).values() for x in (value.values() if isinstance(value, dict) and value is not vars(kernel) else [value])]
+    assert not [x for x in kept if isinstance(x, (FakeTensor, torch.Tensor))]
