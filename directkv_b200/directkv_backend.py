@@ -18,6 +18,8 @@ What is different underneath
   * When the layer's hidden states were not captured (no hook fired) the step runs over SGLang's
     token pool with the K/V SGLang computed - the data flow of the reference's
     ``_sdpa_decode_manual`` / ``_sdpa_extend_manual`` (:835-891) - still on the engine.
+  * A token pool held in 4 bits (``DirectKV4BitTokenToKVPool``) is the cache whether or not hidden states were
+    captured: every step stores to it and attends it, and no request pool is allocated beside it.
 """
 
 from __future__ import annotations
@@ -128,6 +130,7 @@ class DirectKVBackend(AttentionBackend):
         self._cg_seq_lens: Optional[torch.Tensor] = None
         self._cg_rows: Optional[torch.Tensor] = None
         self._cg_req: Optional[torch.Tensor] = None          # rows of req_to_token, for the token-pool path
+        self._four_bit_graphs: set = set()                   # batch sizes captured over a token pool in 4 bits
 
     # ------------------------------------------------------------------ checks
     def _check_args(self, runner) -> None:
@@ -237,6 +240,16 @@ class DirectKVBackend(AttentionBackend):
             return torch.cat([fq.cos(), fq.sin()], dim=-1).contiguous()
         return None
 
+    # ------------------------------------------------------------------ token pool
+    def _token_pool(self, forward_batch=None):
+        """The batch's token pool, or the runner's where the batch names none."""
+        pool = getattr(forward_batch, "token_to_kv_pool", None)
+        return pool if pool is not None else getattr(self._model_runner, "token_to_kv_pool", None)
+
+    def _in_four_bits(self, forward_batch=None) -> bool:
+        """Whether the cache is a token pool in 4 bits.  Requests have no rows in the request pool then."""
+        return isinstance(self._token_pool(forward_batch), DirectKV4BitTokenToKVPool)
+
     # ------------------------------------------------------------------ per-step metadata
     def _sync_rows(self, req_ids: List[int], free_absent: bool = True) -> None:
         """Row lifecycle.  In a DECODE batch every running request is present, so a request that is
@@ -276,17 +289,19 @@ class DirectKVBackend(AttentionBackend):
         sl_host = getattr(forward_batch, "seq_lens_cpu", None)
         seq_lens_cpu = sl_host.tolist() if sl_host is not None else forward_batch.seq_lens.cpu().tolist()
         req_ids_cpu = forward_batch.req_pool_indices.cpu().tolist()
-        self._ensure_pool()
-        self._sync_rows(req_ids_cpu, free_absent=forward_batch.forward_mode.is_decode())
-        for rid, n in zip(req_ids_cpu, seq_lens_cpu):
-            self._last_len[rid] = int(n)
+        four_bits = self._in_four_bits(forward_batch)
+        if not four_bits:
+            self._ensure_pool()
+            self._sync_rows(req_ids_cpu, free_absent=forward_batch.forward_mode.is_decode())
+            for rid, n in zip(req_ids_cpu, seq_lens_cpu):
+                self._last_len[rid] = int(n)
         self._fwd_meta = _FwdMeta(
             seq_lens_cpu=seq_lens_cpu,
             req_pool_indices_cpu=req_ids_cpu,
             extend_seq_lens_cpu=getattr(forward_batch, "extend_seq_lens_cpu", None),
             extend_prefix_lens_cpu=getattr(forward_batch, "extend_prefix_lens_cpu", None),
             seq_lens_dev=forward_batch.seq_lens.to(device=self.device, dtype=torch.int32),
-            rows_dev=self._pool.row_table(req_ids_cpu, self.device),
+            rows_dev=None if four_bits else self._pool.row_table(req_ids_cpu, self.device),
             req_idx_dev=forward_batch.req_pool_indices.to(device=self.device, dtype=torch.int32),
         )
 
@@ -294,7 +309,8 @@ class DirectKVBackend(AttentionBackend):
     def init_cuda_graph_state(self, max_bs: int, max_num_tokens: int) -> None:
         if not self._hooks_ready:
             self._setup_hooks()
-        self._ensure_pool()
+        if not self._in_four_bits():
+            self._ensure_pool()
         self._cg_max_bs = max_bs
         self._cg_seq_lens = torch.ones(max_bs, dtype=torch.int32, device=self.device)
         self._cg_rows = torch.zeros(max_bs, dtype=torch.int32, device=self.device)
@@ -325,6 +341,14 @@ class DirectKVBackend(AttentionBackend):
         they get the pool's spare row and length 1, so what the graph stores for them (the in-place write of
         the "new token") reaches no request's row, and they keep no row of their own."""
         rid_list = req_pool_indices[:bs].cpu().tolist()
+        # A captured batch runs over the runner's pool until forward_decode has seen another, a replayed one over what it was captured with.
+        if self._in_four_bits() if n_real is not None else bs in self._four_bit_graphs:
+            # No rows to keep apart: what a padded entry stores goes to its out_cache_loc, what it attends is nobody's.
+            self._cg_req[:bs].copy_(req_pool_indices[:bs])
+            self._fwd_meta = _FwdMeta(
+                seq_lens_cpu=list(seq_lens_cpu[:bs]), req_pool_indices_cpu=rid_list, extend_seq_lens_cpu=None, extend_prefix_lens_cpu=None,
+                seq_lens_dev=self._cg_seq_lens[:bs], req_idx_dev=self._cg_req[:bs], graph=True)
+            return
         self._ensure_pool()
         if n_real is None:
             n_real = self._count_real(rid_list, seq_lens_cpu)
@@ -368,7 +392,10 @@ class DirectKVBackend(AttentionBackend):
             return torch.zeros(bs, self.num_q_heads * self.head_dim, dtype=q.dtype, device=self.device)
         x = self._hidden.pop(lid, None)
         q2 = q.reshape(bs, self.num_q_heads * self.head_dim).contiguous()
-        if x is None or lid not in self._registered:
+        four_bits = self._in_four_bits(forward_batch)
+        if meta.graph:
+            (self._four_bit_graphs.add if four_bits else self._four_bit_graphs.discard)(len(meta.seq_lens_cpu))
+        if x is None or lid not in self._registered or four_bits:
             return self._decode_token_pool(q2, k, v, layer, forward_batch)
         x2 = x.reshape(bs, self.hidden_size).contiguous()
         if self._dma_staging and save_kv_cache and not meta.graph and not torch.cuda.is_current_stream_capturing():
@@ -388,7 +415,7 @@ class DirectKVBackend(AttentionBackend):
     def _token_layer(self, layer, forward_batch) -> int:
         """Engine registration of SGLang's token-indexed pool for this layer (page size 1 = per-token slots)."""
         lid = layer.layer_id
-        pool = forward_batch.token_to_kv_pool
+        pool = self._token_pool(forward_batch)
         k_buf, v_buf = pool.get_key_buffer(lid), pool.get_value_buffer(lid)
         eng = _TOKEN_POOL_LAYER_BASE + lid
         if self._token_registered.get(lid) != k_buf.data_ptr():
@@ -401,7 +428,7 @@ class DirectKVBackend(AttentionBackend):
         ``req_to_token[req, :seq_len]``."""
         meta = self._fwd_meta
         bs = forward_batch.batch_size
-        pool = forward_batch.token_to_kv_pool
+        pool = self._token_pool(forward_batch)
         pool.set_kv_buffer(layer, forward_batch.out_cache_loc, k, v)
         table = forward_batch.req_to_token_pool.req_to_token
         if isinstance(pool, DirectKV4BitTokenToKVPool):
@@ -420,7 +447,7 @@ class DirectKVBackend(AttentionBackend):
             return q.new_zeros(q.shape[0], nh_q * d)
         x_all = self._hidden.pop(lid, None)
         ext, pre = meta.extend_seq_lens_cpu, meta.extend_prefix_lens_cpu
-        if x_all is None or lid not in self._registered or ext is None:
+        if x_all is None or lid not in self._registered or ext is None or self._in_four_bits(forward_batch):
             return self._extend_token_pool(q, k, v, layer, forward_batch)
         # One launch sequence for the whole ragged batch (the reference calls its kernel once per request,
         # directkv/directkv_backend.py:681-697); requests without new rows take no part.
@@ -442,7 +469,7 @@ class DirectKVBackend(AttentionBackend):
         meta = self._fwd_meta
         bs = forward_batch.batch_size
         nh_q, d = self.num_q_heads, self.head_dim
-        pool = forward_batch.token_to_kv_pool
+        pool = self._token_pool(forward_batch)
         pool.set_kv_buffer(layer, forward_batch.out_cache_loc, k, v)
         four_bits = isinstance(pool, DirectKV4BitTokenToKVPool)
         eng = None if four_bits else self._token_layer(layer, forward_batch)

@@ -6,7 +6,7 @@ import types
 import pytest
 import torch
 
-from fake_sglang import EXTEND, FakeModel, make_batch, make_runner
+from fake_sglang import DECODE, EXTEND, FakeModel, make_batch, make_runner
 
 import directkv_b200
 from directkv_b200 import directkv_backend
@@ -134,3 +134,50 @@ def test_long_prompts_hold_at_most_twice_their_rows_in_bf16(monkeypatch):
     engine.calls.clear()
     _extend(be, r2t, layer, _pool(FourBits), [(1, 40, 20), (2, 50, 60), (3, 32, 0)])
     assert len(engine.calls) == 1
+
+
+def _batch(mode, lens, rids, pool, r2t, ext=None, pre=None):
+    n = sum(ext) if ext else len(lens)
+    return make_batch(mode, lens, rids, "cpu", extend_lens=ext, prefix_lens=pre, token_pool=pool, req_to_token_pool=r2t, out_cache_loc=torch.zeros(n, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("of_runner", [False, True])
+def test_a_running_model_uses_the_four_bit_pool(monkeypatch, of_runner):
+    """The modules' hooks hand over hidden states, as in a served model: the steps store to the 4-bit pool and attend it all the same, and no
+    request pool is made beside it."""
+    engine, be, r2t, layer = _setup(monkeypatch)
+    stored = []
+    pool = _pool(FourBits)
+    monkeypatch.setattr(pool, "set_kv_buffer", lambda layer, loc, k, v: stored.append(k.shape[0]), raising=False)
+    be._model_runner.token_to_kv_pool = pool if of_runner else None
+    given = None if of_runner else pool
+    fb = _batch(EXTEND, [40, 7], [1, 2], given, r2t, [40, 7], [0, 0])
+    be.init_forward_metadata(fb)
+    layer(hidden_states=torch.zeros(47, H, dtype=BF))
+    kv = torch.zeros(47, NH_KV * D, dtype=BF)
+    be.forward_extend(torch.zeros(47, NH_Q * D, dtype=BF), kv, kv, layer.attn, fb)
+    fb = _batch(DECODE, [41, 8], [1, 2], given, r2t)
+    be.init_forward_metadata(fb)
+    layer(hidden_states=torch.zeros(2, H, dtype=BF))
+    be.forward_decode(torch.zeros(2, NH_Q * D, dtype=BF), kv[:2], kv[:2], layer.attn, fb)
+    assert stored == [47, 2] and [c[0] for c in engine.calls] == ["extend", "decode_kv4", "decode_kv4"]
+    assert be._pool is None and not be._hidden and not engine.layers
+
+
+def test_graphs_over_a_four_bit_pool_keep_every_length(monkeypatch):
+    """A replayed batch has the lengths and requests it is given, one of the fill length among them, whatever the request pool knows."""
+    engine, be, r2t, layer = _setup(monkeypatch)
+    monkeypatch.setattr(directkv_backend, "get_context", lambda dev: types.SimpleNamespace(reserve=lambda *a: None))
+    pool = _pool(FourBits)
+    be._model_runner.token_to_kv_pool = pool
+    be.init_cuda_graph_state(4, 4)
+    fill = be.get_cuda_graph_seq_len_fill_value()
+    be.init_forward_metadata_capture_cuda_graph(3, 3, torch.tensor([0, 0, 0]), torch.ones(3), None, DECODE, None)
+    layer(hidden_states=torch.zeros(3, H, dtype=BF))
+    kv = torch.zeros(3, NH_KV * D, dtype=BF)
+    be.forward_decode(torch.zeros(3, NH_Q * D, dtype=BF), kv, kv, layer.attn, _batch(DECODE, [fill] * 3, [0, 0, 0], pool, r2t))
+    lens = torch.tensor([91, 5, fill])
+    be.init_forward_metadata_replay_cuda_graph(3, torch.tensor([4, 2, 6]), lens, int(lens.sum()), None, DECODE, None, seq_lens_cpu=lens)
+    assert be._fwd_meta.seq_lens_dev.tolist() == [91, 5, fill] and be._fwd_meta.req_idx_dev.tolist() == [4, 2, 6]
+    assert be._fwd_meta.seq_lens_dev.data_ptr() == be._cg_seq_lens.data_ptr() and be._fwd_meta.req_idx_dev.data_ptr() == be._cg_req.data_ptr()
+    assert be._pool is None and [c[0] for c in engine.calls] == ["decode_kv4"]

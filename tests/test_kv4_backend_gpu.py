@@ -213,3 +213,76 @@ def test_long_prompts_of_unlike_lengths_are_not_padded_to_the_longest():
             assert ((out[at + m - 9:at + m].cpu().double().view(o.shape) - o).abs() <= bound).all()
         at += m
     assert get_context(0).read_status() == 0
+
+
+@pytest.mark.parametrize("of_runner", [False, True])
+def test_a_served_model_keeps_its_cache_in_four_bits(of_runner):
+    """The attention modules run, so that their hooks hand over the hidden states: prefill, eager steps and replays of a padded graph store to
+    the 4-bit pool and attend it."""
+    be, r2t, layer, pool = _setup("device")
+    if of_runner:
+        be._model_runner.token_to_kv_pool = pool
+    g = torch.Generator().manual_seed(13)
+    ref_kv = Mirror()
+    lens = {2: 62, 4: 9, 5: 130}
+    loc = torch.cat([r2t.req_to_token[r, :n] for r, n in lens.items()])
+    n = sum(lens.values())
+    fb = make_batch(EXTEND, list(lens.values()), list(lens), DEV, extend_lens=list(lens.values()), prefix_lens=[0] * 3, token_pool=pool, req_to_token_pool=r2t,
+                    out_cache_loc=loc)
+    be.init_forward_metadata(fb)
+    q, k, v = _rows(g, n, NH_Q), _rows(g, n, NH_KV), _rows(g, n, NH_KV)
+    layer(hidden_states=torch.randn(n, H, generator=g).to(torch.bfloat16).to(DEV))
+    out = be.forward_extend(q.to(DEV), k.to(DEV), v.to(DEV), layer.attn, fb)
+    at = 0
+    for rid, m in lens.items():
+        ref_kv.add(rid, k[at:at + m], v[at:at + m])
+        ref_kv.check(rid, q[at:at + m], out[at:at + m], extend=m * (NH_Q // NH_KV) >= 128)
+        at += m
+
+    def decode(rids, run):
+        loc = torch.stack([r2t.req_to_token[r, lens[r]] for r in rids])
+        x, q, k, v = torch.randn(len(rids), H, generator=g).to(torch.bfloat16), _rows(g, len(rids), NH_Q), _rows(g, len(rids), NH_KV), _rows(g, len(rids), NH_KV)
+        for r in rids:
+            lens[r] += 1
+        out = run(rids, loc, x, q, k, v)
+        for i, r in enumerate(rids):
+            ref_kv.add(r, k[i:i + 1], v[i:i + 1])
+            ref_kv.check(r, q[i:i + 1], out[i:i + 1], extend=False)
+
+    def eager(rids, loc, x, q, k, v):
+        fb = make_batch(DECODE, [lens[r] for r in rids], rids, DEV, token_pool=pool, req_to_token_pool=r2t, out_cache_loc=loc)
+        be.init_forward_metadata(fb)
+        layer(hidden_states=x.to(DEV))
+        return be.forward_decode(q.to(DEV), k.to(DEV), v.to(DEV), layer.attn, fb)
+
+    decode([4, 2, 5], eager)
+    bs = 4
+    be.init_cuda_graph_state(bs, bs)
+    b = dict(x=torch.zeros(bs, H, dtype=torch.bfloat16, device=DEV), q=torch.zeros(bs, NH_Q * D, dtype=torch.bfloat16, device=DEV),
+             k=torch.zeros(bs, NH_KV * D, dtype=torch.bfloat16, device=DEV), v=torch.zeros(bs, NH_KV * D, dtype=torch.bfloat16, device=DEV),
+             loc=torch.zeros(bs, dtype=torch.int32, device=DEV), rid=torch.zeros(bs, dtype=torch.int64, device=DEV), lens=torch.ones(bs, dtype=torch.int64, device=DEV))
+    be.init_forward_metadata_capture_cuda_graph(bs, bs, b["rid"], b["lens"], None, DECODE, None)
+    fb = make_batch(DECODE, [1] * bs, [0] * bs, DEV, token_pool=pool, req_to_token_pool=r2t, out_cache_loc=b["loc"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer(hidden_states=b["x"])
+        out_g = be.forward_decode(b["q"], b["k"], b["v"], layer.attn, fb)
+
+    def replay(rids, loc, x, q, k, v):
+        n = len(rids)
+        for name, t in (("x", x), ("q", q), ("k", k), ("v", v), ("loc", loc)):
+            b[name][:n].copy_(t)
+        fill = be.get_cuda_graph_seq_len_fill_value()
+        here = torch.tensor([lens[r] for r in rids] + [fill] * (bs - n))
+        b["loc"][n:] = 0
+        b["rid"].copy_(torch.tensor(list(rids) + [0] * (bs - n))), b["lens"].copy_(here)
+        be.init_forward_metadata_replay_cuda_graph(bs, b["rid"], b["lens"], int(here.sum()), None, DECODE, None, seq_lens_cpu=here)
+        graph.replay()
+        torch.cuda.synchronize()
+        return out_g
+
+    for _ in range(3):                                    # request 2 reaches the fill length on the way
+        decode([4, 5, 2], replay)
+    assert lens[2] == 66 and get_context(0).read_status() == 0
+    assert (be._pool is None) == of_runner
+    graph.reset()
