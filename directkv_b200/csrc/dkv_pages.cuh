@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_kernel(const PagesParams 
                     if (pg != page) {
                         page = pg;
                         number = pg >= have ? p.free_pages[top - 1 - (cu_page[lo] + pg - have)] : line[pg];
+                        if (number < 0 || number > (0x7fffffff >> p.page_shift)) atomicOr(p.status, kStatusBadPage);   // no slot
                     }
                     if (pg >= have && (pos & (P - 1)) == 0) line[pg] = number;
                     slot[i] = number >= 0 && number <= (0x7fffffff >> p.page_shift) ? number * P + (pos & (P - 1)) : -1;

@@ -744,7 +744,8 @@ def assign_pages(
     which ``store_kv4`` and ``load_kv4`` pass over, and a position 0 (given tensors: entries that are negative there are
     left as they were).  The call takes effect as a whole or not at all: when the pages run out, a length does not fit the
     table or ``n_tokens``, or two requests with new tokens have one row, everything is left as it was, the slots are -1 and
-    the status word says why.
+    the status word says why.  A page number that gives no slot (a held page that was never entered in the table) is reported
+    there, too; its tokens have slot -1.
     """
     dev, b, a = _pages_args(page_table, lens, new_lens, "new_lens", free_pages, n_free, page_size, rows)
     if not 0 <= n_tokens < 2 ** 31:

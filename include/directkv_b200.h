@@ -440,6 +440,7 @@ int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* args, void* strea
  * -1, no token, and a position 0; entries that are negative there are left as they were); seq_lens[b] = lens[b] + more[b] (may be lens itself); cu_new [batch + 1] is the packed offset
  * of every request.  dkv_release_pages puts the pages of the tokens [more[b], lens[b]) back on the stack - in the
  * opposite order, so that a release of exactly the last assignment restores it - and leaves the table's entries.
+ * A page number on the stack or in the table that gives no slot (negative, say) gives slots of -1 and DKV_STATUS_BAD_PAGE.
  * Requests that change nothing may repeat a row.  A call takes effect as a whole or not at all: a row, length or page beyond the
  * table, two requests that change one row (DKV_STATUS_BAD_PAGE), too few free pages (DKV_STATUS_OUT_OF_PAGES) or more tokens than `capacity`, more pages than free_cap
  * (DKV_STATUS_BAD_SLOT) leave stack, table and lengths as they were, with slots -1, positions 0 and cu_new 0.

@@ -345,3 +345,18 @@ def test_a_replay_with_fewer_tokens_than_the_graph_has_room_for_changes_no_other
         assert torch.equal(got.cpu().double(), want)
         assert torch.equal(back[1].cpu().double()[:n], want[at]) and not back[1][n:].any()
     assert get_context(0).read_status() == 0
+
+
+@pytest.mark.parametrize("number", [-1, -7, 2 ** 28])
+@pytest.mark.parametrize("where", ["table", "stack"])
+def test_page_numbers_that_give_no_slot_are_reported(where, number):
+    """A slot of -1 means no token, which the store passes over in silence: a wrong page number must not look like that."""
+    rows, table, order, spare = _setup([20, 3], 16, 4, 4, 17)
+    if where == "table":
+        table[rows[0], 1] = number
+    else:
+        order[spare - 1] = number
+    got = kernel.assign_pages(table.to(DEV), _i32([20, 3]), _i32([2, 2]) if where == "table" else _i32([13, 0]), order.to(DEV), _i32([spare]), 16,
+                              4 if where == "table" else 13, rows=_i32(rows))
+    assert get_context(0).read_status() == BAD_PAGE
+    assert got[0].tolist()[:2] == [-1, -1] if where == "table" else got[0].tolist()[12] == -1 and min(got[0].tolist()[:12]) >= 0
