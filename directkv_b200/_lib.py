@@ -32,7 +32,7 @@ STATUS_BITS = {
     1 << 2: "a RoPE position was outside the cos/sin table",
     1 << 3: "the tensor-core completion barrier ran out of time",
     1 << 4: "the sequence-split exchange found a record of another step (the ranks' calls do not line up)",
-    1 << 5: "a sequence length or row led outside the page table",
+    1 << 5: "a sequence length or row led outside the page table, or a page number outside the pool",
     1 << 6: "an infinity or a not-a-number was stored to a 4-bit pool",
     1 << 7: "the stack of free pages was too short",
     1 << 8: "(in the KV-streaming kernel)",

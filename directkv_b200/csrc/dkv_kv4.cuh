@@ -19,7 +19,7 @@ namespace dkv {
 
 constexpr int kKv4CodeBytes = 64;    // per row of one head
 constexpr int kKv4ScaleBytes = 8;
-constexpr int kKv4RowThreads = 128;  // of a block that stores or loads rows (8191 tokens of 32 heads both ways: 58 us; 62 with 256, 60 with 64)
+constexpr int kKv4RowThreads = 128;  // of a block that stores or loads rows (8191 tokens of 32 heads both ways: 58.1 us; 62.0 with 256, 59.5 with 64)
 
 // Four bytes of codes to four fp16 pairs (lower dimension in the lower half).
 __device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&h)[4]) {
@@ -161,7 +161,7 @@ __device__ __forceinline__ void kv4_read16(const __nv_bfloat16* src, int wide, u
 }
 
 // A thread takes one block of 16 dimensions of K and the same one of V: 32-byte reads, 8 + 1 byte stores.  Bound by HBM: 8191
-// tokens of 32 heads stored and read back take 58 us for 344 MB (5.9 TB/s, 0.91 of the copy rate); with a division per value
+// tokens of 32 heads stored and read back take 58 to 60 us for 344 MB (5.7 to 5.9 TB/s, 0.88 to 0.91 of the copy rate); with a division per value
 // and 16-byte accesses 157 us.
 __global__ void __launch_bounds__(kKv4RowThreads) kv4_store_kernel(const Kv4RowsParams p) {
     grid_wait();

@@ -16,7 +16,7 @@
 // What bounds it is bytes, 144 per token and KV head, and close behind them the instructions that turn codes into fp16: 64
 // requests of 12000 to 20000 tokens, 32 query heads on 8, take 217 us (5.51 TB/s, 0.84 of the measured copy rate), copies
 // alone 192 us; the arithmetic needs 115 cycles per 16 tokens and SM, HBM 100.  Under sustained load the power limit
-// lowers the clock and with it this kernel (248 us).  So the loop is written for few instructions: 32 tokens
+// lowers the clock (1965 to 1762 MHz and less) and with it this kernel (243 to 260 us).  So the loop is written for few instructions: 32 tokens
 // per step with one vote on the running maximum, table entries looked up for 16 steps at a time, one multiply-add per
 // copy address.
 //
@@ -35,7 +35,7 @@ constexpr int kKv4Stages = 2;
 constexpr int kKv4HalfBytes = 2 * 1024 + 2 * 128;        // 16 tokens: K codes, V codes, K scales, V scales
 constexpr int kKv4StageBytes = 2 * kKv4HalfBytes;
 // Warps of a block and blocks per SM: 16 warps per SM with 8 columns (query fragments in registers), 12 with 16 (in shared
-// memory; 16 drafts of up to 4096 tokens: 32 us; as 16 warps that spill, at the time, 48 us against 37).
+// memory, 68 B of them spilled; 16 drafts of up to 4096 tokens: 32 us; as 16 warps, which spill more, at the time, 48 us against 37).
 template <int NT>
 constexpr int kKv4Warps = NT == 1 ? 8 : 4;
 template <int NT>

@@ -68,7 +68,7 @@ __device__ __forceinline__ void block_scan2(long long& a, long long& b, long lon
 }
 
 // Bound by latency: one scan, one search and one look-up per thread.  64 requests with one more token each and their release take
-// 8.3 us in two launches, 256 prompts of 1.0 M tokens 15 us (8 MB of slots and positions; two blocks per SM, which scan the batch
+// 8.7 us in two launches, 256 prompts of 1.0 M tokens 15 us (8 MB of slots and positions; two blocks per SM, which scan the batch
 // side by side, 17 us); the look for repeated rows is 0.3 and 0.7 us of a launch.
 template <bool RELEASE>
 __global__ void __launch_bounds__(kPagesThreads) pages_kernel(const PagesParams p) {

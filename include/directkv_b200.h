@@ -42,7 +42,7 @@ extern "C" {
 #define DKV_STATUS_BAD_POSITION  (1u << 2)
 #define DKV_STATUS_TMEM_TIMEOUT  (1u << 3)
 #define DKV_STATUS_EXCHANGE_ORDER (1u << 4)  /* dkv_decode_exchange: a record of another step arrived (calls of the ranks do not line up) */
-#define DKV_STATUS_BAD_PAGE      (1u << 5)  /* a length or row led outside the page table; the entry was not read */
+#define DKV_STATUS_BAD_PAGE      (1u << 5)  /* a length or row led outside the page table, or a page number outside the pool; what it names was not read */
 #define DKV_STATUS_NONFINITE     (1u << 6)  /* an infinity or a not-a-number was stored to a 4-bit pool (as the largest value, as zero) */
 #define DKV_STATUS_OUT_OF_PAGES  (1u << 7)  /* dkv_assign_pages: the stack of free pages was too short; nothing was assigned */
 /* Set together with a timeout bit: the kernel that gave up waiting. */
