@@ -5,7 +5,8 @@
 // top of the stack: the i-th page taken is free_pages[n_free - 1 - i].  The packed new tokens get their positions
 // a_b + j and their slots page * P + position % P.  Places behind the last new token (a captured call has room for the most
 // that it may get) hold no token: a slot there becomes -1, which store and load pass over, and a position 0; what is negative already
-// is left.  Without that a later step would store its padding rows into the slots of an earlier one.  Release puts the pages of the tokens [keep_b, len_b) back so that
+// is left.  Without that a later step would store its padding rows into the slots of an earlier one.  Release puts the pages of
+// the tokens [keep_b, len_b) back so that
 // a release of exactly what the last call took restores the stack.
 //
 // A call takes effect as a whole or not at all: too few pages, a row or length outside the table, or more tokens

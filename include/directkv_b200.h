@@ -42,7 +42,7 @@ extern "C" {
 #define DKV_STATUS_BAD_POSITION  (1u << 2)
 #define DKV_STATUS_TMEM_TIMEOUT  (1u << 3)
 #define DKV_STATUS_EXCHANGE_ORDER (1u << 4)  /* dkv_decode_exchange: a record of another step arrived (calls of the ranks do not line up) */
-#define DKV_STATUS_BAD_PAGE      (1u << 5)  /* a length or row led outside the page table, or a page number outside the pool; what it names was not read */
+#define DKV_STATUS_BAD_PAGE      (1u << 5)  /* a length or row led outside the page table, or a page outside the pool; not read */
 #define DKV_STATUS_NONFINITE     (1u << 6)  /* an infinity or a not-a-number was stored to a 4-bit pool (as the largest value, as zero) */
 #define DKV_STATUS_OUT_OF_PAGES  (1u << 7)  /* dkv_assign_pages: the stack of free pages was too short; nothing was assigned */
 /* Set together with a timeout bit: the kernel that gave up waiting. */
@@ -361,7 +361,8 @@ int dkv_kv4_pool_resolve(dkv_context* ctx, dkv_kv4_pool* pool);
 
 /* The 4-bit counterpart of dkv_scatter_kv: row i of k / v ([n_tokens, nh_kv, 128] bf16 device, k_stride / v_stride
  * elements from token to token) is quantised into slot slots[i] (int32 or int64, device).  A slot of -1 stands for no token:
- * the row is passed over.  Another slot outside the pool is not written either (DKV_STATUS_BAD_SLOT).  Two rows for one slot leave either of them or a mixture. */
+ * the row is passed over.  Another slot outside the pool is not written either (DKV_STATUS_BAD_SLOT).  Two rows for one slot
+ * leave either of them or a mixture. */
 int dkv_kv4_store(dkv_context* ctx, const dkv_kv4_pool* pool, const void* slots, int slots_int64, const void* k, int64_t k_stride,
                   const void* v, int64_t v_stride, int64_t n_tokens, void* stream);
 
@@ -437,7 +438,8 @@ int dkv_qk_norm_rope(dkv_context* ctx, const dkv_qk_norm_args* args, void* strea
  * dkv_assign_pages gives request b (row rows[b] of the table, or b) room for more[b] tokens behind its lens[b]: pages
  * come off the top of the stack in request order, then page order, and are entered in the table; slots and positions
  * [capacity] receive slot and position of every new token, packed in request order (behind the last one a slot becomes
- * -1, no token, and a position 0; entries that are negative there are left as they were); seq_lens[b] = lens[b] + more[b] (may be lens itself); cu_new [batch + 1] is the packed offset
+ * -1, no token, and a position 0; entries that are negative there are left as they were); seq_lens[b] = lens[b] + more[b]
+ * (may be lens itself); cu_new [batch + 1] is the packed offset
  * of every request.  dkv_release_pages puts the pages of the tokens [more[b], lens[b]) back on the stack - in the
  * opposite order, so that a release of exactly the last assignment restores it - and leaves the table's entries.
  * A page number on the stack or in the table that gives no slot (negative, say) gives slots of -1 and DKV_STATUS_BAD_PAGE.
